@@ -328,6 +328,84 @@ int pkv_workqueue_decode_fp8(
     int32_t dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * From a prompt to the cache, and decode over block-scaled fp8.  No counterpart in the
+ * reference, whose harness builds its metadata on the host and starts from filled pools.
+ * Token-major inputs (q, k, v, k_new, v_new) are [tokens, heads, 128] with a stride between
+ * tokens in elements (a multiple of 8, at least heads * 128), so that the column ranges of
+ * one fused projection's output need no copy; their heads lie next to one another.  Tensors
+ * are 16-byte aligned.
+ * ------------------------------------------------------------------------------- */
+
+/* The metadata of one step, from lengths on the GPU.  Row b holds cached_lens[b] tokens, and
+ * seq_lens[b] after the step (a row that shrinks takes no tokens and keeps its pages;
+ * negative lengths count as 0):
+ *   token_offsets [batch + 1]  where row b's new tokens start in packed order, and their count
+ *   block_table   [batch, max_pages]  the pages that row b needs beyond the
+ *                 ceil(cached / page_size) it has are entered, taken in row order from the
+ *                 end of the list free_pages[0, num_free); other entries stay as they are
+ *   slot_mapping  [slots]  page * page_size + offset of every new token in packed order; -1
+ *                 for tokens past the table or without a page, and behind the last token
+ *   num_free_out  [1]  num_free less the pages taken; negative when that many were missing
+ *                 (the entries concerned are -1).  It must not be num_free: the inputs
+ *                 stay as they are, and a repeated call gives the same result.
+ * num_free [1] counts as clamped to [0, free_capacity].  At most 8000 rows, and 2^31 - 1 new
+ * tokens.  Returning pages is the caller's: entries copied to the end of free_pages. */
+int pkv_build_block_tables(
+    const int32_t* cached_lens, const int32_t* seq_lens, const int32_t* free_pages,
+    const int32_t* num_free, int32_t* block_table, int32_t* token_offsets, int32_t* slot_mapping,
+    int32_t* num_free_out, int32_t batch, int32_t free_capacity, int32_t max_pages, int32_t slots,
+    int32_t page_size, void* stream);
+
+/* Causal attention over whole prompts: sequence b is the tokens [token_offsets[b],
+ * token_offsets[b + 1]) of q [tokens, num_q_heads, 128] and of k, v [tokens, num_kv_heads,
+ * 128]; its token i attends to its tokens 0 ... i.  output [tokens, num_q_heads, 128],
+ * contiguous; rows outside every sequence are left as they are.  Offsets must not decrease and
+ * count as clamped to [0, tokens].  G = num_q_heads / num_kv_heads in [1, 32]. */
+int pkv_prefill_attention(
+    const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+    int64_t v_stride, const int32_t* token_offsets, void* output, int32_t batch, int32_t tokens,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype, void* stream);
+
+/* Writes k_new[t] and v_new[t] ([num_kv_heads, 128], dtype f16 or bf16) to slot
+ * slot_mapping[t] (page * page_size + offset) of the pools [num_pages, num_kv_heads,
+ * page_size, 128] of the same dtype.  Slots outside the pools are skipped; a slot may occur
+ * only once in a call. */
+int pkv_write_kv(const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride,
+                 void* k_pages, void* v_pages, const int32_t* slot_mapping, int32_t tokens,
+                 int32_t num_kv_heads, int32_t head_dim, int32_t num_pages, int32_t page_size,
+                 int32_t dtype, void* stream);
+
+/* pkv_write_kv into fp8 (OCP e4m3) pools with kv_scales [num_pages, num_kv_heads, 2] (K's
+ * scale, V's scale; 8-byte aligned).  Scales are powers of two in [2^-60, 2^60], the smallest
+ * with amax <= 448 scale over the finite values the block receives; elements are stored as
+ * e4m3(clamp(x / scale, -448, 448)), rounded to nearest even, NaN as NaN.  A page whose first
+ * written offset is 0 starts anew.  Otherwise the tokens before it stay: the scale is at
+ * least the old one (rounded up to a power of two), and where it grows, those tokens are
+ * stored again under it (exact but for subnormals).  The tokens of one page must follow one
+ * another in slot_mapping in ascending slots, and a slot may occur only once in a call; a
+ * call that breaks this leaves the pages concerned with unspecified values. */
+int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_new,
+                           int64_t v_stride, void* k_pages, void* v_pages, float* kv_scales,
+                           const int32_t* slot_mapping, int32_t tokens, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t num_pages, int32_t page_size, int32_t dtype,
+                           void* stream);
+
+/* pkv_paged_attention_masked over such pools: K = kv_scales[p, h, 0] * k8 and
+ * V = kv_scales[p, h, 1] * v8 for every page p and KV head h.  Scales count as clamped to
+ * [2^-60, 2^60] (NaN as the lower end) and need not be powers of two.  page_size must be a
+ * multiple of 16; rows of length 0 give zeros; lengths are clamped to the table, page ids
+ * into the pool.  At most 16000 rows.  The workspace is required:
+ * pkv_fp8_block_workspace_bytes on the same device, for any lengths; it holds nothing
+ * between calls. */
+int pkv_paged_attention_fp8_block(
+    const void* q, const void* k_pages, const void* v_pages, const float* kv_scales,
+    const int32_t* block_table, const int32_t* seq_lens, void* output, void* workspace,
+    size_t workspace_size, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t num_pages, int32_t page_size, int32_t max_pages, int32_t dtype,
+    void* stream);
+size_t pkv_fp8_block_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads);
+
+/* ---------------------------------------------------------------------------------
  * Contiguous-layout decode: K and V are [batch, num_kv_heads, context, 128] (every row
  * holds `context` tokens) and q / output are [batch, num_q_heads, 128].
  * ------------------------------------------------------------------------------- */

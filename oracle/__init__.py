@@ -27,6 +27,12 @@ Modules and what pins each function (the tests named here hold the checks):
     split_offsets is the prefix sum of the row split counts including empty splits,
     rows are padded with the last reserved page).
 
+``prompt`` (tests/test_oracle_prompt.py)
+  * block tables and slots, causal attention over packed prompts, packed K/V writes and
+    block-scaled fp8 pools, in plain loops and 64 bits — pinned by hand-worked answers,
+    by ``attention_fp64`` (the last token of a prompt is a decode step) and by torch's
+    float8_e4m3fn cast.
+
 ``native`` (tests/test_oracle_native.py)
   * C restatement of the reference kernel's fp32 arithmetic and of
     ``tests/smoke_test.cu``'s CPU reference and glibc inputs; pinned against the fp64

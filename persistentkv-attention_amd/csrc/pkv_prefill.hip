@@ -1,0 +1,385 @@
+// pkv_prefill.hip — causal GQA attention over whole prompts, packed one after another
+// (the reference has decode only; its harness starts from a filled pool,
+// tests/benchmark_serving_trace.py:285-298).
+//
+//   o[i] = sum_{j <= i} p_ij v[j],  p_ij = exp(q[i] k[j] / sqrt(128) - m_i) / l_i
+//
+// Rows of work.  The G query heads of a KV head are rows of one matrix product over the same K
+// and V: row r of a (sequence, KV head) is token r / G, head kvh * G + r % G.  A workgroup of
+// eight waves owns 256 consecutive rows (for G = 4: 64 tokens), a wave 32 of them, so K/V
+// tiles are read from L2 once for all heads of the group, any G is served by one kernel, and
+// the masked part of a diagonal tile covers few tokens.
+//
+// Per wave and tile of 64 keys, with v_mfma_f32_32x32x16:
+//   S^T[key, row] = K Q^T   K from LDS as the A operand, Q in registers as the B operand.
+//   A lane then holds 32 keys of ONE row: maximum and sum of the softmax are lane-local but
+//   for one exchange between the wave's halves.
+//   O^T[dim, row] += V^T P^T   P^T's B operand is S^T's own register layout, packed to 16 bits
+//   (the k order of a product is free as long as both operands agree), V^T's A operand comes
+//   from row-major V in LDS through the transposing reads (ds_read_b64_tr_b16).
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "pkv.h"
+
+namespace pkv {
+int fail(int status, const char* fmt, ...);  // pkv_decode.hip: sets pkv_last_error()
+int ok();
+}  // namespace pkv
+
+namespace {
+
+constexpr int kD = 128;
+constexpr int kRowBytes = 2 * kD;
+constexpr int kKeys = 64;    // keys per tile
+constexpr int kWaves = 8;
+constexpr int kWaveRows = 32;
+constexpr int kRows = kWaves * kWaveRows;
+constexpr int kTileBytes = kKeys * kRowBytes;
+constexpr uint32_t kRsrcWord3 = 0x00020000u;  // raw buffer, 32-bit data format (gfx9 family)
+constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
+// The running maximum is replaced only when a score passes it by more than 2^8 in weight:
+// the output is rescaled in few tiles, and weights stay below 2^8, far inside fp16's range.
+constexpr float kSlack = 8.0f / kScaleLog2;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+struct Half {
+  static constexpr uint32_t kExponentStep = 0x04000400u;  // one step of both halves' exponents
+  static constexpr uint32_t kOne = 0x3c00u;
+  __device__ static inline f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  __device__ static inline uint32_t pack2(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+  }
+};
+struct BFloat {
+  static constexpr uint32_t kExponentStep = 0x00800080u;
+  static constexpr uint32_t kOne = 0x3f80u;
+  __device__ static inline f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  __device__ static inline uint32_t pack2(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+  }
+};
+
+struct PrefillArgs {
+  const uint8_t* q;  // token t, head h at q + t * q_stride + h * 256 (bytes)
+  const uint8_t* k;
+  const uint8_t* v;
+  const int32_t* token_offsets;  // [B + 1]
+  uint8_t* output;               // [T, Hq, 128]
+  long q_stride, k_stride, v_stride;
+  int32_t batch, tokens, hq, hkv, group;
+};
+
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline void* uniform_ptr(const void* p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t lo = (uint32_t)uniform((int)(uint32_t)v), hi = (uint32_t)uniform((int)(v >> 32));
+  return (void*)(((uint64_t)hi << 32) | lo);
+}
+
+__device__ inline int offset_of(const PrefillArgs& a, int b) {
+  return min(max(a.token_offsets[b], 0), a.tokens);
+}
+// First workgroup slot of sequence b.  Its rows start at row offset x = offset * G; the slots
+// from x / 256 + b on, up to the next sequence's, are at least as many as its 256-row blocks.
+__device__ inline int first_slot(const PrefillArgs& a, int b) {
+  return (int)((uint32_t)(offset_of(a, b) * a.group) / kRows) + b;
+}
+
+// Two rows of K and of V of a tile in a thread's registers, on their way to LDS.
+struct Stage {
+  u32x4 k[2], v[2];
+};
+
+// The top bits of those halves of a pair of 16-bit floats that are infinite or NaN.
+template <class Elem>
+__device__ inline uint32_t nonfinite_halves(uint32_t x2) {
+  return ((x2 & 0x7fff7fffu) + Elem::kExponentStep) & 0x80008000u;
+}
+template <class Elem>
+__device__ inline uint32_t drop_nonfinite(uint32_t x2) {
+  const uint32_t y = nonfinite_halves<Elem>(x2);
+  return x2 & ~((y >> 15) * 0xffffu);
+}
+// 1 in the halves that are +inf (x) or -inf (y), in both for NaN; 0 elsewhere.
+template <class Elem>
+__device__ inline uint2 infinities(uint32_t x2) {
+  const uint32_t bad = nonfinite_halves<Elem>(x2);
+  const uint32_t nan = (x2 & 0x7fff7fffu) + (Elem::kExponentStep - 0x00010001u);  // top bits
+  return uint2{((bad & (~x2 | nan)) >> 15) * Elem::kOne, ((bad & (x2 | nan)) >> 15) * Elem::kOne};
+}
+
+template <class Elem>
+__global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][kTileBytes];  // [buffer][K, V]
+  __shared__ int nonfinite[2];  // [buffer] 1 + the last tile whose V held an infinity or NaN
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = lane & 31, half = lane >> 5;
+  const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
+  const int slot = uniform((int)(blockIdx.x / (unsigned)a.hkv));
+  int b = 0;
+  for (int n = a.batch; n > 1;) {  // the last sequence whose first slot is at most `slot`
+    const int mid = n >> 1;
+    if (first_slot(a, b + mid) <= slot) b += mid, n -= mid;
+    else n = mid;
+  }
+  const int start = uniform(offset_of(a, b));
+  const int len = uniform(max(offset_of(a, b + 1) - start, 0));
+  const int rows = len * a.group;
+  const int blocks = (rows + kRows - 1) / kRows;
+  const int block = blocks - 1 - (slot - first_slot(a, b));  // the longest first
+  if (block < 0 || block >= blocks) return;  // a slot that no block of a sequence takes
+
+  const int row0 = block * kRows + wave * kWaveRows;
+  const int row = min(row0 + col, rows - 1);
+  const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+  const int wave_first = uniform(min(row0, rows - 1) / a.group);
+  const int wave_last = uniform(min(row0 + kWaveRows - 1, rows - 1) / a.group);
+  const int first = uniform(block * kRows / a.group);  // the workgroup's first and last tokens
+  const int last = uniform(min(block * kRows + kRows - 1, rows - 1) / a.group);
+  const int tiles = last / kKeys + 1;
+
+  u32x4 q[8];
+  const uint8_t* qp = a.q + (start + (long)tok) * a.q_stride + (long)head * kRowBytes + half * 16;
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) q[kk] = *(const u32x4*)(qp + kk * 32);
+
+  // Staging: thread t moves 16-byte chunk t % 16 of rows t / 16 and t / 16 + 32.  Chunks are
+  // stored under an exclusive or with the row, so that reads of one chunk column (K) or of 64
+  // bytes of four rows (V) spread over all banks.
+  const int srow = tid >> 4, chunk = tid & 15;
+  const uint32_t kdst = srow * kRowBytes + ((chunk ^ (srow & 15)) << 4);
+  const uint32_t vdst = srow * kRowBytes + ((chunk ^ ((srow & 3) << 2)) << 4);
+  const uint8_t* kbase = a.k + (long)start * a.k_stride + (long)kvh * kRowBytes;
+  const uint8_t* vbase = a.v + (long)start * a.v_stride + (long)kvh * kRowBytes;
+  const uint32_t koff = (uint32_t)(srow * (int)a.k_stride + chunk * 16);
+  const uint32_t voff = (uint32_t)(srow * (int)a.v_stride + chunk * 16);
+  auto fetch = [&](int tile, Stage& r) {
+    // Rows past the sequence's end read as zero: the descriptor ends with its last row.
+    const int n = min(kKeys, len - tile * kKeys);
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+        uniform_ptr(kbase + (long)tile * kKeys * a.k_stride), (short)0,
+        uniform((n - 1) * (int)a.k_stride + kRowBytes), kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+        uniform_ptr(vbase + (long)tile * kKeys * a.v_stride), (short)0,
+        uniform((n - 1) * (int)a.v_stride + kRowBytes), kRsrcWord3);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r.k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff + i * 32 * (uint32_t)a.k_stride, 0, 0));
+      r.v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff + i * 32 * (uint32_t)a.v_stride, 0, 0));
+    }
+  };
+  // A masked weight is 0, and 0 times an infinity or NaN in V is NaN: tiles that some row of
+  // the workgroup masks in part are looked over on their way, and take another path below
+  // where V is not finite.  Such values then reach the rows from their token on, and no other.
+  auto store = [&](int tile, const Stage& r) {
+    const int buf = tile & 1;
+    if ((tile + 1) * kKeys - 1 > first) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= nonfinite_halves<Elem>(r.v[i][j]);
+      if (bad) nonfinite[buf] = tile + 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *(u32x4*)(&lds[buf][0][kdst + i * 32 * kRowBytes]) = r.k[i];
+      *(u32x4*)(&lds[buf][1][vdst + i * 32 * kRowBytes]) = r.v[i];
+    }
+  };
+  // Reads: lane's K row (key col), chunk 2 kk + half; V rows 4 half + (lane % 16) / 4, four
+  // dims from 32 db + 16 (lane / 16 % 2) + 4 (lane % 4) on.
+  const uint32_t ksrc = col * kRowBytes + ((half ^ (col & 15)) << 4);
+  const int vr = (lane >> 2) & 3;
+  const uint32_t vsrc = (4 * half + vr) * kRowBytes + (vr << 6) + ((lane & 16) << 1) + ((lane & 3) << 3);
+
+  f32x16 o[4] = {};
+  float m = -INFINITY, l = 0.f;
+
+  Stage r;
+  if (tid < 2) nonfinite[tid] = 0;
+  __syncthreads();
+  fetch(0, r);
+  store(0, r);
+  __syncthreads();
+  for (int tile = 0; tile < tiles; ++tile) {
+    const int buf = tile & 1;
+    if (tile + 1 < tiles) fetch(tile + 1, r);
+    const int k0 = tile * kKeys;
+    if (k0 <= wave_last) {
+      const uint8_t* const kt = lds[buf][0];
+      const uint8_t* const vt = lds[buf][1];
+      f32x16 s[2] = {};
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          s[kb] = Elem::mma(*(const u32x4*)(kt + (ksrc ^ (kk << 5)) + kb * 32 * kRowBytes), q[kk], s[kb]);
+      const bool diagonal = k0 + kKeys - 1 > wave_first;
+      if (diagonal) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (k0 + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) > tok) s[kb][i] = -INFINITY;
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float mn = fmaxf(m, mx);
+        const float c = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2);
+        m = mn;
+        l *= c;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[db][i] *= c;
+      }
+      const float ms = m * kScaleLog2;
+      u32x4 p[4];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], kScaleLog2, -ms));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], kScaleLog2, -ms));
+          l += p0 + p1;
+          p[2 * kb + (i >> 3)][(i & 7) >> 1] = Elem::pack2(p0, p1);
+        }
+      auto value = [&](int c, int db) {  // V^T's operand: 16 keys from 16 c on, dims 32 db + lane % 32
+        typedef __attribute__((address_space(3))) s16x4* Lds;
+        const uint8_t* at = vt + (vsrc ^ (db << 6)) + c * 16 * kRowBytes;
+        const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at));
+        const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 8 * kRowBytes)));
+        return u32x4{v0[0], v0[1], v1[0], v1[1]};
+      };
+      auto pv = [&](auto clean) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int db = 0; db < 4; ++db) {
+            if constexpr (decltype(clean)::value) __builtin_amdgcn_sched_barrier(0);
+            u32x4 x = value(c, db);
+            if constexpr (decltype(clean)::value) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = drop_nonfinite<Elem>(x[i]);
+            }
+            o[db] = Elem::mma(x, p[c], o[db]);
+          }
+      };
+      if (diagonal && uniform(nonfinite[buf]) == tile + 1) {
+        pv(std::true_type{});
+        // How many +inf and -inf (a NaN is both) each row sees in each dim, as products too.
+        u32x4 see[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = k0 + 16 * c + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
+            see[c][i] = (key <= tok ? Elem::kOne : 0u) | (key + 1 <= tok ? Elem::kOne << 16 : 0u);
+          }
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          f32x16 up = {}, down = {};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
+            const u32x4 x = value(c, db);
+            u32x4 xu, xd;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint2 n = infinities<Elem>(x[i]);
+              xu[i] = n.x, xd[i] = n.y;
+            }
+            up = Elem::mma(xu, see[c], up);
+            down = Elem::mma(xd, see[c], down);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            o[db][i] += (up[i] > 0.f ? INFINITY : 0.f) + (down[i] > 0.f ? -INFINITY : 0.f);
+        }
+      } else {
+        pv(std::false_type{});
+      }
+    }
+    if (tile + 1 < tiles) store(tile + 1, r);
+    __syncthreads();
+  }
+
+  if (row0 + col >= rows) return;
+  const float inv = 1.0f / (l + __shfl_xor(l, 32));
+  uint8_t* out = a.output + ((start + (long)tok) * a.hq + head) * kRowBytes + half * 8;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *(u32x2*)(out + db * 64 + i * 4) = u32x2{Elem::pack2(o[db][i] * inv, o[db][i + 1] * inv),
+                                               Elem::pack2(o[db][i + 2] * inv, o[db][i + 3] * inv)};
+}
+
+}  // namespace
+
+extern "C" int pkv_prefill_attention(
+    const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+    int64_t v_stride, const int32_t* token_offsets, void* output, int32_t batch, int32_t tokens,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype, void* stream) {
+  using pkv::fail;
+  if (batch < 0 || tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: batch %d, tokens %d, num_q_heads %d, num_kv_heads %d",
+                batch, tokens, num_q_heads, num_kv_heads);
+  if (head_dim != kD) return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: head_dim %d (only 128)", head_dim);
+  if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16)
+    return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: unknown dtype %d", dtype);
+  if (num_q_heads % num_kv_heads)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: Hq must be divisible by Hkv");
+  const int32_t group = num_q_heads / num_kv_heads;
+  if (group > PKV_MAX_GROUP)
+    return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: G=Hq/Hkv %d (at most %d)", group, PKV_MAX_GROUP);
+  if (q_stride < (int64_t)num_q_heads * kD || k_stride < (int64_t)num_kv_heads * kD ||
+      v_stride < (int64_t)num_kv_heads * kD || (q_stride | k_stride | v_stride) % 8)
+    return fail(PKV_ERR_INVALID_ARGUMENT,
+                "prefill_attention: a token stride must hold its heads and be a multiple of 8 elements");
+  if (k_stride > (1 << 23) || v_stride > (1 << 23))  // a tile's rows lie within 2 GiB
+    return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: token strides of K and V up to 2^23 elements");
+  const int64_t slots = (int64_t)tokens * group / kRows + batch;
+  if ((int64_t)tokens * group > INT32_MAX || slots * num_kv_heads > INT32_MAX)
+    return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: too many tokens");
+  if (batch == 0 || tokens == 0) return pkv::ok();
+  if (!q || !k || !v || !token_offsets || !output)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: null pointer");
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)output) & 15)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: tensors must be 16-byte aligned");
+  const PrefillArgs a{(const uint8_t*)q, (const uint8_t*)k, (const uint8_t*)v, token_offsets,
+                      (uint8_t*)output, 2 * q_stride, 2 * k_stride, 2 * v_stride,
+                      batch, tokens, num_q_heads, num_kv_heads, group};
+  const dim3 grid((unsigned)(slots * num_kv_heads)), threads(kWaves * 64);
+  if (dtype == PKV_DTYPE_BF16) prefill_kernel<BFloat><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+  else prefill_kernel<Half><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? pkv::ok()
+                         : fail(PKV_ERR_LAUNCH, "prefill_attention launch: %s", hipGetErrorString(e));
+}

@@ -10,7 +10,9 @@
 // variants of the indexed and work-queue ops, the contiguous-layout decode and
 // query-head baseline of its C++ API (cuh:1077-1108, :1263-1282), and the KV-cache append
 // (fp16 / bf16 / fp8 pools) that a serving loop runs before each decode step, alone or
-// fused into the indexed and work-queue ops (*_append).
+// fused into the indexed and work-queue ops (*_append); and the way from a prompt to the
+// cache: block tables and slots from lengths on the GPU, causal attention over packed
+// prompts, packed K/V writes, and decode over fp8 pools with a scale per (page, head).
 // Work is enqueued on the current HIP stream of the tensors' device without a host sync,
 // so the ops can be captured in HIP graphs.
 
@@ -722,6 +724,191 @@ int64_t persistentkv_split_workspace_floats(int64_t batch, int64_t num_q_heads, 
                    sizeof(float));
 }
 
+namespace {
+
+// Tensors of one op must share a device: the kernels run on the first one's.
+void check_device(const torch::Tensor& t, const char* name, const torch::Tensor& first) {
+  TORCH_CHECK(t.device() == first.device(), name, " is on ", t.device(), ", not on ", first.device());
+}
+
+// [tokens, heads, 128] whose heads lie next to one another; any stride between tokens.
+void check_packed(const torch::Tensor& t, const char* name, at::ScalarType dtype) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == dtype, name, " has wrong dtype");
+  TORCH_CHECK(t.dim() == 3, name, " has wrong rank");
+  TORCH_CHECK(t.size(2) == PKV_HEAD_DIM, "PersistentKV extension currently requires d=128");
+  TORCH_CHECK(t.numel() == 0 || (t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == PKV_HEAD_DIM)),
+              name, " must have contiguous heads");
+}
+int64_t token_stride(const torch::Tensor& t) {
+  return t.size(0) > 1 ? t.stride(0) : t.size(1) * PKV_HEAD_DIM;  // of no meaning for one token
+}
+
+}  // namespace
+
+void persistentkv_build_block_tables(torch::Tensor cached_lens, torch::Tensor seq_lens,
+                                     torch::Tensor free_pages, torch::Tensor num_free,
+                                     torch::Tensor block_table, torch::Tensor token_offsets,
+                                     torch::Tensor slot_mapping, torch::Tensor num_free_out,
+                                     int64_t page_size) {
+  check_tensor(cached_lens, "cached_lens", at::kInt, 1);
+  check_tensor(seq_lens, "seq_lens", at::kInt, 1);
+  check_tensor(free_pages, "free_pages", at::kInt, 1);
+  check_tensor(num_free, "num_free", at::kInt, 1);
+  check_tensor(block_table, "block_table", at::kInt, 2);
+  check_tensor(token_offsets, "token_offsets", at::kInt, 1);
+  check_tensor(slot_mapping, "slot_mapping", at::kInt, 1);
+  check_tensor(num_free_out, "num_free_out", at::kInt, 1);
+  check_device(seq_lens, "seq_lens", cached_lens);
+  check_device(free_pages, "free_pages", cached_lens);
+  check_device(num_free, "num_free", cached_lens);
+  check_device(block_table, "block_table", cached_lens);
+  check_device(token_offsets, "token_offsets", cached_lens);
+  check_device(slot_mapping, "slot_mapping", cached_lens);
+  check_device(num_free_out, "num_free_out", cached_lens);
+  const int64_t B = cached_lens.size(0);
+  TORCH_CHECK(seq_lens.size(0) == B, "seq_lens batch mismatch");
+  TORCH_CHECK(block_table.size(0) == B, "block_table batch mismatch");
+  TORCH_CHECK(token_offsets.size(0) == B + 1, "token_offsets must have batch + 1 elements");
+  TORCH_CHECK(num_free.size(0) == 1 && num_free_out.size(0) == 1, "num_free must have one element");
+  TORCH_CHECK(num_free.data_ptr() != num_free_out.data_ptr(), "num_free_out must not be num_free");
+  TORCH_CHECK(page_size > 0, "page_size must be positive");
+  const c10::DeviceGuard guard(cached_lens.device());
+  raise_on(pkv_build_block_tables(
+      cached_lens.data_ptr<int>(), seq_lens.data_ptr<int>(), free_pages.data_ptr<int>(),
+      num_free.data_ptr<int>(), block_table.data_ptr<int>(), token_offsets.data_ptr<int>(),
+      slot_mapping.data_ptr<int>(), num_free_out.data_ptr<int>(), i32(B, "batch"),
+      i32(free_pages.size(0), "free_pages.size(0)"), i32(block_table.size(1), "block_table.size(1)"),
+      i32(slot_mapping.size(0), "slot_mapping.size(0)"), i32(page_size, "page_size"),
+      stream_of(cached_lens)));
+}
+
+void persistentkv_prefill_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                    torch::Tensor token_offsets, torch::Tensor output) {
+  const auto dt = activation_dtype(q, "q");
+  check_packed(q, "q", dt);
+  check_packed(k, "k", dt);
+  check_packed(v, "v", dt);
+  check_tensor(token_offsets, "token_offsets", at::kInt, 1);
+  check_tensor(output, "output", dt, 3);
+  check_device(k, "k", q);
+  check_device(v, "v", q);
+  check_device(token_offsets, "token_offsets", q);
+  check_device(output, "output", q);
+  TORCH_CHECK(k.size(0) == q.size(0), "k tokens mismatch");
+  TORCH_CHECK(v.sizes() == k.sizes(), "v shape mismatch");
+  TORCH_CHECK(output.sizes() == q.sizes(), "output shape must match q");
+  TORCH_CHECK(token_offsets.size(0) > 0, "token_offsets must have batch + 1 elements");
+  const int32_t Hq = i32(q.size(1), "q.size(1)"), Hkv = i32(k.size(1), "k.size(1)");
+  check_supported_gqa(Hq, Hkv);
+  const c10::DeviceGuard guard(q.device());
+  raise_on(pkv_prefill_attention(
+      q.data_ptr(), token_stride(q), k.data_ptr(), token_stride(k), v.data_ptr(), token_stride(v),
+      token_offsets.data_ptr<int>(), output.data_ptr(), i32(token_offsets.size(0) - 1, "batch"),
+      i32(q.size(0), "q.size(0)"), Hq, Hkv, PKV_HEAD_DIM, pkv_dtype_of(dt), stream_of(q)));
+}
+
+namespace {
+
+// write_kv (kv_scales null) and write_kv_fp8_block.
+void write_op(const torch::Tensor& k_new, const torch::Tensor& v_new, torch::Tensor& k_pages,
+              torch::Tensor& v_pages, const torch::Tensor& slot_mapping, torch::Tensor* kv_scales) {
+  const auto dt = activation_dtype(k_new, "k_new");
+  const auto kv_dt = kv_scales ? at::kFloat8_e4m3fn : dt;
+  check_packed(k_new, "k_new", dt);
+  check_packed(v_new, "v_new", dt);
+  check_tensor(k_pages, "k_pages", kv_dt, 4);
+  check_tensor(v_pages, "v_pages", kv_dt, 4);
+  check_tensor(slot_mapping, "slot_mapping", at::kInt, 1);
+  check_device(k_new, "k_new", k_pages);
+  check_device(v_new, "v_new", k_pages);
+  check_device(v_pages, "v_pages", k_pages);
+  check_device(slot_mapping, "slot_mapping", k_pages);
+  const int64_t T = k_new.size(0), Hkv = k_new.size(1);
+  TORCH_CHECK(v_new.sizes() == k_new.sizes(), "v_new shape mismatch");
+  TORCH_CHECK(k_pages.size(1) == Hkv, "k_pages Hkv mismatch");
+  check_pages(k_pages, v_pages, k_pages.size(2), PKV_HEAD_DIM);
+  TORCH_CHECK(slot_mapping.size(0) == T, "slot_mapping must have one slot a token");
+  const int32_t tokens = i32(T, "k_new.size(0)"), hkv = i32(Hkv, "Hkv");
+  const int32_t pages = i32(k_pages.size(0), "k_pages.size(0)"), ps = i32(k_pages.size(2), "page_size");
+  if (kv_scales) {
+    check_tensor(*kv_scales, "kv_scales", at::kFloat, 3);
+    check_device(*kv_scales, "kv_scales", k_pages);
+    TORCH_CHECK(kv_scales->size(0) == pages && kv_scales->size(1) == Hkv && kv_scales->size(2) == 2,
+                "kv_scales must have shape [num_pages, Hkv, 2]");
+  }
+  const c10::DeviceGuard guard(k_pages.device());
+  raise_on(kv_scales
+               ? pkv_write_kv_fp8_block(k_new.data_ptr(), token_stride(k_new), v_new.data_ptr(),
+                                        token_stride(v_new), k_pages.data_ptr(), v_pages.data_ptr(),
+                                        kv_scales->data_ptr<float>(), slot_mapping.data_ptr<int>(),
+                                        tokens, hkv, PKV_HEAD_DIM, pages, ps, pkv_dtype_of(dt),
+                                        stream_of(k_pages))
+               : pkv_write_kv(k_new.data_ptr(), token_stride(k_new), v_new.data_ptr(),
+                              token_stride(v_new), k_pages.data_ptr(), v_pages.data_ptr(),
+                              slot_mapping.data_ptr<int>(), tokens, hkv, PKV_HEAD_DIM, pages, ps,
+                              pkv_dtype_of(dt), stream_of(k_pages)));
+}
+
+}  // namespace
+
+void persistentkv_write_kv(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor k_pages,
+                           torch::Tensor v_pages, torch::Tensor slot_mapping) {
+  write_op(k_new, v_new, k_pages, v_pages, slot_mapping, nullptr);
+}
+
+void persistentkv_write_kv_fp8_block(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor k_pages,
+                                     torch::Tensor v_pages, torch::Tensor kv_scales,
+                                     torch::Tensor slot_mapping) {
+  write_op(k_new, v_new, k_pages, v_pages, slot_mapping, &kv_scales);
+}
+
+void persistentkv_paged_attention_fp8_block(torch::Tensor q, torch::Tensor k_pages,
+                                            torch::Tensor v_pages, torch::Tensor kv_scales,
+                                            torch::Tensor block_table, torch::Tensor seq_lens,
+                                            torch::Tensor output, torch::Tensor workspace,
+                                            int64_t page_size) {
+  const auto dt = activation_dtype(q, "q");
+  check_tensor(q, "q", dt, 3);
+  check_tensor(k_pages, "k_pages", at::kFloat8_e4m3fn, 4);
+  check_tensor(v_pages, "v_pages", at::kFloat8_e4m3fn, 4);
+  check_tensor(kv_scales, "kv_scales", at::kFloat, 3);
+  check_tensor(block_table, "block_table", at::kInt, 2);
+  check_tensor(seq_lens, "seq_lens", at::kInt, 1);
+  check_tensor(output, "output", dt, 3);
+  check_workspace(workspace);
+  check_device(k_pages, "k_pages", q);
+  check_device(v_pages, "v_pages", q);
+  check_device(kv_scales, "kv_scales", q);
+  check_device(block_table, "block_table", q);
+  check_device(seq_lens, "seq_lens", q);
+  check_device(output, "output", q);
+  check_device(workspace, "workspace", q);
+  const int64_t B = q.size(0), Hq = q.size(1), d = q.size(2), Hkv = k_pages.size(1);
+  TORCH_CHECK(d == PKV_HEAD_DIM, "PersistentKV extension currently requires d=128");
+  TORCH_CHECK(output.sizes() == q.sizes(), "output shape must match q");
+  TORCH_CHECK(seq_lens.size(0) == B, "seq_lens batch mismatch");
+  TORCH_CHECK(block_table.size(0) == B, "block_table batch mismatch");
+  TORCH_CHECK(page_size > 0, "page_size must be positive");
+  check_pages(k_pages, v_pages, page_size, PKV_HEAD_DIM);
+  TORCH_CHECK(kv_scales.size(0) == k_pages.size(0) && kv_scales.size(1) == Hkv && kv_scales.size(2) == 2,
+              "kv_scales must have shape [num_pages, Hkv, 2]");
+  check_supported_gqa(i32(Hq, "q.size(1)"), i32(Hkv, "k_pages.size(1)"));
+  const c10::DeviceGuard guard(q.device());
+  raise_on(pkv_paged_attention_fp8_block(
+      q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), kv_scales.data_ptr<float>(),
+      block_table.data_ptr<int>(), seq_lens.data_ptr<int>(), output.data_ptr(), ws_ptr(workspace),
+      ws_bytes(workspace), i32(B, "batch"), (int32_t)Hq, (int32_t)Hkv, PKV_HEAD_DIM,
+      i32(k_pages.size(0), "k_pages.size(0)"), i32(page_size, "page_size"),
+      i32(block_table.size(1), "block_table.size(1)"), pkv_dtype_of(dt), stream_of(q)));
+}
+
+int64_t persistentkv_fp8_block_workspace_floats(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads) {
+  return (int64_t)(pkv_fp8_block_workspace_bytes(i32(batch, "batch"), i32(num_q_heads, "Hq"),
+                                                 i32(num_kv_heads, "Hkv")) /
+                   sizeof(float));
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention_workqueue_stage", &persistentkv_paged_attention_workqueue_stage,
         "one stage (1 decode, 2 merge) of paged_attention_workqueue in the schedule it takes");
@@ -769,6 +956,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "write each row's newest token's K/V into its tail page (position seq_lens - 1)");
   m.def("append_kv_fp8", &persistentkv_append_kv_fp8,
         "append_kv into float8_e4m3fn pools, quantising x / scale with round-to-nearest-even");
+  m.def("build_block_tables", &persistentkv_build_block_tables,
+        "block-table entries, token offsets and slots of a step's new tokens, from lengths and "
+        "a list of free pages on the GPU");
+  m.def("prefill_attention", &persistentkv_prefill_attention,
+        "causal GQA attention over packed prompts [tokens, H, 128]");
+  m.def("write_kv", &persistentkv_write_kv, "write packed K/V tokens into the page pools by slot");
+  m.def("write_kv_fp8_block", &persistentkv_write_kv_fp8_block,
+        "write_kv into float8_e4m3fn pools with one scale per (page, KV head), K and V apart");
+  m.def("paged_attention_fp8_block", &persistentkv_paged_attention_fp8_block,
+        "paged decode attention over float8_e4m3fn pools with one scale per (page, KV head)");
+  m.def("fp8_block_workspace_floats", &persistentkv_fp8_block_workspace_floats,
+        "fp32 workspace elements of paged_attention_fp8_block on the current device");
   m.def("attention_query_head_baseline", &persistentkv_attention_query_head_baseline,
         "Query-head baseline over contiguous K/V (each query head streams its KV head)");
 }

@@ -1,0 +1,272 @@
+// pkv_write.hip — writes packed K/V tokens (a batch of prompts, or one token a row) into the
+// page pools, each token to a slot (page * page_size + offset): a copy into fp16 / bf16 pools,
+// or a quantisation to fp8 (OCP e4m3) with one scale per (page, KV head), K and V apart.
+// The reference never writes K/V (tests/benchmark_serving_trace.py:285-298).
+//
+// Block scales are powers of two in [2^-60, 2^60], the smallest with amax <= 448 scale over the
+// finite values of the block.  A power of two makes x / scale exact, and growing a scale later
+// (a token with a larger magnitude joins a part-filled page) leaves every stored value as it is
+// but those that become subnormal, which round once; an arbitrary scale would round every value
+// of the page again at each growth.  It costs nothing in precision: e4m3 is a floating format.
+//
+// Tokens outside the pools (slot < 0 or past the last page) are skipped.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "pkv.h"
+#include "pkv_e4m3.h"
+
+namespace pkv {
+int fail(int status, const char* fmt, ...);  // pkv_decode.hip: sets pkv_last_error()
+int ok();
+}  // namespace pkv
+
+namespace {
+
+constexpr int kD = 128;
+constexpr int kRowBytes = 2 * kD;
+constexpr int kScaleExp = 60;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+struct WriteArgs {
+  const uint8_t* k_new;  // token t, head h at k_new + t * k_stride + h * 256 (bytes)
+  const uint8_t* v_new;
+  uint8_t* k_pages;      // [num_pages, Hkv, ps, 128]
+  uint8_t* v_pages;
+  float* kv_scales;      // [num_pages, Hkv, 2] (block-scaled fp8)
+  const int32_t* slots;  // [tokens]
+  long k_stride, v_stride;
+  int32_t tokens, hkv, page_size;
+  int32_t num_slots;     // num_pages * page_size
+};
+
+// Sixteen lanes copy one (token, head) row of 256 bytes, K and V.
+__global__ __launch_bounds__(256) void write_kernel(WriteArgs a) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long row = i >> 4;
+  const int t = (int)(row / a.hkv), h = (int)(row - (long)t * a.hkv);
+  if (t >= a.tokens) return;
+  const int slot = a.slots[t];
+  if (slot < 0 || slot >= a.num_slots) return;
+  const int c = (int)(i & 15) * 16;
+  const int page = slot / a.page_size, off = slot - page * a.page_size;
+  const long to = (((long)page * a.hkv + h) * a.page_size + off) * kRowBytes + c;
+  const u32x4 k = *(const u32x4*)(a.k_new + t * a.k_stride + (long)h * kRowBytes + c);
+  const u32x4 v = *(const u32x4*)(a.v_new + t * a.v_stride + (long)h * kRowBytes + c);
+  *(u32x4*)(a.k_pages + to) = k;
+  *(u32x4*)(a.v_pages + to) = v;
+}
+
+// ---------------------------------------------------------------------------------
+// Block-scaled fp8.
+// ---------------------------------------------------------------------------------
+// Magnitudes of two 16-bit floats in an order in which every infinity and NaN lies below
+// every finite value: (|x| + one step of the exponent) mod 2^15.
+template <bool BF16>
+__device__ inline uint32_t finite_order(uint32_t x2) {
+  return ((x2 & 0x7fff7fffu) + (BF16 ? 0x00800080u : 0x04000400u)) & 0x7fff7fffu;
+}
+__device__ inline uint32_t max2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
+}
+template <bool BF16>
+__device__ inline uint32_t finite_max(uint32_t m, u32x4 x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max2(m, finite_order<BF16>(x[i]));
+  return m;
+}
+// The largest finite magnitude of a wave's values, from its lanes' finite_max.
+template <bool BF16>
+__device__ inline float wave_amax(uint32_t m) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = max2(m, __shfl_xor(m, d));
+  const uint32_t z = max(m & 0xffffu, m >> 16), one = BF16 ? 0x80u : 0x400u;
+  return pkv::half_bits_to_float<BF16>(z > one ? z - one : 0u);
+}
+
+// 2^e of the smallest power of two >= x, within the range of block scales (x not positive or
+// NaN: the smallest).  `top`: the mantissa up to which 2^exponent(x) itself is large enough.
+__device__ inline int pow2_exponent(float x, uint32_t top) {
+  const uint32_t b = __float_as_uint(x);
+  const int e = (int)(b >> 23) - 127 + ((b & 0x7fffffu) > top ? 1 : 0);
+  return x > 0.f ? e : -kScaleExp;
+}
+__device__ inline int clamp_exponent(int e) { return min(max(e, -kScaleExp), kScaleExp); }
+__device__ inline float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// 448 = 1.75 * 2^8: amax = m 2^e needs 2^(e - 8) if m <= 1.75 and 2^(e - 7) otherwise.
+__device__ inline int scale_exponent(float amax) {
+  return clamp_exponent(pow2_exponent(amax, 0x600000u) - 8);
+}
+__device__ inline int old_exponent(float scale) {
+  return scale > 0.f ? clamp_exponent(pow2_exponent(scale, 0u)) : -kScaleExp;
+}
+
+template <bool BF16>
+__device__ inline u32x2 encode8(u32x4 x, float inv) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    b[i] = pkv::e4m3_encode2(pkv::half_bits_to_float<BF16>(x[i] & 0xffffu) * inv,
+                             pkv::half_bits_to_float<BF16>(x[i] >> 16) * inv);
+  return u32x2{b[0] | b[1] << 16, b[2] | b[3] << 16};
+}
+
+// x * r in 32 bits rounded to odd: a later rounding to fewer bits is then the exact product's
+// (an old scale need not be a power of two, and x * r could otherwise round to a tie first).
+__device__ inline float mul_odd(float x, float r) {
+  const float p = x * r, err = __builtin_fmaf(x, r, -p);
+  const uint32_t b = __float_as_uint(p);
+  if (err == 0.f || (b & 1u)) return p;
+  return __uint_as_float((err > 0.f) == (p > 0.f) ? b + 1 : b - 1);
+}
+
+// The stored rows [0, rows) of one (page, head) block, times r (at most 1), rounded again.
+__device__ inline void rescale_rows(uint8_t* block, int rows, float r, int lane) {
+  for (int t = lane >> 4; t < rows; t += 4) {
+    u32x2* const p = (u32x2*)(block + (long)t * kD + (lane & 15) * 8);
+    u32x2 x = *p;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[i], false);
+      const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[i], true);
+      x[i] = pkv::e4m3_encode2(mul_odd(lo[0], r), mul_odd(lo[1], r)) |
+             pkv::e4m3_encode2(mul_odd(hi[0], r), mul_odd(hi[1], r)) << 16;
+    }
+    *p = x;
+  }
+}
+
+// One wave writes one run: `count` tokens from t0 on, in consecutive slots of one page.
+template <bool BF16>
+__device__ void write_run(const WriteArgs& a, int t0, int count, int page, int off, int h, int lane) {
+  const long block = (long)page * a.hkv + h;
+  float* const scales = a.kv_scales + 2 * block;
+  const long from = (long)h * kRowBytes + (lane & 15) * 16;
+  uint32_t mk = 0, mv = 0;
+  for (int t = lane >> 4; t < count; t += 4) {
+    mk = finite_max<BF16>(mk, *(const u32x4*)(a.k_new + (t0 + t) * a.k_stride + from));
+    mv = finite_max<BF16>(mv, *(const u32x4*)(a.v_new + (t0 + t) * a.v_stride + from));
+  }
+  int ek = scale_exponent(wave_amax<BF16>(mk)), ev = scale_exponent(wave_amax<BF16>(mv));
+  uint8_t* const kb = a.k_pages + block * a.page_size * kD;
+  uint8_t* const vb = a.v_pages + block * a.page_size * kD;
+  if (off > 0) {  // earlier tokens share the block: its scales can only grow
+    const float lo = pow2(-kScaleExp), hi = pow2(kScaleExp);
+    const float ks = fminf(fmaxf(scales[0], lo), hi), vs = fminf(fmaxf(scales[1], lo), hi);
+    ek = max(ek, old_exponent(ks));
+    ev = max(ev, old_exponent(vs));
+    if (ks != pow2(ek)) rescale_rows(kb, off, ks * pow2(-ek), lane);
+    if (vs != pow2(ev)) rescale_rows(vb, off, vs * pow2(-ev), lane);
+  }
+  const float ik = pow2(-ek), iv = pow2(-ev);
+  for (int t = lane >> 4; t < count; t += 4) {
+    const long to = (long)(off + t) * kD + (lane & 15) * 8;
+    *(u32x2*)(kb + to) = encode8<BF16>(*(const u32x4*)(a.k_new + (t0 + t) * a.k_stride + from), ik);
+    *(u32x2*)(vb + to) = encode8<BF16>(*(const u32x4*)(a.v_new + (t0 + t) * a.v_stride + from), iv);
+  }
+  if (lane == 0) *(f32x2*)scales = f32x2{pow2(ek), pow2(ev)};
+}
+
+// A wave takes the runs that begin in its `window` tokens, for one head.
+template <bool BF16>
+__global__ __launch_bounds__(256) void write_block_kernel(WriteArgs a, int window) {
+  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane((int)(id / a.hkv));
+  const int h = __builtin_amdgcn_readfirstlane((int)(id - (long)w * a.hkv));
+  const int first = (int)min((long)w * window, (long)a.tokens);
+  const int last = (int)min((long)first + window, (long)a.tokens);
+  for (int t = first; t < last; ++t) {
+    const int slot = a.slots[t];
+    if (slot < 0 || slot >= a.num_slots) continue;
+    const int page = slot / a.page_size, off = slot - page * a.page_size;
+    if (t > 0 && off > 0 && a.slots[t - 1] == slot - 1) continue;  // inside another run
+    const int most = min(a.page_size - off, a.tokens - t);
+    int count = 1;
+    for (bool more = true; more && count < most;) {  // slots that follow one another
+      const int i = count + lane;
+      const bool in = i < most && a.slots[t + i] == slot + i;
+      const uint64_t out = ~__builtin_amdgcn_ballot_w64(in);
+      const int n = out ? __builtin_ctzll(out) : 64;
+      count += n;
+      more = n == 64;
+    }
+    write_run<BF16>(a, t, count, page, off, h, lane);
+  }
+}
+
+int check_write(const char* op, const WriteArgs& a, int32_t head_dim, int32_t num_pages, int32_t dtype) {
+  using pkv::fail;
+  if (a.tokens < 0 || a.hkv <= 0 || a.page_size <= 0 || num_pages <= 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "%s: tokens %d, num_kv_heads %d, page_size %d, num_pages %d",
+                op, a.tokens, a.hkv, a.page_size, num_pages);
+  if (head_dim != kD) return fail(PKV_ERR_UNSUPPORTED, "%s: head_dim %d (only 128)", op, head_dim);
+  if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", op, dtype);
+  if ((long)num_pages * a.page_size > INT32_MAX)
+    return fail(PKV_ERR_UNSUPPORTED, "%s: num_pages * page_size does not fit in int32", op);
+  if ((long)a.tokens * a.hkv > (1L << 32))
+    return fail(PKV_ERR_UNSUPPORTED, "%s: tokens * num_kv_heads too large", op);
+  if (a.k_stride < (long)a.hkv * kRowBytes || a.v_stride < (long)a.hkv * kRowBytes ||
+      a.k_stride % 16 || a.v_stride % 16)
+    return fail(PKV_ERR_INVALID_ARGUMENT,
+                "%s: a token stride must hold num_kv_heads * 128 elements and be a multiple of 8", op);
+  if (a.tokens == 0) return PKV_OK;
+  if (!a.k_new || !a.v_new || !a.k_pages || !a.v_pages || !a.slots)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "%s: null pointer", op);
+  if (((uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages) & 15)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "%s: K and V must be 16-byte aligned", op);
+  return PKV_OK;
+}
+
+int launched(const char* op) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? pkv::ok() : pkv::fail(PKV_ERR_LAUNCH, "%s launch: %s", op, hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" {
+
+int pkv_write_kv(const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride,
+                 void* k_pages, void* v_pages, const int32_t* slot_mapping, int32_t tokens,
+                 int32_t num_kv_heads, int32_t head_dim, int32_t num_pages, int32_t page_size,
+                 int32_t dtype, void* stream) {
+  const WriteArgs a{(const uint8_t*)k_new, (const uint8_t*)v_new, (uint8_t*)k_pages,
+                    (uint8_t*)v_pages, nullptr, slot_mapping, 2 * k_stride, 2 * v_stride, tokens,
+                    num_kv_heads, page_size, (int32_t)((int64_t)num_pages * page_size)};
+  const int st = check_write("write_kv", a, head_dim, num_pages, dtype);
+  if (st != PKV_OK || tokens == 0) return st == PKV_OK ? pkv::ok() : st;
+  const long lanes = (long)tokens * num_kv_heads * 16;
+  write_kernel<<<dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, (hipStream_t)stream>>>(a);
+  return launched("write_kv");
+}
+
+int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_new,
+                           int64_t v_stride, void* k_pages, void* v_pages, float* kv_scales,
+                           const int32_t* slot_mapping, int32_t tokens, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t num_pages, int32_t page_size, int32_t dtype,
+                           void* stream) {
+  const WriteArgs a{(const uint8_t*)k_new, (const uint8_t*)v_new, (uint8_t*)k_pages,
+                    (uint8_t*)v_pages, kv_scales, slot_mapping, 2 * k_stride, 2 * v_stride, tokens,
+                    num_kv_heads, page_size, (int32_t)((int64_t)num_pages * page_size)};
+  const int st = check_write("write_kv_fp8_block", a, head_dim, num_pages, dtype);
+  if (st != PKV_OK || tokens == 0) return st == PKV_OK ? pkv::ok() : st;
+  if (!kv_scales || ((uintptr_t)kv_scales & 7))
+    return pkv::fail(PKV_ERR_INVALID_ARGUMENT, "write_kv_fp8_block: kv_scales null or not 8-byte aligned");
+  const int window = (long)tokens * num_kv_heads <= 16384 ? 1 : 16;
+  const long waves = (long)((tokens + window - 1) / window) * num_kv_heads;
+  const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
+  if (dtype == PKV_DTYPE_BF16) write_block_kernel<true><<<grid, block, 0, (hipStream_t)stream>>>(a, window);
+  else write_block_kernel<false><<<grid, block, 0, (hipStream_t)stream>>>(a, window);
+  return launched("write_kv_fp8_block");
+}
+
+}  // extern "C"

@@ -72,6 +72,21 @@ paged_attention_workqueue_append = _ext.paged_attention_workqueue_append
 paged_attention_indexed_fp8_append = _ext.paged_attention_indexed_fp8_append
 paged_attention_workqueue_fp8_append = _ext.paged_attention_workqueue_fp8_append
 
+# From a prompt to the cache.  build_block_tables(cached_lens, seq_lens, free_pages, num_free,
+# block_table, token_offsets, slot_mapping, num_free_out, page_size) gives a step's new tokens
+# their pages and slots; prefill_attention(q, k, v, token_offsets, output) is causal attention
+# over the packed prompts; write_kv(k_new, v_new, k_pages, v_pages, slot_mapping) and
+# write_kv_fp8_block(k_new, v_new, k_pages, v_pages, kv_scales, slot_mapping) store their K/V.
+build_block_tables = _ext.build_block_tables
+prefill_attention = _ext.prefill_attention
+write_kv = _ext.write_kv
+write_kv_fp8_block = _ext.write_kv_fp8_block
+# Decode over fp8 pools with kv_scales [pages, Hkv, 2] (K's and V's scale of each page and KV
+# head): (q, k_pages, v_pages, kv_scales, block_table, seq_lens, output, workspace, page_size),
+# with a workspace of fp8_block_workspace_floats(batch, Hq, Hkv) fp32 elements.
+paged_attention_fp8_block = _ext.paged_attention_fp8_block
+fp8_block_workspace_floats = _ext.fp8_block_workspace_floats
+
 # fp32 workspace elements with which a direct (num_splits == 1) launch of paged_attention,
 # paged_attention_masked / _indexed or attention_contiguous runs its full internal split
 # (0 when it is not split; a smaller workspace gives a smaller split, an empty one none).
@@ -101,6 +116,8 @@ __all__ = [
     "attention_query_head_baseline", "append_kv", "append_kv_fp8",
     "paged_attention_masked_append", "paged_attention_indexed_append",
     "paged_attention_workqueue_append",
-    "paged_attention_indexed_fp8_append", "paged_attention_workqueue_fp8_append", "workspace_floats",
+    "paged_attention_indexed_fp8_append", "paged_attention_workqueue_fp8_append",
+    "build_block_tables", "prefill_attention", "write_kv", "write_kv_fp8_block",
+    "paged_attention_fp8_block", "fp8_block_workspace_floats", "workspace_floats",
     "workqueue_workspace_floats", "direct_workspace_floats", "split_workspace_floats", "EXTENSION_PATH", "LIBRARY_PATH",
 ]

@@ -1,0 +1,55 @@
+"""Seeded inputs and tolerances shared by the tests of the operators between a prompt and the
+cache (CPU tensors)."""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}  # half a step, relative
+F32 = 2.0 ** -24
+
+
+def packed_inputs(lengths, hq, hkv, dtype, seed, lead=0, trail=0):
+    """Column ranges q, k, v of one fused projection [lead + tokens + trail, (hq + 2 hkv), 128],
+    and the sequences' offsets."""
+    gen = torch.Generator().manual_seed(seed)
+    tokens = lead + sum(lengths) + trail
+    qkv = torch.randn(tokens, hq + 2 * hkv, 128, generator=gen).to(dtype)
+    offsets = np.concatenate([[0], np.cumsum(lengths)]) + lead
+    return qkv, torch.tensor(offsets, dtype=torch.int32)
+
+
+def split_qkv(qkv, hq, hkv):
+    return qkv[:, :hq], qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+
+
+def attention_tolerance(out, weight, score, tokens, dtype, p_step, tiny):
+    """Bound on |kernel - exact| per element.
+
+    * The output's rounding: half a step of its type, and below its normal range half a step of
+      the subnormals, which are 2^-24 apart in fp16 and 2^-133 in bf16.
+    * Weights p_j enter the product with V rounded to `p_step` relative (half a step of the
+      product's operands), against a sum of unrounded weights: p_step * sum p_j |v_j|.
+    * A score is a sum of 128 products in 32 bits, off by at most 128 * 2^-24 * sum |q k| /
+      sqrt(128) (order free), and then scaled, shifted and exponentiated with a few more
+      roundings of values of up to |x| + 100 in log2: delta.  Relative errors of the weights of
+      up to delta move the quotient by at most 2 delta sum p_j |v_j|.
+    * The sums over the tokens in 32 bits: each at most (tokens + 16) 2^-24 of its weights,
+      numerator and denominator.
+    * `tiny`: what weights below the operand type's normal range may lose in all.
+    """
+    delta = 130 * F32 * score[..., None] + 64 * F32 * (1 + score[..., None]) + 200 * F32
+    sums = 2 * (tokens + 16) * F32
+    least = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}[dtype]
+    return U[dtype] * np.abs(out) + least + (1 + U[dtype]) * ((p_step + 2 * delta + sums) * weight + tiny)
+
+
+def assert_within(got, want, bound, what=""):
+    got = got.double().cpu().numpy()
+    finite = np.isfinite(want)
+    assert (np.isnan(got) == np.isnan(want)).all(), f"{what}: NaN in other places"
+    assert (got[~finite & ~np.isnan(want)] == want[~finite & ~np.isnan(want)]).all(), what
+    ratio = np.abs(got[finite] - want[finite]) / np.broadcast_to(bound, want.shape)[finite]
+    worst = float(ratio.max()) if ratio.size else 0.0
+    print(f"{what}: at most {worst:.3f} of the bound")
+    assert worst <= 1.0, (what, worst)

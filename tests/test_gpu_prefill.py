@@ -1,0 +1,142 @@
+"""prefill_attention against causal attention in 64 bits, element by element.
+
+Weights reach the product with V in the activation type (half a step: fp16 2^-11, bf16 2^-8),
+and in fp16 a weight below 2^-14 of the running maximum's is subnormal, off by up to 2^-25;
+the sum of weights is at least 1 in those units (the largest weight is).
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import prompt
+from prompt_cases import U, assert_within, attention_tolerance, packed_inputs, split_qkv
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _check(ext, gpu, qkv, offsets, hq, hkv, what=""):
+    dtype = qkv.dtype
+    q, k, v = split_qkv(qkv, hq, hkv)
+    out = torch.full(q.shape, 7.0, dtype=dtype, device=gpu)
+    ext.prefill_attention(*split_qkv(qkv.to(gpu), hq, hkv), offsets.to(gpu), out)
+    torch.cuda.synchronize()
+    off = offsets.tolist()
+    want, weight, vmax, score = prompt.prefill(q.double(), k.double(), v.double(), off)
+    inside = np.zeros(len(want), dtype=bool)
+    for s, e in zip(off, off[1:]):
+        inside[s:e] = True
+    assert (out[~torch.from_numpy(inside)].float() == 7.0).all()  # left as they were
+    longest = max([e - s for s, e in zip(off, off[1:])] + [1])
+    tiny = longest * 2.0 ** -25 * vmax if dtype == F16 else 0.0
+    bound = attention_tolerance(want, weight, score, longest, dtype, U[dtype], tiny)
+    sel = torch.from_numpy(inside)
+    assert_within(out.cpu()[sel], want[inside], bound[inside], what)
+    return out
+
+
+LENGTHS = [[1], [2], [31], [64], [65], [500], [63, 1, 64, 2, 65, 0, 3], [0, 0], [1] * 70, [130, 257, 5], [1000, 17]]
+
+
+@pytest.mark.parametrize("lengths", LENGTHS, ids=lambda x: "-".join(map(str, x[:8])))
+@pytest.mark.parametrize("hq,hkv,dtype", [(8, 2, F16), (8, 2, BF16), (3, 3, F16)])
+def test_lengths(ext, gpu, lengths, hq, hkv, dtype):
+    qkv, off = packed_inputs(lengths, hq, hkv, dtype, seed=sum(lengths))
+    _check(ext, gpu, qkv, off, hq, hkv, f"{lengths[:8]}")
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (2, 1), (3, 1), (5, 1), (8, 1), (10, 2), (16, 1), (31, 1), (32, 1), (12, 4), (9, 9)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_head_layouts(ext, gpu, hq, hkv, dtype):
+    lengths = [77, 1, 300]
+    qkv, off = packed_inputs(lengths, hq, hkv, dtype, seed=hq * 40 + hkv)
+    _check(ext, gpu, qkv, off, hq, hkv, f"Hq {hq} Hkv {hkv}")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_tokens_outside_every_sequence(ext, gpu, dtype):
+    """Tokens before the first and behind the last sequence hold NaN: nothing reads them, and
+    their output rows stay."""
+    qkv, off = packed_inputs([70, 3, 129], 8, 2, dtype, seed=3, lead=300, trail=90)
+    qkv[:300] = float("nan")
+    qkv[300 + 202:] = float("nan")
+    _check(ext, gpu, qkv, off, 8, 2)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (2, 2), (16, 1)])
+def test_nonfinite_values_reach_later_tokens_only(ext, gpu, dtype, hq, hkv):
+    qkv, off = packed_inputs([100, 150, 64], hq, hkv, dtype, seed=4)
+    k, v = qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    inf, nan = float("inf"), float("nan")
+    v[70, 0, 3], v[90, 0, 3], v[40, 0, 127], v[99, hkv - 1, 0] = inf, -inf, nan, nan
+    v[100 + 149, 0, 64], v[100, 0, 17] = nan, inf
+    k[100 + 130, 0, 5] = nan     # every score of the tokens from 130 on
+    v[250 + 63, 0, :] = nan
+    _check(ext, gpu, qkv, off, hq, hkv)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_growing_and_peaked_scores(ext, gpu, dtype):
+    """Scores that grow along the prompt (the running maximum moves in every tile) and ones so
+    far apart that a single token takes all the weight."""
+    qkv, off = packed_inputs([400], 4, 1, dtype, seed=6)
+    ramp = torch.linspace(0.0, 6.0, 400)[:, None]
+    qkv[:, :4] = 1.0
+    qkv[:, 4] = ramp.to(dtype)
+    _check(ext, gpu, qkv, off, 4, 1, "ramp")
+    qkv[:, 4] = -ramp.to(dtype)
+    _check(ext, gpu, qkv, off, 4, 1, "falling ramp")
+    qkv[:, 4] = 0.0
+    qkv[199, 4] = 40.0
+    _check(ext, gpu, qkv, off, 4, 1, "one peak")
+
+
+def test_contiguous_and_offset_inputs(ext, gpu):
+    qkv, off = packed_inputs([150, 33], 8, 2, F16, seed=8)
+    ref = _check(ext, gpu, qkv, off, 8, 2)
+    q, k, v = (x.contiguous().to(gpu) for x in split_qkv(qkv, 8, 2))
+    out = torch.empty_like(q)
+    ext.prefill_attention(q, k, v, off.to(gpu), out)
+    assert torch.equal(out, ref)
+    ext.prefill_attention(q, k, v, off.to(gpu), q)  # in place: a row is read before it is written
+    assert torch.equal(q, ref)
+
+
+def test_bad_offsets_stay_inside(ext, gpu):
+    """Offsets past the tokens, or negative, count as clamped."""
+    qkv, _ = packed_inputs([200], 4, 2, F16, seed=9)
+    a = torch.full((200, 4, 128), 7.0, dtype=F16, device=gpu)
+    b = a.clone()
+    parts = split_qkv(qkv.to(gpu), 4, 2)
+    ext.prefill_attention(*parts, torch.tensor([-5, 60, 900], dtype=torch.int32, device=gpu), a)
+    ext.prefill_attention(*parts, torch.tensor([0, 60, 200], dtype=torch.int32, device=gpu), b)
+    assert torch.equal(a, b)
+
+
+def test_streams_and_graph_replays(ext, gpu):
+    cases = [packed_inputs(l, 8, 2, F16, seed=s) for s, l in ((1, [300, 41]), (2, [129, 212]))]
+    refs = [_check(ext, gpu, *c, 8, 2) for c in cases]
+    outs = [torch.zeros_like(r) for r in refs]
+    ins = [(c[0].to(gpu), c[1].to(gpu)) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for st, (qkv, off), out in zip(streams, ins, outs):
+            with torch.cuda.stream(st):
+                ext.prefill_attention(*split_qkv(qkv, 8, 2), off, out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, r) for o, r in zip(outs, refs))
+    qkv, off = ins[0][0].clone(), ins[0][1].clone()
+    out = torch.zeros_like(refs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ext.prefill_attention(*split_qkv(qkv, 8, 2), off, out)
+    for i in (0, 1, 0, 1):  # the captured call follows its inputs, the lengths among them
+        qkv.copy_(ins[i][0])
+        off.copy_(ins[i][1])
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, refs[i])

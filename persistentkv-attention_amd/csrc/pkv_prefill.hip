@@ -36,7 +36,7 @@ namespace {
 constexpr int kD = 128;
 constexpr int kRowBytes = 2 * kD;
 constexpr int kKeys = 64;    // keys per tile
-constexpr int kWaves = 8;
+constexpr int kWaves = 4;
 constexpr int kWaveRows = 32;
 constexpr int kRows = kWaves * kWaveRows;
 constexpr int kTileBytes = kKeys * kRowBytes;
@@ -105,10 +105,17 @@ __device__ inline int first_slot(const PrefillArgs& a, int b) {
   return (int)((uint32_t)(offset_of(a, b) * a.group) / kRows) + b;
 }
 
-// Two rows of K and of V of a tile in a thread's registers, on their way to LDS.
-struct Stage {
-  u32x4 k[2], v[2];
-};
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+// 64 x 16 bytes from a buffer straight to LDS, lane l's to `lds` + 16 l.  In assembly because the
+// compiler lets every LDS read wait for every such load in flight, the next tile's among them;
+// landed() is the wait, before the barrier behind which the tile is read.  No registers are
+// written.
+__device__ inline void load_to_lds(uint32_t lds, i32x4 rsrc, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(lds), "v"(offset), "s"(rsrc) : "memory");
+}
+__device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // The top bits of those halves of a pair of 16-bit floats that are infinite or NaN.
 template <class Elem>
@@ -129,24 +136,26 @@ __device__ inline uint2 infinities(uint32_t x2) {
 }
 
 template <class Elem>
-__global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
+__global__ __launch_bounds__(kWaves * 64, 2) void prefill_kernel(PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][kTileBytes];  // [buffer][K, V]
-  __shared__ int nonfinite[2];  // [buffer] 1 + the last tile whose V held an infinity or NaN
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int col = lane & 31, half = lane >> 5;
   const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
   const int slot = uniform((int)(blockIdx.x / (unsigned)a.hkv));
+  // The last sequence whose first slot is at most `slot`, 64 candidates at a time.
   int b = 0;
-  for (int n = a.batch; n > 1;) {  // the last sequence whose first slot is at most `slot`
-    const int mid = n >> 1;
-    if (first_slot(a, b + mid) <= slot) b += mid, n -= mid;
-    else n = mid;
+  for (int n = a.batch; n > 1;) {  // it is one of b ... b + n - 1
+    const int step = (n + 63) >> 6, at = lane * step;
+    const uint64_t fits = __builtin_amdgcn_ballot_w64(at < n && first_slot(a, b + at) <= slot);
+    const int found = fits ? (63 - __builtin_clzll(fits)) * step : 0;
+    b += found;
+    n = min(step, n - found);
   }
   const int start = uniform(offset_of(a, b));
   const int len = uniform(max(offset_of(a, b + 1) - start, 0));
   const int rows = len * a.group;
   const int blocks = (rows + kRows - 1) / kRows;
-  const int block = blocks - 1 - (slot - first_slot(a, b));  // the longest first
+  const int block = blocks - 1 - (slot - uniform(first_slot(a, b)));  // the longest first
   if (block < 0 || block >= blocks) return;  // a slot that no block of a sequence takes
 
   const int row0 = block * kRows + wave * kWaveRows;
@@ -154,7 +163,6 @@ __global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
   const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
   const int wave_first = uniform(min(row0, rows - 1) / a.group);
   const int wave_last = uniform(min(row0 + kWaveRows - 1, rows - 1) / a.group);
-  const int first = uniform(block * kRows / a.group);  // the workgroup's first and last tokens
   const int last = uniform(min(block * kRows + kRows - 1, rows - 1) / a.group);
   const int tiles = last / kKeys + 1;
 
@@ -163,49 +171,32 @@ __global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) q[kk] = *(const u32x4*)(qp + kk * 32);
 
-  // Staging: thread t moves 16-byte chunk t % 16 of rows t / 16 and t / 16 + 32.  Chunks are
-  // stored under an exclusive or with the row, so that reads of one chunk column (K) or of 64
-  // bytes of four rows (V) spread over all banks.
-  const int srow = tid >> 4, chunk = tid & 15;
-  const uint32_t kdst = srow * kRowBytes + ((chunk ^ (srow & 15)) << 4);
-  const uint32_t vdst = srow * kRowBytes + ((chunk ^ ((srow & 3) << 2)) << 4);
+  // A wave moves rows 16 wave + 4 i + lane / 16 of a tile, 256 bytes a row.  16-byte chunk p of
+  // row r in LDS is chunk p ^ r of K's row (p ^ 4 r of V's), so that reads of one chunk column
+  // (K) or of 64 bytes of four rows (V) spread over all banks.
+  const int srow = wave * (kKeys / kWaves) + (lane >> 4), chunk = lane & 15;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0][0][0] +
+                        (uint32_t)(wave * (kKeys / kWaves) * kRowBytes);
   const uint8_t* kbase = a.k + (long)start * a.k_stride + (long)kvh * kRowBytes;
   const uint8_t* vbase = a.v + (long)start * a.v_stride + (long)kvh * kRowBytes;
-  const uint32_t koff = (uint32_t)(srow * (int)a.k_stride + chunk * 16);
-  const uint32_t voff = (uint32_t)(srow * (int)a.v_stride + chunk * 16);
-  auto fetch = [&](int tile, Stage& r) {
+  const uint32_t koff = (uint32_t)(srow * (int)a.k_stride), kchunk = (chunk ^ (srow & 15)) << 4;
+  const uint32_t voff = (uint32_t)(srow * (int)a.v_stride) + ((chunk ^ ((srow & 3) << 2)) << 4);
+  auto rsrc = [&](const uint8_t* base, long stride, int tile, int n) {
     // Rows past the sequence's end read as zero: the descriptor ends with its last row.
-    const int n = min(kKeys, len - tile * kKeys);
-    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-        uniform_ptr(kbase + (long)tile * kKeys * a.k_stride), (short)0,
-        uniform((n - 1) * (int)a.k_stride + kRowBytes), kRsrcWord3);
-    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-        uniform_ptr(vbase + (long)tile * kKeys * a.v_stride), (short)0,
-        uniform((n - 1) * (int)a.v_stride + kRowBytes), kRsrcWord3);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      r.k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff + i * 32 * (uint32_t)a.k_stride, 0, 0));
-      r.v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff + i * 32 * (uint32_t)a.v_stride, 0, 0));
-    }
+    const uint64_t at = (uint64_t)(base + (long)tile * kKeys * stride);
+    return i32x4{uniform((int)at), uniform((int)(at >> 32) & 0xffff),
+                 uniform((n - 1) * (int)stride + kRowBytes), (int)kRsrcWord3};
   };
-  // A masked weight is 0, and 0 times an infinity or NaN in V is NaN: tiles that some row of
-  // the workgroup masks in part are looked over on their way, and take another path below
-  // where V is not finite.  Such values then reach the rows from their token on, and no other.
-  auto store = [&](int tile, const Stage& r) {
-    const int buf = tile & 1;
-    if ((tile + 1) * kKeys - 1 > first) {
-      uint32_t bad = 0;
+  auto fetch = [&](int tile) {
+    const int n = min(kKeys, len - tile * kKeys);
+    const i32x4 rk = rsrc(kbase, a.k_stride, tile, n), rv = rsrc(vbase, a.v_stride, tile, n);
+    const uint32_t to = (uint32_t)uniform((int)(lds0 + (tile & 1) * 2 * kTileBytes));
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kKeys / kWaves / 4; ++i)
+      load_to_lds(to + i * 4 * kRowBytes, rk, koff + (kchunk ^ (i << 6)) + i * 4 * (uint32_t)a.k_stride);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bad |= nonfinite_halves<Elem>(r.v[i][j]);
-      if (bad) nonfinite[buf] = tile + 1;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      *(u32x4*)(&lds[buf][0][kdst + i * 32 * kRowBytes]) = r.k[i];
-      *(u32x4*)(&lds[buf][1][vdst + i * 32 * kRowBytes]) = r.v[i];
-    }
+    for (int i = 0; i < kKeys / kWaves / 4; ++i)
+      load_to_lds(to + kTileBytes + i * 4 * kRowBytes, rv, voff + i * 4 * (uint32_t)a.v_stride);
   };
   // Reads: lane's K row (key col), chunk 2 kk + half; V rows 4 half + (lane % 16) / 4, four
   // dims from 32 db + 16 (lane / 16 % 2) + 4 (lane % 4) on.
@@ -213,122 +204,133 @@ __global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
   const int vr = (lane >> 2) & 3;
   const uint32_t vsrc = (4 * half + vr) * kRowBytes + (vr << 6) + ((lane & 16) << 1) + ((lane & 3) << 3);
 
-  f32x16 o[4] = {};
-  float m = -INFINITY, l = 0.f;
-
-  Stage r;
-  if (tid < 2) nonfinite[tid] = 0;
-  __syncthreads();
-  fetch(0, r);
-  store(0, r);
-  __syncthreads();
-  for (int tile = 0; tile < tiles; ++tile) {
-    const int buf = tile & 1;
-    if (tile + 1 < tiles) fetch(tile + 1, r);
-    const int k0 = tile * kKeys;
-    if (k0 <= wave_last) {
-      const uint8_t* const kt = lds[buf][0];
-      const uint8_t* const vt = lds[buf][1];
-      f32x16 s[2] = {};
+  f32x16 o[4];
+  float m, l;
+  auto sweep = [&](auto careful) {
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
+    for (int db = 0; db < 4; ++db) o[db] = f32x16{};
+    m = -INFINITY, l = 0.f;
+    fetch(0);
+    landed();
+    __syncthreads();
+    for (int tile = 0; tile < tiles; ++tile) {
+      const int buf = tile & 1;
+      if (tile + 1 < tiles) fetch(tile + 1);
+      const int k0 = tile * kKeys;
+      if (k0 <= wave_last) {
+        const uint8_t* const kt = lds[buf][0];
+        const uint8_t* const vt = lds[buf][1];
+        f32x16 s[2] = {};
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          s[kb] = Elem::mma(*(const u32x4*)(kt + (ksrc ^ (kk << 5)) + kb * 32 * kRowBytes), q[kk], s[kb]);
-      const bool diagonal = k0 + kKeys - 1 > wave_first;
-      if (diagonal) {
+        for (int kk = 0; kk < 8; ++kk)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < 2; ++kb)
+            s[kb] = Elem::mma(*(const u32x4*)(kt + (ksrc ^ (kk << 5)) + kb * 32 * kRowBytes), q[kk], s[kb]);
+        const bool diagonal = k0 + kKeys - 1 > wave_first;
+        if (diagonal) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (k0 + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) > tok) s[kb][i] = -INFINITY;
-      }
-      float mx = s[0][0];
+          for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx);
-        const float c = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2);
-        m = mn;
-        l *= c;
-#pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[db][i] *= c;
-      }
-      const float ms = m * kScaleLog2;
-      u32x4 p[4];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], kScaleLog2, -ms));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], kScaleLog2, -ms));
-          l += p0 + p1;
-          p[2 * kb + (i >> 3)][(i & 7) >> 1] = Elem::pack2(p0, p1);
+            for (int i = 0; i < 16; ++i)
+              if (k0 + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) > tok) s[kb][i] = -INFINITY;
         }
-      auto value = [&](int c, int db) {  // V^T's operand: 16 keys from 16 c on, dims 32 db + lane % 32
-        typedef __attribute__((address_space(3))) s16x4* Lds;
-        const uint8_t* at = vt + (vsrc ^ (db << 6)) + c * 16 * kRowBytes;
-        const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at));
-        const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 8 * kRowBytes)));
-        return u32x4{v0[0], v0[1], v1[0], v1[1]};
-      };
-      auto pv = [&](auto clean) {
+        float mx = s[0][0];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int db = 0; db < 4; ++db) {
-            if constexpr (decltype(clean)::value) __builtin_amdgcn_sched_barrier(0);
-            u32x4 x = value(c, db);
-            if constexpr (decltype(clean)::value) {
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+        if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float mn = fmaxf(m, mx);
+          const float c = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2);
+          m = mn;
+          l *= c;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[i] = drop_nonfinite<Elem>(x[i]);
+          for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] *= c;
+        }
+        const float ms = m * kScaleLog2;
+        u32x4 p[4];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], kScaleLog2, -ms));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], kScaleLog2, -ms));
+            l += p0 + p1;
+            p[2 * kb + (i >> 3)][(i & 7) >> 1] = Elem::pack2(p0, p1);
+          }
+        auto value = [&](int c, int db) {  // V^T's operand: 16 keys from 16 c on, dims 32 db + lane % 32
+          typedef __attribute__((address_space(3))) s16x4* Lds;
+          const uint8_t* at = vt + (vsrc ^ (db << 6)) + c * 16 * kRowBytes;
+          const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at));
+          const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 8 * kRowBytes)));
+          return u32x4{v0[0], v0[1], v1[0], v1[1]};
+        };
+        auto pv = [&](auto clean) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int db = 0; db < 4; ++db) {
+              if constexpr (decltype(clean)::value) __builtin_amdgcn_sched_barrier(0);
+              u32x4 x = value(c, db);
+              if constexpr (decltype(clean)::value) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = drop_nonfinite<Elem>(x[i]);
+              }
+              o[db] = Elem::mma(x, p[c], o[db]);
             }
-            o[db] = Elem::mma(x, p[c], o[db]);
-          }
-      };
-      if (diagonal && uniform(nonfinite[buf]) == tile + 1) {
-        pv(std::true_type{});
-        // How many +inf and -inf (a NaN is both) each row sees in each dim, as products too.
-        u32x4 see[4];
+        };
+        if (decltype(careful)::value && diagonal) {
+          pv(std::true_type{});
+          // How many +inf and -inf (a NaN is both) each row sees in each dim, as products too.
+          u32x4 see[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = k0 + 16 * c + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
-            see[c][i] = (key <= tok ? Elem::kOne : 0u) | (key + 1 <= tok ? Elem::kOne << 16 : 0u);
-          }
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          f32x16 up = {}, down = {};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
-            const u32x4 x = value(c, db);
-            u32x4 xu, xd;
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint2 n = infinities<Elem>(x[i]);
-              xu[i] = n.x, xd[i] = n.y;
+              const int key = k0 + 16 * c + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
+              see[c][i] = (key <= tok ? Elem::kOne : 0u) | (key + 1 <= tok ? Elem::kOne << 16 : 0u);
             }
-            up = Elem::mma(xu, see[c], up);
-            down = Elem::mma(xd, see[c], down);
-          }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            o[db][i] += (up[i] > 0.f ? INFINITY : 0.f) + (down[i] > 0.f ? -INFINITY : 0.f);
+          for (int db = 0; db < 4; ++db) {
+            f32x16 up = {}, down = {};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
+              const u32x4 x = value(c, db);
+              u32x4 xu, xd;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint2 n = infinities<Elem>(x[i]);
+                xu[i] = n.x, xd[i] = n.y;
+              }
+              up = Elem::mma(xu, see[c], up);
+              down = Elem::mma(xd, see[c], down);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              o[db][i] += (up[i] > 0.f ? INFINITY : 0.f) + (down[i] > 0.f ? -INFINITY : 0.f);
+          }
+        } else {
+          pv(std::false_type{});
         }
-      } else {
-        pv(std::false_type{});
       }
+      landed();
+      __syncthreads();
     }
-    if (tile + 1 < tiles) store(tile + 1, r);
-    __syncthreads();
-  }
+  };
+  sweep(std::false_type{});
+  // A masked weight is 0, and 0 times an infinity or NaN in V is NaN.  So where a row comes out
+  // not finite, its workgroup computes once more with such values taken out of the tiles that
+  // a row masks in part, and put back for the rows from their token on.
+  float zero = 0.f;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(o[db][i], 0.f, zero);
+  if (__syncthreads_or(zero != 0.f)) sweep(std::true_type{});
 
   if (row0 + col >= rows) return;
   const float inv = 1.0f / (l + __shfl_xor(l, 32));

@@ -6,13 +6,14 @@
 //
 // Rows of work.  The G query heads of a KV head are rows of one matrix product over the same K
 // and V: row r of a (sequence, KV head) is token r / G, head kvh * G + r % G.  A workgroup of
-// eight waves owns 256 consecutive rows (for G = 4: 64 tokens), a wave 32 of them, so K/V
+// four waves owns 128 consecutive rows (for G = 4: 32 tokens), a wave 32 of them, so K/V
 // tiles are read from L2 once for all heads of the group, any G is served by one kernel, and
-// the masked part of a diagonal tile covers few tokens.
+// the masked part of a diagonal tile covers few tokens.  Consecutive workgroups take the KV
+// heads in turn: with 8 heads, or a multiple, each XCD's L2 holds the K/V of its own.
 //
-// Per wave and tile of 64 keys, with v_mfma_f32_32x32x16:
+// Per wave and tile of 32 keys, with v_mfma_f32_32x32x16:
 //   S^T[key, row] = K Q^T   K from LDS as the A operand, Q in registers as the B operand.
-//   A lane then holds 32 keys of ONE row: maximum and sum of the softmax are lane-local but
+//   A lane then holds 16 keys of ONE row: maximum and sum of the softmax are lane-local but
 //   for one exchange between the wave's halves.
 //   O^T[dim, row] += V^T P^T   P^T's B operand is S^T's own register layout, packed to 16 bits
 //   (the k order of a product is free as long as both operands agree), V^T's A operand comes
@@ -35,7 +36,8 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kRowBytes = 2 * kD;
-constexpr int kKeys = 64;    // keys per tile
+constexpr int kKeys = 32;    // keys per tile
+constexpr int kBuffers = 3;  // tiles in LDS: one read, one landed, one on its way
 constexpr int kWaves = 4;
 constexpr int kWaveRows = 32;
 constexpr int kRows = kWaves * kWaveRows;
@@ -59,6 +61,9 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 struct Half {
   static constexpr uint32_t kExponentStep = 0x04000400u;  // one step of both halves' exponents
   static constexpr uint32_t kOne = 0x3c00u;
+  __device__ static inline float sum2(uint32_t x, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, kOne * 0x10001u), c, false);
+  }
   __device__ static inline f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -70,6 +75,9 @@ struct Half {
 struct BFloat {
   static constexpr uint32_t kExponentStep = 0x00800080u;
   static constexpr uint32_t kOne = 0x3f80u;
+  __device__ static inline float sum2(uint32_t x, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, kOne * 0x10001u), c, false);
+  }
   __device__ static inline f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -99,10 +107,10 @@ __device__ inline void* uniform_ptr(const void* p) {
 __device__ inline int offset_of(const PrefillArgs& a, int b) {
   return min(max(a.token_offsets[b], 0), a.tokens);
 }
-// First workgroup slot of sequence b.  Its rows start at row offset x = offset * G; the slots
-// from x / 256 + b on, up to the next sequence's, are at least as many as its 256-row blocks.
-__device__ inline int first_slot(const PrefillArgs& a, int b) {
-  return (int)((uint32_t)(offset_of(a, b) * a.group) / kRows) + b;
+// First workgroup slot of sequence b, from its offset.  Its rows start at x = offset * G; the slots
+// from x / kRows + b on, up to the next sequence's, are at least as many as its blocks of rows.
+__device__ inline int first_slot(const PrefillArgs& a, int offset, int b) {
+  return (int)((uint32_t)(offset * a.group) / kRows) + b;
 }
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
@@ -115,7 +123,14 @@ __device__ inline void load_to_lds(uint32_t lds, i32x4 rsrc, uint32_t offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(lds), "v"(offset), "s"(rsrc) : "memory");
 }
-__device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits until at most N of the wave's loads are in flight.
+template <int N>
+__device__ inline void landed() {
+  static_assert(N < 16);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | N);  // vmcnt(N), nothing else
+  asm volatile("" ::: "memory");
+}
 
 // The top bits of those halves of a pair of 16-bit floats that are infinite or NaN.
 template <class Elem>
@@ -136,26 +151,28 @@ __device__ inline uint2 infinities(uint32_t x2) {
 }
 
 template <class Elem>
-__global__ __launch_bounds__(kWaves * 64, 2) void prefill_kernel(PrefillArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][kTileBytes];  // [buffer][K, V]
+__global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers * 2 * kTileBytes];  // K and V of each tile
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int col = lane & 31, half = lane >> 5;
   const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
   const int slot = uniform((int)(blockIdx.x / (unsigned)a.hkv));
-  // The last sequence whose first slot is at most `slot`, 64 candidates at a time.
-  int b = 0;
-  for (int n = a.batch; n > 1;) {  // it is one of b ... b + n - 1
-    const int step = (n + 63) >> 6, at = lane * step;
-    const uint64_t fits = __builtin_amdgcn_ballot_w64(at < n && first_slot(a, b + at) <= slot);
-    const int found = fits ? (63 - __builtin_clzll(fits)) * step : 0;
-    b += found;
-    n = min(step, n - found);
-  }
-  const int start = uniform(offset_of(a, b));
-  const int len = uniform(max(offset_of(a, b + 1) - start, 0));
+  // The last sequence whose first slot is at most `slot`, 63 candidates at a time; the last
+  // round's lanes hold its offset and its successor's.
+  int b = 0, n = a.batch, stride, offset, found;
+  do {
+    stride = (n + 62) / 63;
+    offset = offset_of(a, min(b + min(lane * stride, n), a.batch));
+    const uint64_t fits = __builtin_amdgcn_ballot_w64(lane * stride < n && first_slot(a, offset, b + lane * stride) <= slot);
+    found = fits ? 63 - __builtin_clzll(fits) : 0;
+    b += found * stride;
+    n = min(stride, n - found * stride);
+  } while (stride > 1);
+  const int start = __builtin_amdgcn_readlane(offset, found);
+  const int len = max(__builtin_amdgcn_readlane(offset, found + 1) - start, 0);
   const int rows = len * a.group;
   const int blocks = (rows + kRows - 1) / kRows;
-  const int block = blocks - 1 - (slot - uniform(first_slot(a, b)));  // the longest first
+  const int block = blocks - 1 - (slot - first_slot(a, start, b));  // the longest first
   if (block < 0 || block >= blocks) return;  // a slot that no block of a sequence takes
 
   const int row0 = block * kRows + wave * kWaveRows;
@@ -175,7 +192,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prefill_kernel(PrefillArgs a) 
   // row r in LDS is chunk p ^ r of K's row (p ^ 4 r of V's), so that reads of one chunk column
   // (K) or of 64 bytes of four rows (V) spread over all banks.
   const int srow = wave * (kKeys / kWaves) + (lane >> 4), chunk = lane & 15;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0][0][0] +
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0] +
                         (uint32_t)(wave * (kKeys / kWaves) * kRowBytes);
   const uint8_t* kbase = a.k + (long)start * a.k_stride + (long)kvh * kRowBytes;
   const uint8_t* vbase = a.v + (long)start * a.v_stride + (long)kvh * kRowBytes;
@@ -187,15 +204,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prefill_kernel(PrefillArgs a) 
     return i32x4{uniform((int)at), uniform((int)(at >> 32) & 0xffff),
                  uniform((n - 1) * (int)stride + kRowBytes), (int)kRsrcWord3};
   };
-  auto fetch = [&](int tile) {
+  constexpr int kLoads = kKeys / kWaves / 4;  // per wave and tile of K, and of V
+  auto fetch = [&](int tile, int buf) __attribute__((always_inline)) {
     const int n = min(kKeys, len - tile * kKeys);
     const i32x4 rk = rsrc(kbase, a.k_stride, tile, n), rv = rsrc(vbase, a.v_stride, tile, n);
-    const uint32_t to = (uint32_t)uniform((int)(lds0 + (tile & 1) * 2 * kTileBytes));
+    const uint32_t to = (uint32_t)uniform((int)(lds0 + buf * 2 * kTileBytes));
 #pragma unroll
-    for (int i = 0; i < kKeys / kWaves / 4; ++i)
+    for (int i = 0; i < kLoads; ++i)
       load_to_lds(to + i * 4 * kRowBytes, rk, koff + (kchunk ^ (i << 6)) + i * 4 * (uint32_t)a.k_stride);
 #pragma unroll
-    for (int i = 0; i < kKeys / kWaves / 4; ++i)
+    for (int i = 0; i < kLoads; ++i)
       load_to_lds(to + kTileBytes + i * 4 * kRowBytes, rv, voff + i * 4 * (uint32_t)a.v_stride);
   };
   // Reads: lane's K row (key col), chunk 2 kk + half; V rows 4 half + (lane % 16) / 4, four
@@ -206,119 +224,126 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prefill_kernel(PrefillArgs a) 
 
   f32x16 o[4];
   float m, l;
-  auto sweep = [&](auto careful) {
+  const uint8_t* kat[8];
+  const uint8_t* vat[4];
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) kat[kk] = lds + (ksrc ^ (kk << 5));
+#pragma unroll
+  for (int db = 0; db < 4; ++db) vat[db] = lds + kTileBytes + (vsrc ^ (db << 6));
+
+  // Tile `tile`, which lies in buffer `buf`; `careful`: see below.
+  auto step = [&](int tile, int buf, auto careful) __attribute__((always_inline)) {
+    const int at = buf * 2 * kTileBytes;
+    if (tile + 2 < tiles) fetch(tile + 2, buf >= 1 ? buf - 1 : buf + 2);
+    const int k0 = tile * kKeys;
+    if (k0 <= wave_last) {
+      f32x16 s = {};
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) s = Elem::mma(*(const u32x4*)(kat[kk] + at), q[kk], s);
+      auto value = [&](int c, int db) __attribute__((always_inline)) {  // keys 16 c ..., dims 32 db + lane % 32
+        typedef __attribute__((address_space(3))) s16x4* Lds;
+        const uint8_t* v = vat[db] + at + c * 16 * kRowBytes;
+        const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)v));
+        const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v + 8 * kRowBytes)));
+        return u32x4{v0[0], v0[1], v1[0], v1[1]};
+      };
+      u32x4 v0[4];
+#pragma unroll
+      for (int db = 0; db < 4; ++db) v0[db] = value(0, db);
+      const bool diagonal = k0 + kKeys - 1 > wave_first;
+      if (diagonal) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (k0 + 8 * (i >> 2) + 4 * half + (i & 3) > tok) s[i] = -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float mn = fmaxf(m, mx);
+        const float c = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2);
+        m = mn;
+        l *= c;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[db][i] *= c;
+      }
+      const float ms = m * kScaleLog2;
+      u32x4 p[2];
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t x = Elem::pack2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kScaleLog2, -ms)),
+                                       __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], kScaleLog2, -ms)));
+        p[i >> 3][(i & 7) >> 1] = x;
+        l = Elem::sum2(x, l);
+      }
+      if (decltype(careful)::value && diagonal) {
+        // How many +inf and -inf (a NaN is both) each row sees in each dim, as products too.
+        u32x4 see[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = k0 + 16 * c + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
+            see[c][i] = (key <= tok ? Elem::kOne : 0u) | (key + 1 <= tok ? Elem::kOne << 16 : 0u);
+          }
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          f32x16 up = {}, down = {};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
+            u32x4 x = value(c, db), xu, xd;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint2 n = infinities<Elem>(x[i]);
+              xu[i] = n.x, xd[i] = n.y;
+              x[i] = drop_nonfinite<Elem>(x[i]);
+            }
+            up = Elem::mma(xu, see[c], up);
+            down = Elem::mma(xd, see[c], down);
+            o[db] = Elem::mma(x, p[c], o[db]);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            o[db][i] += (up[i] > 0.f ? INFINITY : 0.f) + (down[i] > 0.f ? -INFINITY : 0.f);
+        }
+      } else {
+        u32x4 v1[4];
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          v1[db] = value(1, db);
+          o[db] = Elem::mma(v0[db], p[0], o[db]);
+        }
+#pragma unroll
+        for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v1[db], p[1], o[db]);
+      }
+    }
+    // The next tile has landed, and behind the barrier this one's place is free.
+    if (tile + 2 < tiles) landed<2 * kLoads>();
+    else landed<0>();
+    __syncthreads();
+  };
+  auto sweep = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
     for (int db = 0; db < 4; ++db) o[db] = f32x16{};
     m = -INFINITY, l = 0.f;
-    fetch(0);
-    landed();
+    fetch(0, 0);
+    if (tiles > 1) fetch(1, 1);
+    landed<0>();
     __syncthreads();
-    for (int tile = 0; tile < tiles; ++tile) {
-      const int buf = tile & 1;
-      if (tile + 1 < tiles) fetch(tile + 1);
-      const int k0 = tile * kKeys;
-      if (k0 <= wave_last) {
-        const uint8_t* const kt = lds[buf][0];
-        const uint8_t* const vt = lds[buf][1];
-        f32x16 s[2] = {};
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-            s[kb] = Elem::mma(*(const u32x4*)(kt + (ksrc ^ (kk << 5)) + kb * 32 * kRowBytes), q[kk], s[kb]);
-        const bool diagonal = k0 + kKeys - 1 > wave_first;
-        if (diagonal) {
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (k0 + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) > tok) s[kb][i] = -INFINITY;
-        }
-        float mx = s[0][0];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-        if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
-          mx = fmaxf(mx, __shfl_xor(mx, 32));
-          const float mn = fmaxf(m, mx);
-          const float c = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2);
-          m = mn;
-          l *= c;
-#pragma unroll
-          for (int db = 0; db < 4; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[db][i] *= c;
-        }
-        const float ms = m * kScaleLog2;
-        u32x4 p[4];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], kScaleLog2, -ms));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], kScaleLog2, -ms));
-            l += p0 + p1;
-            p[2 * kb + (i >> 3)][(i & 7) >> 1] = Elem::pack2(p0, p1);
-          }
-        auto value = [&](int c, int db) {  // V^T's operand: 16 keys from 16 c on, dims 32 db + lane % 32
-          typedef __attribute__((address_space(3))) s16x4* Lds;
-          const uint8_t* at = vt + (vsrc ^ (db << 6)) + c * 16 * kRowBytes;
-          const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at));
-          const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 8 * kRowBytes)));
-          return u32x4{v0[0], v0[1], v1[0], v1[1]};
-        };
-        auto pv = [&](auto clean) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int db = 0; db < 4; ++db) {
-              if constexpr (decltype(clean)::value) __builtin_amdgcn_sched_barrier(0);
-              u32x4 x = value(c, db);
-              if constexpr (decltype(clean)::value) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = drop_nonfinite<Elem>(x[i]);
-              }
-              o[db] = Elem::mma(x, p[c], o[db]);
-            }
-        };
-        if (decltype(careful)::value && diagonal) {
-          pv(std::true_type{});
-          // How many +inf and -inf (a NaN is both) each row sees in each dim, as products too.
-          u32x4 see[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int key = k0 + 16 * c + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
-              see[c][i] = (key <= tok ? Elem::kOne : 0u) | (key + 1 <= tok ? Elem::kOne << 16 : 0u);
-            }
-#pragma unroll
-          for (int db = 0; db < 4; ++db) {
-            f32x16 up = {}, down = {};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
-              const u32x4 x = value(c, db);
-              u32x4 xu, xd;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint2 n = infinities<Elem>(x[i]);
-                xu[i] = n.x, xd[i] = n.y;
-              }
-              up = Elem::mma(xu, see[c], up);
-              down = Elem::mma(xd, see[c], down);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              o[db][i] += (up[i] > 0.f ? INFINITY : 0.f) + (down[i] > 0.f ? -INFINITY : 0.f);
-          }
-        } else {
-          pv(std::false_type{});
-        }
+    if constexpr (decltype(careful)::value) {
+      for (int tile = 0; tile < tiles; ++tile) step(tile, tile % kBuffers, careful);
+    } else {  // places in LDS known at compile time: no address arithmetic
+      for (int tile = 0; tile < tiles; tile += kBuffers) {
+        step(tile, 0, careful);
+        if (tile + 1 >= tiles) break;
+        step(tile + 1, 1, careful);
+        if (tile + 2 >= tiles) break;
+        step(tile + 2, 2, careful);
       }
-      landed();
-      __syncthreads();
     }
   };
   sweep(std::false_type{});
@@ -332,15 +357,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prefill_kernel(PrefillArgs a) 
     for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(o[db][i], 0.f, zero);
   if (__syncthreads_or(zero != 0.f)) sweep(std::true_type{});
 
-  if (row0 + col >= rows) return;
+  // The wave's 32 rows pass through LDS, so that 16 lanes write one row of 256 bytes; 16-byte
+  // chunks lie under an exclusive or with the row.
   const float inv = 1.0f / (l + __shfl_xor(l, 32));
-  uint8_t* out = a.output + ((start + (long)tok) * a.hq + head) * kRowBytes + half * 8;
+  uint8_t* const mine = lds + wave * kWaveRows * kRowBytes;
 #pragma unroll
   for (int db = 0; db < 4; ++db)
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
-      *(u32x2*)(out + db * 64 + i * 4) = u32x2{Elem::pack2(o[db][i] * inv, o[db][i + 1] * inv),
-                                               Elem::pack2(o[db][i + 2] * inv, o[db][i + 3] * inv)};
+      *(u32x2*)(mine + col * kRowBytes + (((4 * db + (i >> 2)) ^ (col & 15)) << 4) + 8 * half) =
+          u32x2{Elem::pack2(o[db][i] * inv, o[db][i + 1] * inv), Elem::pack2(o[db][i + 2] * inv, o[db][i + 3] * inv)};
+#pragma unroll
+  for (int i = 0; i < kWaveRows / 4; ++i) {
+    const int r = 4 * i + (lane >> 4);
+    if (row0 + r < rows) {
+      const int t = (row0 + r) / a.group;
+      *(u32x4*)(a.output + ((start + (long)t) * a.hq + kvh * a.group + (row0 + r - t * a.group)) * kRowBytes + (lane & 15) * 16) =
+          *(const u32x4*)(mine + r * kRowBytes + (((lane & 15) ^ (r & 15)) << 4));
+    }
+  }
 }
 
 }  // namespace

@@ -29,7 +29,8 @@ def attention_tolerance(out, weight, score, tokens, dtype, p_step, tiny):
     * The output's rounding: half a step of its type, and below its normal range half a step of
       the subnormals, which are 2^-24 apart in fp16 and 2^-133 in bf16.
     * Weights p_j enter the product with V rounded to `p_step` relative (half a step of the
-      product's operands), against a sum of unrounded weights: p_step * sum p_j |v_j|.
+      product's operands): p_step * sum p_j |v_j| in the numerator, and at most p_step * |out|
+      more where the sum is of the rounded weights.
     * A score is a sum of 128 products in 32 bits, off by at most 128 * 2^-24 * sum |q k| /
       sqrt(128) (order free), and then scaled, shifted and exponentiated with a few more
       roundings of values of up to |x| + 100 in log2: delta.  Relative errors of the weights of
@@ -41,7 +42,7 @@ def attention_tolerance(out, weight, score, tokens, dtype, p_step, tiny):
     delta = 130 * F32 * score[..., None] + 64 * F32 * (1 + score[..., None]) + 200 * F32
     sums = 2 * (tokens + 16) * F32
     least = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}[dtype]
-    return U[dtype] * np.abs(out) + least + (1 + U[dtype]) * ((p_step + 2 * delta + sums) * weight + tiny)
+    return U[dtype] * np.abs(out) + least + (1 + U[dtype]) * ((p_step + 2 * delta + sums) * weight + p_step * np.abs(out) + tiny)
 
 
 def assert_within(got, want, bound, what=""):

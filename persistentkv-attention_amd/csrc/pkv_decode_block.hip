@@ -41,7 +41,8 @@ constexpr int kWaves = 4;            // per workgroup, one workgroup per CU
 constexpr int kPieceCost = 2;        // positions that a pair's start counts for
 constexpr int kMinShare = 2;         // positions of a share
 constexpr int kMaxRows = 16000;      // an LDS prefix of 4 bytes a row
-constexpr int kStateFloats = kD + 2; // m, l, acc
+constexpr int kStateFloats = kD + 2; // acc, m, l
+constexpr int kMergeWaves = 4;
 constexpr int kKvLoadPolicy = 2;     // non-temporal: K/V bytes are read once
 constexpr uint32_t kRsrcWord3 = 0x00020000u;  // raw buffer, 32-bit data format (gfx9 family)
 constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
@@ -96,7 +97,8 @@ struct BlockArgs {
   const int32_t* block_table; // [B, max_pages]
   const int32_t* seq_lens;    // [B]
   uint8_t* output;            // [B, Hq, 128]
-  float* states;              // [2 * waves, G, 130]
+  float* acc;                 // [2 * waves, G, 128] partial states: sum 2^(y - m) v8,
+  f32x2* ml;                  // [2 * waves, G] m, and sum 2^(y - m) / vs
   int2* plan;                 // [B * Hkv] first and last wave of the pair (first > last: empty)
   int32_t batch, hkv, group, num_pages, page_size, page_shift, max_pages, waves;
 };
@@ -320,13 +322,14 @@ __device__ void piece(const BlockArgs& a, int row, int kvh, int t0, int t1, int 
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[i] = pack8<Elem>(st.o[hb], i, inv);
     } else {
-      float* s = a.states + ((long)state * a.group + head) * kStateFloats;
-      if (g == 0) s[0] = st.m[hb], s[1] = l;
-      float* acc = s + 2 + g * 32;
+      const long at = (long)state * a.group + head;
+      if (g == 0) a.ml[at] = f32x2{st.m[hb], l};
+      f32x4* acc = (f32x4*)(a.acc + at * kD + g * 32);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int jj = 0; jj < 8; jj += 2) *(f32x2*)(acc + 8 * i + jj) = f32x2{st.o[hb][jj][i], st.o[hb][jj + 1][i]};
+        for (int jj = 0; jj < 8; jj += 4)
+          acc[2 * i + jj / 4] = f32x4{st.o[hb][jj][i], st.o[hb][jj + 1][i], st.o[hb][jj + 2][i], st.o[hb][jj + 3][i]};
     }
   }
 }
@@ -401,32 +404,63 @@ __global__ __launch_bounds__(kWaves * 64) void decode_block_kernel(BlockArgs a) 
   }
 }
 
-// One wave joins the partial states of one (pair, head); an empty row's output is zero.
+// Joins the partial states of one (pair, head); an empty row's output is zero.  Every wave
+// computes the states' weights 2^(m - M) for itself, a state a lane; then half a wave reads one
+// state's 512 bytes of sums, so that a workgroup has 8 states in flight in each of kUnroll steps.
+// (One wave a head, a state after another, took 10 to 22 us where this takes 3 to 5.)
 template <class Elem>
-__global__ __launch_bounds__(256) void merge_block_kernel(BlockArgs a) {
-  const int id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (id >= a.batch * a.hkv * a.group) return;
+__global__ __launch_bounds__(kMergeWaves * 64) void merge_block_kernel(BlockArgs a) {
+  constexpr int kUnroll = 4, kHalves = 2 * kMergeWaves;
+  __shared__ f32x4 part[kHalves][kD / 4];
+  const int id = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int pair = id / a.group, head = id - pair * a.group;
   const int2 p = a.plan[pair];
-  uint32_t* out = (uint32_t*)(a.output + (long)id * (2 * kD)) + lane;
+  uint8_t* const out = a.output + (long)id * (2 * kD);
+  if (p.x == p.y) return;
   if (p.x > p.y) {
-    *out = 0;
+    if (tid < kD / 4) *(u32x2*)(out + tid * 8) = u32x2{0, 0};
     return;
   }
-  if (p.x == p.y) return;
-  float m = -INFINITY, l = 0.f;
-  f32x2 acc = {0.f, 0.f};
-  for (int w = p.x; w <= p.y; ++w) {
-    const float* s = a.states + ((long)(2 * w + (w == p.x ? 1 : 0)) * a.group + head) * kStateFloats;
-    const float mw = s[0], lw = s[1];
-    const f32x2 aw = *(const f32x2*)(s + 2 + 2 * lane);
-    const float mn = fmaxf(m, mw);
-    const float c = __builtin_amdgcn_exp2f(m - mn), cw = __builtin_amdgcn_exp2f(mw - mn);
-    l = l * c + lw * cw;
-    acc = acc * c + aw * cw;
-    m = mn;
+  const int n = p.y - p.x + 1;  // state i is wave p.x + i's: its last piece for i = 0, else its first
+  auto state = [&](int i) { return (long)(2 * (p.x + i) + (i == 0 ? 1 : 0)) * a.group + head; };
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, a.ml[state(i)][0]);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  float l = 0.f;
+  for (int i = lane; i < n; i += 64) {
+    const f32x2 x = a.ml[state(i)];
+    l = __builtin_fmaf(x[1], __builtin_amdgcn_exp2f(x[0] - m), l);
   }
-  *out = Elem::pack2(acc[0] / l, acc[1] / l);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+  const int half = tid >> 5, c = tid & 31;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = half; i0 < n; i0 += kHalves * kUnroll) {
+    f32x4 x[kUnroll];
+    float w[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = min(i0 + u * kHalves, n - 1);
+      x[u] = *(const f32x4*)(a.acc + state(i) * kD + 4 * c);
+      w[u] = a.ml[state(i)][0];
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i0 + u * kHalves < n) {
+        const float f = __builtin_amdgcn_exp2f(w[u] - m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(x[u][j], f, acc[j]);
+      }
+  }
+  part[half][c] = acc;
+  __syncthreads();
+  if (tid < kD / 4) {
+    f32x4 sum = part[0][tid];
+#pragma unroll
+    for (int h = 1; h < kHalves; ++h) sum += part[h][tid];
+    *(u32x2*)(out + tid * 8) = u32x2{Elem::pack2(sum[0] / l, sum[1] / l), Elem::pack2(sum[2] / l, sum[3] / l)};
+  }
 }
 
 int compute_units() {
@@ -447,7 +481,7 @@ void launch(const BlockArgs& a, hipStream_t s) {
   const size_t lds = (size_t)(a.batch + 1 + kWaves) * sizeof(uint32_t);
   decode_block_kernel<Elem, HB><<<dim3((unsigned)(a.waves / kWaves)), dim3(kWaves * 64), lds, s>>>(a);
   const long heads = (long)a.batch * a.hkv * a.group;
-  merge_block_kernel<Elem><<<dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s>>>(a);
+  merge_block_kernel<Elem><<<dim3((unsigned)heads), dim3(kMergeWaves * 64), 0, s>>>(a);
 }
 
 }  // namespace
@@ -507,7 +541,8 @@ int pkv_paged_attention_fp8_block(
   a.block_table = block_table;
   a.seq_lens = seq_lens;
   a.output = (uint8_t*)output;
-  a.states = (float*)workspace;
+  a.acc = (float*)workspace;
+  a.ml = (f32x2*)(a.acc + 2 * (size_t)waves * group * kD);
   a.plan = (int2*)((uint8_t*)workspace + need - (size_t)batch * num_kv_heads * sizeof(int2));
   a.batch = batch;
   a.hkv = num_kv_heads;

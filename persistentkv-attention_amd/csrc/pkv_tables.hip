@@ -44,14 +44,32 @@ struct TableArgs {
   int32_t* slot_mapping;       // [slots]
   int32_t* num_free_out;       // [1]
   int32_t batch, free_capacity, max_pages, slots, page_size;
+  int32_t page_shift;  // log2(page_size), or -1
 };
 
 // Sums that stop at 2^31 - 1 (addends of at most that much each; associative).
 __device__ inline uint32_t add_sat(uint32_t a, uint32_t b) { return min(a + b, kTop); }
 
+__device__ inline int page_index(const TableArgs& a, int token) {
+  return a.page_shift >= 0 ? token >> a.page_shift : token / a.page_size;
+}
 __device__ inline int pages_of(const TableArgs& a, int tokens) {
-  const int p = tokens / a.page_size + (tokens % a.page_size != 0);
-  return min(p, a.max_pages);
+  const int p = page_index(a, tokens);
+  return min(p + (p * a.page_size < tokens), a.max_pages);
+}
+
+// Inclusive saturating sum over the wave by DPP: within rows of 16 lanes, then across them.
+template <int CTRL, int ROW_MASK>
+__device__ inline uint32_t dpp_add_sat(uint32_t x) {
+  return add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROW_MASK, 0xf, false));
+}
+__device__ inline uint32_t wave_scan(uint32_t x) {
+  x = dpp_add_sat<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = dpp_add_sat<0x112, 0xf>(x);
+  x = dpp_add_sat<0x114, 0xf>(x);
+  x = dpp_add_sat<0x118, 0xf>(x);
+  x = dpp_add_sat<0x142, 0xa>(x);  // row_bcast 15, 31
+  return dpp_add_sat<0x143, 0xc>(x);
 }
 
 __device__ inline void row_counts(const TableArgs& a, int row, uint32_t& tokens, uint32_t& pages) {
@@ -60,16 +78,20 @@ __device__ inline void row_counts(const TableArgs& a, int row, uint32_t& tokens,
   pages = (uint32_t)(pages_of(a, len) - pages_of(a, cached));
 }
 
-// The last row whose prefix is at most x (rows without elements share their successor's
-// prefix and are passed over); prefix has n + 1 entries and prefix[n] > x.
-__device__ inline int row_of(const uint32_t* prefix, int n, uint32_t x) {
-  int lo = 0, hi = n;  // prefix[lo] <= x < prefix[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= x) lo = mid;
-    else hi = mid;
+// For N values x at once: the last row whose prefix is at most x (rows without elements share
+// their successor's prefix and are passed over).  `top`: the largest power of two below n,
+// or 0; the steps of the N bisections are independent LDS reads.
+template <int N>
+__device__ inline void rows_of(const uint32_t* prefix, int n, int top, const uint32_t (&x)[N], int (&row)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) row[i] = 0;
+  for (int step = top; step; step >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = row[i] + step;
+      if (at < n && prefix[at] <= x[i]) row[i] = at;
+    }
   }
-  return lo;
 }
 
 __global__ __launch_bounds__(kThreads) void tables_kernel(TableArgs a) {
@@ -78,18 +100,14 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(TableArgs a) {
   uint32_t* const pag = lds + a.batch + 1;      // [B + 1] exclusive prefix of new pages
   uint32_t* const sums = pag + a.batch + 1;     // [2 * kWaves]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int avail = min(max(*a.num_free, 0), a.free_capacity);
 
   uint32_t tok0 = 0, pag0 = 0;
   for (int base = 0; base < a.batch; base += kThreads) {
     const int row = base + tid;
     uint32_t t = 0, p = 0;
     if (row < a.batch) row_counts(a, row, t, p);
-    uint32_t ti = t, pi = p;  // inclusive over the wave
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t tu = __shfl_up(ti, d), pu = __shfl_up(pi, d);
-      if (lane >= d) ti = add_sat(ti, tu), pi = add_sat(pi, pu);
-    }
+    const uint32_t ti = wave_scan(t), pi = wave_scan(p);
     if (lane == 63) sums[wave] = ti, sums[kWaves + wave] = pi;
     __syncthreads();
     uint32_t tw = tok0, pw = pag0;
@@ -107,7 +125,6 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(TableArgs a) {
   if (tid == 0) tok[0] = 0, pag[0] = 0;
   __syncthreads();
 
-  const int avail = min(max(*a.num_free, 0), a.free_capacity);
   const uint32_t total_tok = tok[a.batch], total_pag = pag[a.batch];
   const uint32_t gid = blockIdx.x * kThreads + tid, threads = gridDim.x * kThreads;
 
@@ -115,38 +132,44 @@ __global__ __launch_bounds__(kThreads) void tables_kernel(TableArgs a) {
   if (gid == 0) {
     *a.num_free_out = avail - (int32_t)total_pag;  // at least -(2^31 - 1)
   }
+  const int top = a.batch > 1 ? 1 << (31 - __builtin_clz(a.batch - 1)) : 0;
   // The new pages of the table rows.
   for (uint32_t r = gid; r < total_pag; r += threads) {
-    const int row = row_of(pag, a.batch, r);
-    const int held = pages_of(a, max(a.cached_lens[row], 0));
+    int row[1];
+    rows_of<1>(pag, a.batch, top, {r}, row);
+    const int held = pages_of(a, max(a.cached_lens[row[0]], 0));
     const long at = (long)avail - 1 - (long)r;
-    a.block_table[(long)row * a.max_pages + held + (int)(r - pag[row])] = at >= 0 ? a.free_pages[at] : -1;
+    a.block_table[(long)row[0] * a.max_pages + held + (int)(r - pag[row[0]])] = at >= 0 ? a.free_pages[at] : -1;
   }
   // The slots.  A new page's id comes from the list, not from the table, whose new entries
   // another workgroup may not have written yet.
-  for (uint32_t t0 = gid * kTokensPerThread; t0 < (uint32_t)a.slots; t0 += threads * kTokensPerThread) {
+  for (uint32_t base = blockIdx.x * kThreads * kTokensPerThread; base < (uint32_t)a.slots;
+       base += threads * kTokensPerThread) {
+    uint32_t t[kTokensPerThread];
+    int row[kTokensPerThread], slot[kTokensPerThread];
 #pragma unroll
-    for (uint32_t i = 0; i < kTokensPerThread; ++i) {
-      const uint32_t t = t0 + i;
-      int32_t slot = -1;
-      if (t < total_tok) {
-        const int row = row_of(tok, a.batch, t);
-        const int cached = max(a.cached_lens[row], 0);
-        const int pos = cached + (int)(t - tok[row]);
-        const int logical = pos / a.page_size, held = pages_of(a, cached);
+    for (int i = 0; i < kTokensPerThread; ++i) t[i] = base + i * kThreads + tid;
+    rows_of<kTokensPerThread>(tok, a.batch, top, t, row);
+#pragma unroll
+    for (int i = 0; i < kTokensPerThread; ++i) {
+      slot[i] = -1;
+      if (t[i] < min(total_tok, (uint32_t)a.slots)) {
+        const int cached = max(a.cached_lens[row[i]], 0);
+        const int pos = cached + (int)(t[i] - tok[row[i]]);
+        const int logical = page_index(a, pos), held = pages_of(a, cached);
         if (logical < a.max_pages) {
-          int page = -1;
-          if (logical < held) page = a.block_table[(long)row * a.max_pages + logical];
-          else {
-            const long at = (long)avail - 1 - (long)pag[row] - (logical - held);
-            if (at >= 0) page = a.free_pages[at];
-          }
+          const long at = (long)avail - 1 - (long)pag[row[i]] - (logical - held);
+          const int32_t* p = logical < held ? a.block_table + (long)row[i] * a.max_pages + logical
+                                            : a.free_pages + at;
+          const int page = logical < held || at >= 0 ? *p : -1;
           const long s = (long)page * a.page_size + (pos - logical * a.page_size);
-          if (page >= 0 && s <= INT32_MAX) slot = (int32_t)s;
+          if (page >= 0 && s <= INT32_MAX) slot[i] = (int32_t)s;
         }
       }
-      if (t < (uint32_t)a.slots) a.slot_mapping[t] = slot;
     }
+#pragma unroll
+    for (int i = 0; i < kTokensPerThread; ++i)
+      if (t[i] < (uint32_t)a.slots) a.slot_mapping[t[i]] = slot[i];
   }
 }
 
@@ -171,7 +194,8 @@ extern "C" int pkv_build_block_tables(
   if (num_free == num_free_out)
     return fail(PKV_ERR_INVALID_ARGUMENT, "build_block_tables: num_free_out must not be num_free");
   const TableArgs a{cached_lens, seq_lens, free_pages, num_free, block_table, token_offsets,
-                    slot_mapping, num_free_out, batch, free_capacity, max_pages, slots, page_size};
+                    slot_mapping, num_free_out, batch, free_capacity, max_pages, slots, page_size,
+                    (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1};
   const long work = (long)(slots > batch ? slots : batch);
   long groups = (work + kThreads * kTokensPerThread - 1) / (kThreads * kTokensPerThread);
   groups = groups < 1 ? 1 : groups > 1024 ? 1024 : groups;

@@ -143,62 +143,102 @@ __device__ inline void rescale_rows(uint8_t* block, int rows, float r, int lane)
   }
 }
 
-// One wave writes one run: `count` tokens from t0 on, in consecutive slots of one page.
-template <bool BF16>
+// One wave writes one run: `count` tokens from t0 on, in consecutive slots of one page.  Up to
+// 16 * CHUNKS tokens stay in registers between the search for the largest magnitude and the
+// rounding (all of their loads are in flight at once); those of longer runs are read again.
+template <bool BF16, int CHUNKS>
 __device__ void write_run(const WriteArgs& a, int t0, int count, int page, int off, int h, int lane) {
+  constexpr int kRows = 4 * CHUNKS;  // registers' rows of four tokens
   const long block = (long)page * a.hkv + h;
   float* const scales = a.kv_scales + 2 * block;
-  const long from = (long)h * kRowBytes + (lane & 15) * 16;
+  const int sub = lane >> 4;
+  const uint8_t* const kn = a.k_new + t0 * a.k_stride + (long)h * kRowBytes + (lane & 15) * 16;
+  const uint8_t* const vn = a.v_new + t0 * a.v_stride + (long)h * kRowBytes + (lane & 15) * 16;
+  f32x2 old = {1.f, 1.f};
+  if (off > 0) old = *(const f32x2*)scales;
+  u32x4 k[kRows], v[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int t = 4 * i + sub;
+    if (t < count) {
+      k[i] = *(const u32x4*)(kn + t * a.k_stride);
+      v[i] = *(const u32x4*)(vn + t * a.v_stride);
+    } else {
+      k[i] = v[i] = u32x4{0, 0, 0, 0};
+    }
+  }
   uint32_t mk = 0, mv = 0;
-  for (int t = lane >> 4; t < count; t += 4) {
-    mk = finite_max<BF16>(mk, *(const u32x4*)(a.k_new + (t0 + t) * a.k_stride + from));
-    mv = finite_max<BF16>(mv, *(const u32x4*)(a.v_new + (t0 + t) * a.v_stride + from));
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) mk = finite_max<BF16>(mk, k[i]), mv = finite_max<BF16>(mv, v[i]);
+  for (int t = 4 * kRows + sub; t < count; t += 4) {
+    mk = finite_max<BF16>(mk, *(const u32x4*)(kn + t * a.k_stride));
+    mv = finite_max<BF16>(mv, *(const u32x4*)(vn + t * a.v_stride));
   }
   int ek = scale_exponent(wave_amax<BF16>(mk)), ev = scale_exponent(wave_amax<BF16>(mv));
   uint8_t* const kb = a.k_pages + block * a.page_size * kD;
   uint8_t* const vb = a.v_pages + block * a.page_size * kD;
   if (off > 0) {  // earlier tokens share the block: its scales can only grow
     const float lo = pow2(-kScaleExp), hi = pow2(kScaleExp);
-    const float ks = fminf(fmaxf(scales[0], lo), hi), vs = fminf(fmaxf(scales[1], lo), hi);
+    const float ks = fminf(fmaxf(old[0], lo), hi), vs = fminf(fmaxf(old[1], lo), hi);
     ek = max(ek, old_exponent(ks));
     ev = max(ev, old_exponent(vs));
     if (ks != pow2(ek)) rescale_rows(kb, off, ks * pow2(-ek), lane);
     if (vs != pow2(ev)) rescale_rows(vb, off, vs * pow2(-ev), lane);
   }
   const float ik = pow2(-ek), iv = pow2(-ev);
-  for (int t = lane >> 4; t < count; t += 4) {
-    const long to = (long)(off + t) * kD + (lane & 15) * 8;
-    *(u32x2*)(kb + to) = encode8<BF16>(*(const u32x4*)(a.k_new + (t0 + t) * a.k_stride + from), ik);
-    *(u32x2*)(vb + to) = encode8<BF16>(*(const u32x4*)(a.v_new + (t0 + t) * a.v_stride + from), iv);
+  const long to = (long)off * kD + (lane & 15) * 8;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int t = 4 * i + sub;
+    if (t < count) {
+      *(u32x2*)(kb + to + t * kD) = encode8<BF16>(k[i], ik);
+      *(u32x2*)(vb + to + t * kD) = encode8<BF16>(v[i], iv);
+    }
+  }
+  for (int t = 4 * kRows + sub; t < count; t += 4) {
+    *(u32x2*)(kb + to + (long)t * kD) = encode8<BF16>(*(const u32x4*)(kn + t * a.k_stride), ik);
+    *(u32x2*)(vb + to + (long)t * kD) = encode8<BF16>(*(const u32x4*)(vn + t * a.v_stride), iv);
   }
   if (lane == 0) *(f32x2*)scales = f32x2{pow2(ek), pow2(ev)};
 }
 
-// A wave takes the runs that begin in its `window` tokens, for one head.
-template <bool BF16>
+// A wave takes the runs that begin in its `window` (at most 16) tokens, for one head.  Its
+// lanes hold the slots of 64 tokens from the one before the window on.
+template <bool BF16, int CHUNKS>
 __global__ __launch_bounds__(256) void write_block_kernel(WriteArgs a, int window) {
   const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane((int)(id / a.hkv));
   const int h = __builtin_amdgcn_readfirstlane((int)(id - (long)w * a.hkv));
   const int first = (int)min((long)w * window, (long)a.tokens);
-  const int last = (int)min((long)first + window, (long)a.tokens);
-  for (int t = first; t < last; ++t) {
-    const int slot = a.slots[t];
-    if (slot < 0 || slot >= a.num_slots) continue;
-    const int page = slot / a.page_size, off = slot - page * a.page_size;
-    if (t > 0 && off > 0 && a.slots[t - 1] == slot - 1) continue;  // inside another run
-    const int most = min(a.page_size - off, a.tokens - t);
-    int count = 1;
-    for (bool more = true; more && count < most;) {  // slots that follow one another
-      const int i = count + lane;
-      const bool in = i < most && a.slots[t + i] == slot + i;
-      const uint64_t out = ~__builtin_amdgcn_ballot_w64(in);
-      const int n = out ? __builtin_ctzll(out) : 64;
-      count += n;
-      more = n == 64;
+  const int t = first - 1 + lane;
+  const int slot = t >= 0 && t < a.tokens ? a.slots[t] : -1;
+  const bool valid = slot >= 0 && slot < a.num_slots;
+  const int page = valid ? slot / a.page_size : 0, off = slot - page * a.page_size;
+  const int before = __shfl_up(slot, 1);  // by every lane: a lane out of step would read as 0
+  const bool follows = valid && off > 0 && lane > 0 && before == slot - 1;
+  const uint64_t joined = __builtin_amdgcn_ballot_w64(follows);
+  const uint64_t mine = ((1ull << window) - 1) << 1;  // lanes of the window's tokens
+  uint64_t starts = __builtin_amdgcn_ballot_w64(valid && !follows) & mine;
+  while (starts) {
+    const int i = __builtin_ctzll(starts);
+    starts &= starts - 1;
+    const int s0 = __builtin_amdgcn_readlane(slot, i), t0 = first - 1 + i;
+    const int p0 = __builtin_amdgcn_readlane(page, i), o0 = __builtin_amdgcn_readlane(off, i);
+    // 1 + the lanes behind lane i that follow one another; past lane 63, token by token.
+    const uint64_t after = i < 63 ? ~(joined >> (i + 1)) : 1;
+    int count = 1 + min(__builtin_ctzll(after | 1ull << (63 - i)), 63 - i);
+    if (i + count == 64) {
+      const int most = min(a.page_size - o0, a.tokens - t0);
+      for (bool more = true; more && count < most;) {
+        const int j = count + lane;
+        const uint64_t out = ~__builtin_amdgcn_ballot_w64(j < most && a.slots[t0 + j] == s0 + j);
+        const int n = out ? __builtin_ctzll(out) : 64;
+        count += n;
+        more = n == 64;
+      }
     }
-    write_run<BF16>(a, t, count, page, off, h, lane);
+    write_run<BF16, CHUNKS>(a, t0, count, p0, o0, h, lane);
   }
 }
 
@@ -264,8 +304,12 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
   const int window = (long)tokens * num_kv_heads <= 16384 ? 1 : 16;
   const long waves = (long)((tokens + window - 1) / window) * num_kv_heads;
   const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
-  if (dtype == PKV_DTYPE_BF16) write_block_kernel<true><<<grid, block, 0, (hipStream_t)stream>>>(a, window);
-  else write_block_kernel<false><<<grid, block, 0, (hipStream_t)stream>>>(a, window);
+  const bool bf16 = dtype == PKV_DTYPE_BF16;
+  const int chunks = page_size <= 16 || window == 1 ? 1 : page_size <= 32 ? 2 : 4;
+  auto* const kernel = chunks == 1 ? (bf16 ? write_block_kernel<true, 1> : write_block_kernel<false, 1>)
+                     : chunks == 2 ? (bf16 ? write_block_kernel<true, 2> : write_block_kernel<false, 2>)
+                                   : (bf16 ? write_block_kernel<true, 4> : write_block_kernel<false, 4>);
+  kernel<<<grid, block, 0, (hipStream_t)stream>>>(a, window);
   return launched("write_kv_fp8_block");
 }
 

@@ -423,28 +423,34 @@ __global__ __launch_bounds__(kMergeWaves * 64) void merge_block_kernel(BlockArgs
   }
   const int n = p.y - p.x + 1;  // state i is wave p.x + i's: its last piece for i = 0, else its first
   auto state = [&](int i) { return (long)(2 * (p.x + i) + (i == 0 ? 1 : 0)) * a.group + head; };
+  // The sums' first loads go out before the maxima are known: only the pair's waves place them.
+  const int half = tid >> 5, c = tid & 31;
+  f32x4 x[kUnroll];
+  float w[kUnroll];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const long at = state(min(i0 + u * kHalves, n - 1));
+      x[u] = *(const f32x4*)(a.acc + at * kD + 4 * c);
+      w[u] = a.ml[at][0];
+    }
+  };
+  load(half);
   float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, a.ml[state(i)][0]);
+  const f32x2 own = lane < n ? a.ml[state(lane)] : f32x2{-INFINITY, 0.f};
+  for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, a.ml[state(i)][0]);
+  m = fmaxf(m, own[0]);
 #pragma unroll
   for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  float l = 0.f;
-  for (int i = lane; i < n; i += 64) {
-    const f32x2 x = a.ml[state(i)];
-    l = __builtin_fmaf(x[1], __builtin_amdgcn_exp2f(x[0] - m), l);
+  float l = own[1] * __builtin_amdgcn_exp2f(own[0] - m);
+  for (int i = lane + 64; i < n; i += 64) {
+    const f32x2 y = a.ml[state(i)];
+    l = __builtin_fmaf(y[1], __builtin_amdgcn_exp2f(y[0] - m), l);
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
-  const int half = tid >> 5, c = tid & 31;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = half; i0 < n; i0 += kHalves * kUnroll) {
-    f32x4 x[kUnroll];
-    float w[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = min(i0 + u * kHalves, n - 1);
-      x[u] = *(const f32x4*)(a.acc + state(i) * kD + 4 * c);
-      w[u] = a.ml[state(i)][0];
-    }
+  for (int i0 = half;;) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (i0 + u * kHalves < n) {
@@ -452,6 +458,9 @@ __global__ __launch_bounds__(kMergeWaves * 64) void merge_block_kernel(BlockArgs
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(x[u][j], f, acc[j]);
       }
+    i0 += kHalves * kUnroll;
+    if (i0 >= n) break;
+    load(i0);
   }
   part[half][c] = acc;
   __syncthreads();

@@ -61,8 +61,15 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 struct Half {
   static constexpr uint32_t kExponentStep = 0x04000400u;  // one step of both halves' exponents
   static constexpr uint32_t kOne = 0x3c00u;
+  __device__ static inline float widen(uint32_t x2, bool high) {
+    return (float)__builtin_bit_cast(f16x2, x2)[high];
+  }
+  // c plus both halves; c where both are finite, else NaN.
   __device__ static inline float sum2(uint32_t x, float c) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, kOne * 0x10001u), c, false);
+  }
+  __device__ static inline float times0(uint32_t x, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), f16x2{0, 0}, c, false);
   }
   __device__ static inline f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
@@ -75,8 +82,14 @@ struct Half {
 struct BFloat {
   static constexpr uint32_t kExponentStep = 0x00800080u;
   static constexpr uint32_t kOne = 0x3f80u;
+  __device__ static inline float widen(uint32_t x2, bool high) {
+    return __uint_as_float(high ? x2 & 0xffff0000u : x2 << 16);
+  }
   __device__ static inline float sum2(uint32_t x, float c) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, kOne * 0x10001u), c, false);
+  }
+  __device__ static inline float times0(uint32_t x, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), bf16x2{0, 0}, c, false);
   }
   __device__ static inline f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
@@ -95,6 +108,7 @@ struct PrefillArgs {
   uint8_t* output;               // [T, Hq, 128]
   long q_stride, k_stride, v_stride;
   int32_t batch, tokens, hq, hkv, group;
+  float inv_group;
 };
 
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -107,10 +121,36 @@ __device__ inline void* uniform_ptr(const void* p) {
 __device__ inline int offset_of(const PrefillArgs& a, int b) {
   return min(max(a.token_offsets[b], 0), a.tokens);
 }
-// First workgroup slot of sequence b, from its offset.  Its rows start at x = offset * G; the slots
-// from x / kRows + b on, up to the next sequence's, are at least as many as its blocks of rows.
-__device__ inline int first_slot(const PrefillArgs& a, int offset, int b) {
-  return (int)((uint32_t)(offset * a.group) / kRows) + b;
+__device__ inline int blocks_of(const PrefillArgs& a, int len) {
+  return (int)(((uint32_t)(len * a.group) + kRows - 1) / kRows);
+}
+
+// A block of rows: block `index` of the sequence of `len` tokens from `start` on.  index < 0: none.
+struct Block {
+  int start, len, index;
+};
+
+// The `slot`-th block: sequence after sequence, each with its longest block first.
+// Sequence b, whose rows start at x = offset * G, has the slots from x / kRows + b on, which
+// are, up to the next sequence's, at least as many as its blocks.  It is the last one whose
+// first slot is at most `slot`, found among 63 candidates at a time; the last round's lanes
+// hold its offset and its successor's.
+__device__ inline Block packed_order(const PrefillArgs& a, int slot, int lane) {
+  auto first_slot = [&](int offset, int b) { return (int)((uint32_t)(offset * a.group) / kRows) + b; };
+  int b = 0, n = a.batch, stride, offset, found;
+  do {
+    stride = (n + 62) / 63;
+    const int at = b + min(lane * stride, n);
+    offset = offset_of(a, min(at, a.batch));
+    const uint64_t fits = __builtin_amdgcn_ballot_w64(lane * stride < n && first_slot(offset, at) <= slot);
+    found = fits ? 63 - __builtin_clzll(fits) : 0;
+    b += found * stride;
+    n = min(stride, n - found * stride);
+  } while (stride > 1);
+  const int start = __builtin_amdgcn_readlane(offset, found);
+  const int len = max(__builtin_amdgcn_readlane(offset, found + 1) - start, 0);
+  const int blocks = blocks_of(a, len), index = blocks - 1 - (slot - first_slot(start, b));
+  return {start, len, index < blocks ? index : -1};
 }
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
@@ -142,14 +182,6 @@ __device__ inline uint32_t drop_nonfinite(uint32_t x2) {
   const uint32_t y = nonfinite_halves<Elem>(x2);
   return x2 & ~((y >> 15) * 0xffffu);
 }
-// 1 in the halves that are +inf (x) or -inf (y), in both for NaN; 0 elsewhere.
-template <class Elem>
-__device__ inline uint2 infinities(uint32_t x2) {
-  const uint32_t bad = nonfinite_halves<Elem>(x2);
-  const uint32_t nan = (x2 & 0x7fff7fffu) + (Elem::kExponentStep - 0x00010001u);  // top bits
-  return uint2{((bad & (~x2 | nan)) >> 15) * Elem::kOne, ((bad & (x2 | nan)) >> 15) * Elem::kOne};
-}
-
 template <class Elem>
 __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers * 2 * kTileBytes];  // K and V of each tile
@@ -157,65 +189,65 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
   const int col = lane & 31, half = lane >> 5;
   const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
   const int slot = uniform((int)(blockIdx.x / (unsigned)a.hkv));
-  // The last sequence whose first slot is at most `slot`, 63 candidates at a time; the last
-  // round's lanes hold its offset and its successor's.
-  int b = 0, n = a.batch, stride, offset, found;
-  do {
-    stride = (n + 62) / 63;
-    offset = offset_of(a, min(b + min(lane * stride, n), a.batch));
-    const uint64_t fits = __builtin_amdgcn_ballot_w64(lane * stride < n && first_slot(a, offset, b + lane * stride) <= slot);
-    found = fits ? 63 - __builtin_clzll(fits) : 0;
-    b += found * stride;
-    n = min(stride, n - found * stride);
-  } while (stride > 1);
-  const int start = __builtin_amdgcn_readlane(offset, found);
-  const int len = max(__builtin_amdgcn_readlane(offset, found + 1) - start, 0);
+  const Block work = packed_order(a, slot, lane);
+  if (work.index < 0) return;
+  const int start = uniform(work.start), len = uniform(work.len), block = uniform(work.index);
   const int rows = len * a.group;
-  const int blocks = (rows + kRows - 1) / kRows;
-  const int block = blocks - 1 - (slot - first_slot(a, start, b));  // the longest first
-  if (block < 0 || block >= blocks) return;  // a slot that no block of a sequence takes
 
-  const int row0 = block * kRows + wave * kWaveRows;
-  const int row = min(row0 + col, rows - 1);
-  const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
-  const int wave_first = uniform(min(row0, rows - 1) / a.group);
-  const int wave_last = uniform(min(row0 + kWaveRows - 1, rows - 1) / a.group);
-  const int last = uniform(min(block * kRows + kRows - 1, rows - 1) / a.group);
+  // Row row0 + r of the wave is token tok0 + (rem + r) / G: a quotient of numbers below 64, which
+  // the product with 1 / G in 32 bits gives exactly (it is off by less than 1 / (2 G)).
+  const int row0 = uniform(min(block * kRows + wave * kWaveRows, rows));
+  const int tok0 = row0 / a.group, rem = row0 - tok0 * a.group, live = rows - row0;  // may be 0
+  auto token_of = [&](int r) { return (int)(((float)(rem + r) + 0.5f) * a.inv_group); };
+  const int last_row = max(min(kWaveRows, live) - 1, 0);
+  const int r = min(col, last_row), dt = token_of(r), tok = tok0 + dt;
+  const int wave_first = tok0, wave_last = tok0 + uniform(token_of(last_row));
+  const int last = (min((block + 1) * kRows, rows) - 1) / a.group;
   const int tiles = last / kKeys + 1;
-
-  u32x4 q[8];
-  const uint8_t* qp = a.q + (start + (long)tok) * a.q_stride + (long)head * kRowBytes + half * 16;
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk) q[kk] = *(const u32x4*)(qp + kk * 32);
 
   // A wave moves rows 16 wave + 4 i + lane / 16 of a tile, 256 bytes a row.  16-byte chunk p of
   // row r in LDS is chunk p ^ r of K's row (p ^ 4 r of V's), so that reads of one chunk column
   // (K) or of 64 bytes of four rows (V) spread over all banks.
   const int srow = wave * (kKeys / kWaves) + (lane >> 4), chunk = lane & 15;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0] +
-                        (uint32_t)(wave * (kKeys / kWaves) * kRowBytes);
-  const uint8_t* kbase = a.k + (long)start * a.k_stride + (long)kvh * kRowBytes;
-  const uint8_t* vbase = a.v + (long)start * a.v_stride + (long)kvh * kRowBytes;
+  const uint32_t lds0 = (uint32_t)uniform((int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0] +
+                                                (uint32_t)(wave * (kKeys / kWaves) * kRowBytes)));
+  const uint8_t* const kbase = a.k + (long)start * a.k_stride + (long)kvh * kRowBytes;
+  const uint8_t* const vbase = a.v + (long)start * a.v_stride + (long)kvh * kRowBytes;
   const uint32_t koff = (uint32_t)(srow * (int)a.k_stride), kchunk = (chunk ^ (srow & 15)) << 4;
   const uint32_t voff = (uint32_t)(srow * (int)a.v_stride) + ((chunk ^ ((srow & 3) << 2)) << 4);
-  auto rsrc = [&](const uint8_t* base, long stride, int tile, int n) {
-    // Rows past the sequence's end read as zero: the descriptor ends with its last row.
-    const uint64_t at = (uint64_t)(base + (long)tile * kKeys * stride);
-    return i32x4{uniform((int)at), uniform((int)(at >> 32) & 0xffff),
-                 uniform((n - 1) * (int)stride + kRowBytes), (int)kRsrcWord3};
-  };
   constexpr int kLoads = kKeys / kWaves / 4;  // per wave and tile of K, and of V
-  auto fetch = [&](int tile, int buf) __attribute__((always_inline)) {
-    const int n = min(kKeys, len - tile * kKeys);
-    const i32x4 rk = rsrc(kbase, a.k_stride, tile, n), rv = rsrc(vbase, a.v_stride, tile, n);
-    const uint32_t to = (uint32_t)uniform((int)(lds0 + buf * 2 * kTileBytes));
+  // The next tile to fetch: where it lies, and the rows from it to the sequence's end.
+  uint64_t kp, vp;
+  int left;
+  auto fetch = [&](int buf) __attribute__((always_inline)) {
+    // Rows past the sequence's end read as zero: the descriptor ends with its last row.
+    const int n = min(kKeys, left) - 1;
+    const i32x4 rk{(int)kp, (int)(kp >> 32) & 0xffff, n * (int)a.k_stride + kRowBytes, (int)kRsrcWord3};
+    const i32x4 rv{(int)vp, (int)(vp >> 32) & 0xffff, n * (int)a.v_stride + kRowBytes, (int)kRsrcWord3};
+    const uint32_t to = lds0 + buf * 2 * kTileBytes;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       load_to_lds(to + i * 4 * kRowBytes, rk, koff + (kchunk ^ (i << 6)) + i * 4 * (uint32_t)a.k_stride);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       load_to_lds(to + kTileBytes + i * 4 * kRowBytes, rv, voff + i * 4 * (uint32_t)a.v_stride);
+    kp += (uint64_t)(kKeys * a.k_stride);
+    vp += (uint64_t)(kKeys * a.v_stride);
+    left -= kKeys;
   };
+  auto begin = [&]() __attribute__((always_inline)) {
+    kp = (uint64_t)uniform_ptr(kbase), vp = (uint64_t)uniform_ptr(vbase), left = len;
+    fetch(0);
+    if (tiles > 1) fetch(1);
+  };
+  begin();  // before Q's loads: nothing that waits for those comes between
+
+  u32x4 q[8];
+  const uint8_t* qp = a.q + (start + (long)min(tok, len - 1)) * a.q_stride +
+                      (long)(kvh * a.group + rem + r - dt * a.group) * kRowBytes + half * 16;
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) q[kk] = *(const u32x4*)(qp + kk * 32);
+
   // Reads: lane's K row (key col), chunk 2 kk + half; V rows 4 half + (lane % 16) / 4, four
   // dims from 32 db + 16 (lane / 16 % 2) + 4 (lane % 4) on.
   const uint32_t ksrc = col * kRowBytes + ((half ^ (col & 15)) << 4);
@@ -231,12 +263,32 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
 #pragma unroll
   for (int db = 0; db < 4; ++db) vat[db] = lds + kTileBytes + (vsrc ^ (db << 6));
 
-  // Tile `tile`, which lies in buffer `buf`; `careful`: see below.
-  auto step = [&](int tile, int buf, auto careful) __attribute__((always_inline)) {
+  // A masked weight is 0, and 0 times an infinity or NaN in V is NaN.  So where a row comes out
+  // not finite, its workgroup computes once more, `careful`: such values are taken out of the
+  // tiles that a row of it masks in part, those from `masked` on, and put back at the end for
+  // the rows from their token on.
+  bool careful = false;
+  const int masked = block * kRows / a.group / kKeys;
+  auto clean = [&](int buf) {
+    u32x4* const v = (u32x4*)(lds + buf * 2 * kTileBytes + kTileBytes) + tid;
+    for (int i = 0; i < kTileBytes / 16; i += kWaves * 64) {
+      u32x4 x = v[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = drop_nonfinite<Elem>(x[j]);
+      v[i] = x;
+    }
+    __syncthreads();
+  };
+
+  // Tile `tile`, which lies in buffer `buf`; `first`: tile 0, which sets the running maximum,
+  // sums and output.
+  auto step = [&](int tile, int buf, auto first) __attribute__((always_inline)) {
+    constexpr bool kFirst = decltype(first)::value;
     const int at = buf * 2 * kTileBytes;
-    if (tile + 2 < tiles) fetch(tile + 2, buf >= 1 ? buf - 1 : buf + 2);
+    if (careful && tile >= masked) clean(buf);
+    if (tile + 2 < tiles) fetch(buf >= 1 ? buf - 1 : buf + 2);
     const int k0 = tile * kKeys;
-    if (k0 <= wave_last) {
+    if (kFirst || k0 <= wave_last) {
       f32x16 s = {};
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) s = Elem::mma(*(const u32x4*)(kat[kk] + at), q[kk], s);
@@ -250,16 +302,19 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
       u32x4 v0[4];
 #pragma unroll
       for (int db = 0; db < 4; ++db) v0[db] = value(0, db);
-      const bool diagonal = k0 + kKeys - 1 > wave_first;
-      if (diagonal) {
+      if (k0 + kKeys - 1 > wave_first) {
+        const int visible = tok - k0 - 4 * half;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (k0 + 8 * (i >> 2) + 4 * half + (i & 3) > tok) s[i] = -INFINITY;
+          if (8 * (i >> 2) + (i & 3) > visible) s[i] = -INFINITY;
       }
       float mx = s[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+      if constexpr (kFirst) {
+        m = fmaxf(mx, __shfl_xor(mx, 32));
+        l = 0.f;
+      } else if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float mn = fmaxf(m, mx);
         const float c = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2);
@@ -279,102 +334,74 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
         p[i >> 3][(i & 7) >> 1] = x;
         l = Elem::sum2(x, l);
       }
-      if (decltype(careful)::value && diagonal) {
-        // How many +inf and -inf (a NaN is both) each row sees in each dim, as products too.
-        u32x4 see[2];
+      u32x4 v1[4];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = k0 + 16 * c + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
-            see[c][i] = (key <= tok ? Elem::kOne : 0u) | (key + 1 <= tok ? Elem::kOne << 16 : 0u);
-          }
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          f32x16 up = {}, down = {};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
-            u32x4 x = value(c, db), xu, xd;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint2 n = infinities<Elem>(x[i]);
-              xu[i] = n.x, xd[i] = n.y;
-              x[i] = drop_nonfinite<Elem>(x[i]);
-            }
-            up = Elem::mma(xu, see[c], up);
-            down = Elem::mma(xd, see[c], down);
-            o[db] = Elem::mma(x, p[c], o[db]);
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            o[db][i] += (up[i] > 0.f ? INFINITY : 0.f) + (down[i] > 0.f ? -INFINITY : 0.f);
-        }
-      } else {
-        u32x4 v1[4];
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          v1[db] = value(1, db);
-          o[db] = Elem::mma(v0[db], p[0], o[db]);
-        }
-#pragma unroll
-        for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v1[db], p[1], o[db]);
+      for (int db = 0; db < 4; ++db) {
+        v1[db] = value(1, db);
+        o[db] = Elem::mma(v0[db], p[0], kFirst ? f32x16{} : o[db]);
       }
+#pragma unroll
+      for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v1[db], p[1], o[db]);
     }
     // The next tile has landed, and behind the barrier this one's place is free.
     if (tile + 2 < tiles) landed<2 * kLoads>();
     else landed<0>();
     __syncthreads();
   };
-  auto sweep = [&](auto careful) __attribute__((always_inline)) {
-#pragma unroll
-    for (int db = 0; db < 4; ++db) o[db] = f32x16{};
-    m = -INFINITY, l = 0.f;
-    fetch(0, 0);
-    if (tiles > 1) fetch(1, 1);
+  u32x2 out[16];
+  for (;;) {
     landed<0>();
     __syncthreads();
-    if constexpr (decltype(careful)::value) {
-      for (int tile = 0; tile < tiles; ++tile) step(tile, tile % kBuffers, careful);
-    } else {  // places in LDS known at compile time: no address arithmetic
-      for (int tile = 0; tile < tiles; tile += kBuffers) {
-        step(tile, 0, careful);
-        if (tile + 1 >= tiles) break;
-        step(tile + 1, 1, careful);
-        if (tile + 2 >= tiles) break;
-        step(tile + 2, 2, careful);
+    step(0, 0, std::true_type{});
+    for (int tile = 1; tile < tiles; tile += kBuffers) {  // LDS places known at compile time
+      step(tile, 1, std::false_type{});
+      if (tile + 1 >= tiles) break;
+      step(tile + 1, 2, std::false_type{});
+      if (tile + 2 >= tiles) break;
+      step(tile + 2, 0, std::false_type{});
+    }
+    if (careful) {
+      for (int key = masked * kKeys; key <= tok; ++key) {
+        const u32x2* const x = (const u32x2*)(vbase + (long)key * a.v_stride) + half;
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float y = Elem::widen(x[2 * c][i >> 1], i & 1);
+            o[c >> 2][4 * (c & 3) + i] += __builtin_isfinite(y) ? 0.f : y;
+          }
       }
     }
-  };
-  sweep(std::false_type{});
-  // A masked weight is 0, and 0 times an infinity or NaN in V is NaN.  So where a row comes out
-  // not finite, its workgroup computes once more with such values taken out of the tiles that
-  // a row masks in part, and put back for the rows from their token on.
-  float zero = 0.f;
+    // The rows in the output's type; `zero` turns NaN where a value is not finite.
+    const float inv = 1.0f / (l + __shfl_xor(l, 32));
+    float zero = 0.f;
 #pragma unroll
-  for (int db = 0; db < 4; ++db)
+    for (int db = 0; db < 4; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(o[db][i], 0.f, zero);
-  if (__syncthreads_or(zero != 0.f)) sweep(std::true_type{});
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t x = Elem::pack2(o[db][i] * inv, o[db][i + 1] * inv);
+        out[4 * db + (i >> 2)][(i >> 1) & 1] = x;
+        zero = Elem::times0(x, zero);
+      }
+    if (careful || !__syncthreads_or(zero != 0.f)) break;
+    careful = true;
+    begin();
+  }
 
   // The wave's 32 rows pass through LDS, so that 16 lanes write one row of 256 bytes; 16-byte
   // chunks lie under an exclusive or with the row.
-  const float inv = 1.0f / (l + __shfl_xor(l, 32));
   uint8_t* const mine = lds + wave * kWaveRows * kRowBytes;
 #pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      *(u32x2*)(mine + col * kRowBytes + (((4 * db + (i >> 2)) ^ (col & 15)) << 4) + 8 * half) =
-          u32x2{Elem::pack2(o[db][i] * inv, o[db][i + 1] * inv), Elem::pack2(o[db][i + 2] * inv, o[db][i + 3] * inv)};
+  for (int c = 0; c < 16; ++c) *(u32x2*)(mine + col * kRowBytes + ((c ^ (col & 15)) << 4) + 8 * half) = out[c];
+  // Row R of the (sequence, KV head), a row of its token t, is row R + t (Hq - G) of the output.
+  uint8_t* const to = a.output + ((long)start * a.hq + kvh * a.group + row0 + (long)tok0 * (a.hq - a.group)) * kRowBytes +
+                      (lane & 15) * 16;
 #pragma unroll
   for (int i = 0; i < kWaveRows / 4; ++i) {
-    const int r = 4 * i + (lane >> 4);
-    if (row0 + r < rows) {
-      const int t = (row0 + r) / a.group;
-      *(u32x4*)(a.output + ((start + (long)t) * a.hq + kvh * a.group + (row0 + r - t * a.group)) * kRowBytes + (lane & 15) * 16) =
-          *(const u32x4*)(mine + r * kRowBytes + (((lane & 15) ^ (r & 15)) << 4));
-    }
+    const int j = 4 * i + (lane >> 4);
+    if (j < live)
+      *(u32x4*)(to + (long)(j + token_of(j) * (a.hq - a.group)) * kRowBytes) =
+          *(const u32x4*)(mine + j * kRowBytes + (((lane & 15) ^ (j & 15)) << 4));
   }
 }
 
@@ -412,7 +439,7 @@ extern "C" int pkv_prefill_attention(
     return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: tensors must be 16-byte aligned");
   const PrefillArgs a{(const uint8_t*)q, (const uint8_t*)k, (const uint8_t*)v, token_offsets,
                       (uint8_t*)output, 2 * q_stride, 2 * k_stride, 2 * v_stride,
-                      batch, tokens, num_q_heads, num_kv_heads, group};
+                      batch, tokens, num_q_heads, num_kv_heads, group, 1.0f / (float)group};
   const dim3 grid((unsigned)(slots * num_kv_heads)), threads(kWaves * 64);
   if (dtype == PKV_DTYPE_BF16) prefill_kernel<BFloat><<<grid, threads, 0, (hipStream_t)stream>>>(a);
   else prefill_kernel<Half><<<grid, threads, 0, (hipStream_t)stream>>>(a);

@@ -130,7 +130,51 @@ struct Block {
   int start, len, index;
 };
 
-// The `slot`-th block: sequence after sequence, each with its longest block first.
+template <int CTRL, int ROW_MASK>
+__device__ inline int from_lane(int x) {  // 0 where the lane has no source
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ inline int wave_scan(int x) {  // inclusive sums
+  x += from_lane<0x111, 0xf>(x);          // row_shr 1, 2, 4, 8: within 16 lanes
+  x += from_lane<0x112, 0xf>(x);
+  x += from_lane<0x114, 0xf>(x);
+  x += from_lane<0x118, 0xf>(x);
+  x += from_lane<0x142, 0xa>(x);          // row_bcast 15, 31
+  return x + from_lane<0x143, 0xc>(x);
+}
+__device__ inline int wave_max(int x) {  // of values that are not negative
+  x = max(x, from_lane<0x111, 0xf>(x));
+  x = max(x, from_lane<0x112, 0xf>(x));
+  x = max(x, from_lane<0x114, 0xf>(x));
+  x = max(x, from_lane<0x118, 0xf>(x));
+  x = max(x, from_lane<0x142, 0xa>(x));
+  return __builtin_amdgcn_readlane(max(x, from_lane<0x143, 0xc>(x)), 63);
+}
+
+// The `slot`-th block of up to 64 sequences: those longer than half the longest first, then
+// those longer than a quarter, an eighth, and the others; sequence after sequence in each
+// class, its longest block first.  So the blocks that start last, and that the GPU waits for
+// at the end, are short, and the blocks at work at one time still share their K/V in L2 (all
+// blocks by length would not: slower).
+__device__ inline Block by_length(const PrefillArgs& a, int slot, int lane) {
+  const int start = offset_of(a, min(lane, a.batch));
+  const int len = max(offset_of(a, min(lane + 1, a.batch)) - start, 0);
+  const int blocks = blocks_of(a, len), top = wave_max(blocks);
+  for (int k = 0; k < 4; ++k) {
+    const int n = blocks <= top >> k && (k == 3 || blocks > top >> (k + 1)) ? blocks : 0;
+    const int sums = wave_scan(n);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(sums > slot);
+    if (past) {
+      const int b = __builtin_ctzll(past);
+      return {__builtin_amdgcn_readlane(start, b), __builtin_amdgcn_readlane(len, b),
+              __builtin_amdgcn_readlane(sums, b) - 1 - slot};
+    }
+    slot -= __builtin_amdgcn_readlane(sums, 63);
+  }
+  return {0, 0, -1};
+}
+
+// The `slot`-th block of more sequences: sequence after sequence, its longest block first.
 // Sequence b, whose rows start at x = offset * G, has the slots from x / kRows + b on, which
 // are, up to the next sequence's, at least as many as its blocks.  It is the last one whose
 // first slot is at most `slot`, found among 63 candidates at a time; the last round's lanes
@@ -182,6 +226,7 @@ __device__ inline uint32_t drop_nonfinite(uint32_t x2) {
   const uint32_t y = nonfinite_halves<Elem>(x2);
   return x2 & ~((y >> 15) * 0xffffu);
 }
+
 template <class Elem>
 __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers * 2 * kTileBytes];  // K and V of each tile
@@ -189,7 +234,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
   const int col = lane & 31, half = lane >> 5;
   const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
   const int slot = uniform((int)(blockIdx.x / (unsigned)a.hkv));
-  const Block work = packed_order(a, slot, lane);
+  const Block work = a.batch <= 64 ? by_length(a, slot, lane) : packed_order(a, slot, lane);
   if (work.index < 0) return;
   const int start = uniform(work.start), len = uniform(work.len), block = uniform(work.index);
   const int rows = len * a.group;
@@ -200,8 +245,9 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
   const int tok0 = row0 / a.group, rem = row0 - tok0 * a.group, live = rows - row0;  // may be 0
   auto token_of = [&](int r) { return (int)(((float)(rem + r) + 0.5f) * a.inv_group); };
   const int last_row = max(min(kWaveRows, live) - 1, 0);
-  const int r = min(col, last_row), dt = token_of(r), tok = tok0 + dt;
-  const int wave_first = tok0, wave_last = tok0 + uniform(token_of(last_row));
+  const int r = min(col, last_row), dt = token_of(r);
+  const int tok = min(tok0 + dt, len - 1);  // a wave past the last row takes the last token's
+  const int wave_first = tok0, wave_last = live > 0 ? tok0 + uniform(token_of(last_row)) : -1;
   const int last = (min((block + 1) * kRows, rows) - 1) / a.group;
   const int tiles = last / kKeys + 1;
 
@@ -243,7 +289,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
   begin();  // before Q's loads: nothing that waits for those comes between
 
   u32x4 q[8];
-  const uint8_t* qp = a.q + (start + (long)min(tok, len - 1)) * a.q_stride +
+  const uint8_t* qp = a.q + (start + (long)tok) * a.q_stride +
                       (long)(kvh * a.group + rem + r - dt * a.group) * kRowBytes + half * 16;
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) q[kk] = *(const u32x4*)(qp + kk * 32);

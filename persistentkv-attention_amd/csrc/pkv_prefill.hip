@@ -37,11 +37,10 @@ namespace {
 constexpr int kD = 128;
 constexpr int kRowBytes = 2 * kD;
 constexpr int kKeys = 32;    // keys per tile
-constexpr int kBuffers = 3;  // tiles in LDS: one read, one landed, one on its way
 constexpr int kWaves = 4;
 constexpr int kWaveRows = 32;
-constexpr int kRows = kWaves * kWaveRows;
 constexpr int kTileBytes = kKeys * kRowBytes;
+constexpr int kBuffers = 3;  // tiles in LDS: one read, one landed, one on its way
 constexpr uint32_t kRsrcWord3 = 0x00020000u;  // raw buffer, 32-bit data format (gfx9 family)
 constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
 // The running maximum is replaced only when a score passes it by more than 2^8 in weight:
@@ -121,8 +120,9 @@ __device__ inline void* uniform_ptr(const void* p) {
 __device__ inline int offset_of(const PrefillArgs& a, int b) {
   return min(max(a.token_offsets[b], 0), a.tokens);
 }
+template <int ROWS>  // of a block
 __device__ inline int blocks_of(const PrefillArgs& a, int len) {
-  return (int)(((uint32_t)(len * a.group) + kRows - 1) / kRows);
+  return (int)(((uint32_t)(len * a.group) + ROWS - 1) / ROWS);
 }
 
 // A block of rows: block `index` of the sequence of `len` tokens from `start` on.  index < 0: none.
@@ -156,10 +156,11 @@ __device__ inline int wave_max(int x) {  // of values that are not negative
 // class, its longest block first.  So the blocks that start last, and that the GPU waits for
 // at the end, are short, and the blocks at work at one time still share their K/V in L2 (all
 // blocks by length would not: slower).
+template <int ROWS>
 __device__ inline Block by_length(const PrefillArgs& a, int slot, int lane) {
   const int start = offset_of(a, min(lane, a.batch));
   const int len = max(offset_of(a, min(lane + 1, a.batch)) - start, 0);
-  const int blocks = blocks_of(a, len), top = wave_max(blocks);
+  const int blocks = blocks_of<ROWS>(a, len), top = wave_max(blocks);
   for (int k = 0; k < 4; ++k) {
     const int n = blocks <= top >> k && (k == 3 || blocks > top >> (k + 1)) ? blocks : 0;
     const int sums = wave_scan(n);
@@ -175,12 +176,13 @@ __device__ inline Block by_length(const PrefillArgs& a, int slot, int lane) {
 }
 
 // The `slot`-th block of more sequences: sequence after sequence, its longest block first.
-// Sequence b, whose rows start at x = offset * G, has the slots from x / kRows + b on, which
+// Sequence b, whose rows start at x = offset * G, has the slots from x / ROWS + b on, which
 // are, up to the next sequence's, at least as many as its blocks.  It is the last one whose
 // first slot is at most `slot`, found among 63 candidates at a time; the last round's lanes
 // hold its offset and its successor's.
+template <int ROWS>
 __device__ inline Block packed_order(const PrefillArgs& a, int slot, int lane) {
-  auto first_slot = [&](int offset, int b) { return (int)((uint32_t)(offset * a.group) / kRows) + b; };
+  auto first_slot = [&](int offset, int b) { return (int)((uint32_t)(offset * a.group) / ROWS) + b; };
   int b = 0, n = a.batch, stride, offset, found;
   do {
     stride = (n + 62) / 63;
@@ -193,7 +195,7 @@ __device__ inline Block packed_order(const PrefillArgs& a, int slot, int lane) {
   } while (stride > 1);
   const int start = __builtin_amdgcn_readlane(offset, found);
   const int len = max(__builtin_amdgcn_readlane(offset, found + 1) - start, 0);
-  const int blocks = blocks_of(a, len), index = blocks - 1 - (slot - first_slot(start, b));
+  const int blocks = blocks_of<ROWS>(a, len), index = blocks - 1 - (slot - first_slot(start, b));
   return {start, len, index < blocks ? index : -1};
 }
 
@@ -227,14 +229,23 @@ __device__ inline uint32_t drop_nonfinite(uint32_t x2) {
   return x2 & ~((y >> 15) * 0xffffu);
 }
 
-template <class Elem>
-__global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers * 2 * kTileBytes];  // K and V of each tile
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// GROUPS = 2: two waves for 64 rows' even tiles and two for their odd ones, whose states are
+// joined at the end.  A step takes about 0.65 us however little the GPU has to do, so where
+// blocks are few, half the steps on twice the CUs count for more than the second reading of
+// K/V: one prompt of 500 tokens (8 KV heads) 15.2 -> 12.4 us, 4000 (1 KV head) 82 -> 52 us; with
+// blocks for every CU it is no faster.
+template <class Elem, int GROUPS>
+__global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void prefill_kernel(PrefillArgs a) {
+  constexpr int kGroupWaves = kWaves / GROUPS, kRows = kGroupWaves * kWaveRows;
+  constexpr int kGroupBytes = kBuffers * 2 * kTileBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t all_lds[GROUPS * kGroupBytes];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int group = GROUPS == 1 ? 0 : uniform(tid >> 6) / kGroupWaves, wave = (tid >> 6) - group * kGroupWaves;
+  uint8_t* const lds = all_lds + group * kGroupBytes;  // K and V of the group's tiles
   const int col = lane & 31, half = lane >> 5;
   const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
   const int slot = uniform((int)(blockIdx.x / (unsigned)a.hkv));
-  const Block work = a.batch <= 64 ? by_length(a, slot, lane) : packed_order(a, slot, lane);
+  const Block work = a.batch <= 64 ? by_length<kRows>(a, slot, lane) : packed_order<kRows>(a, slot, lane);
   if (work.index < 0) return;
   const int start = uniform(work.start), len = uniform(work.len), block = uniform(work.index);
   const int rows = len * a.group;
@@ -249,41 +260,48 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
   const int tok = min(tok0 + dt, len - 1);  // a wave past the last row takes the last token's
   const int wave_first = tok0, wave_last = live > 0 ? tok0 + uniform(token_of(last_row)) : -1;
   const int last = (min((block + 1) * kRows, rows) - 1) / a.group;
-  const int tiles = last / kKeys + 1;
+  const int all_tiles = last / kKeys + 1;
+  const int tiles = (all_tiles - group + GROUPS - 1) / GROUPS;  // the group's: GROUPS i + group
+  const int steps = (all_tiles + GROUPS - 1) / GROUPS;
 
-  // A wave moves rows 16 wave + 4 i + lane / 16 of a tile, 256 bytes a row.  16-byte chunk p of
+  // A wave moves rows kMoved wave + 4 i + lane / 16 of a tile, 256 bytes a row.  16-byte chunk p of
   // row r in LDS is chunk p ^ r of K's row (p ^ 4 r of V's), so that reads of one chunk column
   // (K) or of 64 bytes of four rows (V) spread over all banks.
-  const int srow = wave * (kKeys / kWaves) + (lane >> 4), chunk = lane & 15;
-  const uint32_t lds0 = (uint32_t)uniform((int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0] +
-                                                (uint32_t)(wave * (kKeys / kWaves) * kRowBytes)));
+  constexpr int kMoved = kKeys / kGroupWaves;
+  const int srow = wave * kMoved + (lane >> 4), chunk = lane & 15;
+  const uint32_t lds0 = (uint32_t)uniform((int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds +
+                                                (uint32_t)(wave * kMoved * kRowBytes)));
   const uint8_t* const kbase = a.k + (long)start * a.k_stride + (long)kvh * kRowBytes;
   const uint8_t* const vbase = a.v + (long)start * a.v_stride + (long)kvh * kRowBytes;
   const uint32_t koff = (uint32_t)(srow * (int)a.k_stride), kchunk = (chunk ^ (srow & 15)) << 4;
   const uint32_t voff = (uint32_t)(srow * (int)a.v_stride) + ((chunk ^ ((srow & 3) << 2)) << 4);
-  constexpr int kLoads = kKeys / kWaves / 4;  // per wave and tile of K, and of V
+  constexpr int kLoads = kMoved / 4;  // per wave and tile of K, and of V
   // The next tile to fetch: where it lies, and the rows from it to the sequence's end.
   uint64_t kp, vp;
   int left;
   auto fetch = [&](int buf) __attribute__((always_inline)) {
     // Rows past the sequence's end read as zero: the descriptor ends with its last row.
     const int n = min(kKeys, left) - 1;
-    const i32x4 rk{(int)kp, (int)(kp >> 32) & 0xffff, n * (int)a.k_stride + kRowBytes, (int)kRsrcWord3};
-    const i32x4 rv{(int)vp, (int)(vp >> 32) & 0xffff, n * (int)a.v_stride + kRowBytes, (int)kRsrcWord3};
-    const uint32_t to = lds0 + buf * 2 * kTileBytes;
+    const i32x4 rk{uniform((int)kp), uniform((int)(kp >> 32) & 0xffff),
+                   uniform(n * (int)a.k_stride + kRowBytes), (int)kRsrcWord3};
+    const i32x4 rv{uniform((int)vp), uniform((int)(vp >> 32) & 0xffff),
+                   uniform(n * (int)a.v_stride + kRowBytes), (int)kRsrcWord3};
+    const uint32_t to = (uint32_t)uniform((int)(lds0 + buf * 2 * kTileBytes));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       load_to_lds(to + i * 4 * kRowBytes, rk, koff + (kchunk ^ (i << 6)) + i * 4 * (uint32_t)a.k_stride);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       load_to_lds(to + kTileBytes + i * 4 * kRowBytes, rv, voff + i * 4 * (uint32_t)a.v_stride);
-    kp += (uint64_t)(kKeys * a.k_stride);
-    vp += (uint64_t)(kKeys * a.v_stride);
-    left -= kKeys;
+    kp += (uint64_t)(GROUPS * kKeys * a.k_stride);
+    vp += (uint64_t)(GROUPS * kKeys * a.v_stride);
+    left -= GROUPS * kKeys;
   };
   auto begin = [&]() __attribute__((always_inline)) {
-    kp = (uint64_t)uniform_ptr(kbase), vp = (uint64_t)uniform_ptr(vbase), left = len;
-    fetch(0);
+    kp = (uint64_t)uniform_ptr(kbase + (long)group * kKeys * a.k_stride);
+    vp = (uint64_t)uniform_ptr(vbase + (long)group * kKeys * a.v_stride);
+    left = len - group * kKeys;
+    if (tiles > 0) fetch(0);
     if (tiles > 1) fetch(1);
   };
   begin();  // before Q's loads: nothing that waits for those comes between
@@ -311,13 +329,13 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
 
   // A masked weight is 0, and 0 times an infinity or NaN in V is NaN.  So where a row comes out
   // not finite, its workgroup computes once more, `careful`: such values are taken out of the
-  // tiles that a row of it masks in part, those from `masked` on, and put back at the end for
+  // tiles that a row of it masks in part, those of the steps from `masked` on, and put back at the end for
   // the rows from their token on.
   bool careful = false;
-  const int masked = block * kRows / a.group / kKeys;
+  const int masked = block * kRows / a.group / kKeys / GROUPS;  // a step: the same for all groups
   auto clean = [&](int buf) {
-    u32x4* const v = (u32x4*)(lds + buf * 2 * kTileBytes + kTileBytes) + tid;
-    for (int i = 0; i < kTileBytes / 16; i += kWaves * 64) {
+    u32x4* const v = (u32x4*)(lds + buf * 2 * kTileBytes + kTileBytes) + wave * 64 + lane;
+    for (int i = 0; i < kTileBytes / 16; i += kGroupWaves * 64) {
       u32x4 x = v[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = drop_nonfinite<Elem>(x[j]);
@@ -326,15 +344,15 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
     __syncthreads();
   };
 
-  // Tile `tile`, which lies in buffer `buf`; `first`: tile 0, which sets the running maximum,
-  // sums and output.
-  auto step = [&](int tile, int buf, auto first) __attribute__((always_inline)) {
+  // The group's i-th tile, which lies in buffer `buf`; `first`: i = 0, which sets the running
+  // maximum, sums and output.
+  auto step = [&](int i0, int buf, auto first) __attribute__((always_inline)) {
     constexpr bool kFirst = decltype(first)::value;
     const int at = buf * 2 * kTileBytes;
-    if (careful && tile >= masked) clean(buf);
-    if (tile + 2 < tiles) fetch(buf >= 1 ? buf - 1 : buf + 2);
-    const int k0 = tile * kKeys;
-    if (kFirst || k0 <= wave_last) {
+    if (careful && i0 >= masked) clean(buf);
+    if (i0 + 2 < tiles) fetch(buf >= 1 ? buf - 1 : buf + 2);
+    const int k0 = (GROUPS * i0 + group) * kKeys;
+    if ((kFirst && GROUPS == 1) || (k0 <= wave_last && (GROUPS == 1 || i0 < tiles))) {
       f32x16 s = {};
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) s = Elem::mma(*(const u32x4*)(kat[kk] + at), q[kk], s);
@@ -359,6 +377,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
       if constexpr (kFirst) {
         m = fmaxf(mx, __shfl_xor(mx, 32));
+        if constexpr (GROUPS > 1) m = fmaxf(m, -1e30f);  // finite where a row sees no key of the tile
         l = 0.f;
       } else if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
         mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -390,7 +409,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
       for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v1[db], p[1], o[db]);
     }
     // The next tile has landed, and behind the barrier this one's place is free.
-    if (tile + 2 < tiles) landed<2 * kLoads>();
+    if (i0 + 2 < tiles) landed<2 * kLoads>();
     else landed<0>();
     __syncthreads();
   };
@@ -398,16 +417,38 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
   for (;;) {
     landed<0>();
     __syncthreads();
+    if constexpr (GROUPS > 1) {  // a wave without a key: weight 0
+      m = -1e30f, l = 0.f;
+#pragma unroll
+      for (int db = 0; db < 4; ++db) o[db] = f32x16{};
+    }
     step(0, 0, std::true_type{});
-    for (int tile = 1; tile < tiles; tile += kBuffers) {  // LDS places known at compile time
-      step(tile, 1, std::false_type{});
-      if (tile + 1 >= tiles) break;
-      step(tile + 1, 2, std::false_type{});
-      if (tile + 2 >= tiles) break;
-      step(tile + 2, 0, std::false_type{});
+    for (int i = 1; i < steps; i += kBuffers) {  // LDS places known at compile time
+      step(i, 1, std::false_type{});
+      if (i + 1 >= steps) break;
+      step(i + 1, 2, std::false_type{});
+      if (i + 2 >= steps) break;
+      step(i + 2, 0, std::false_type{});
+    }
+    if constexpr (GROUPS > 1) {  // the second group's states to the first's waves
+      float* const at = (float*)all_lds + wave * 66 * 64 + lane;
+      if (group == 1) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) at[j * 64] = o[j >> 4][j & 15];
+        at[64 * 64] = m, at[65 * 64] = l;
+      }
+      __syncthreads();
+      if (group == 0) {
+        const float m1 = at[64 * 64], l1 = at[65 * 64], mn = fmaxf(m, m1);
+        const float c0 = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2), c1 = __builtin_amdgcn_exp2f((m1 - mn) * kScaleLog2);
+        m = mn, l = l * c0 + l1 * c1;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) o[j >> 4][j & 15] = o[j >> 4][j & 15] * c0 + at[j * 64] * c1;
+      }
+      __syncthreads();  // the places are free
     }
     if (careful) {
-      for (int key = masked * kKeys; key <= tok; ++key) {
+      for (int key = masked * GROUPS * kKeys; key <= tok; ++key) {
         const u32x2* const x = (const u32x2*)(vbase + (long)key * a.v_stride) + half;
 #pragma unroll
         for (int c = 0; c < 16; ++c)
@@ -429,11 +470,12 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
         out[4 * db + (i >> 2)][(i >> 1) & 1] = x;
         zero = Elem::times0(x, zero);
       }
-    if (careful || !__syncthreads_or(zero != 0.f)) break;
+    if (careful || !__syncthreads_or(group == 0 && live > 0 && zero != 0.f)) break;
     careful = true;
     begin();
   }
 
+  if (group != 0) return;
   // The wave's 32 rows pass through LDS, so that 16 lanes write one row of 256 bytes; 16-byte
   // chunks lie under an exclusive or with the row.
   uint8_t* const mine = lds + wave * kWaveRows * kRowBytes;
@@ -449,6 +491,14 @@ __global__ __launch_bounds__(kWaves * 64, 3) void prefill_kernel(PrefillArgs a) 
       *(u32x4*)(to + (long)(j + token_of(j) * (a.hq - a.group)) * kRowBytes) =
           *(const u32x4*)(mine + j * kRowBytes + (((lane & 15) ^ (j & 15)) << 4));
   }
+}
+
+int compute_units() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
+    return 256;
+  return n;
 }
 
 }  // namespace
@@ -475,8 +525,8 @@ extern "C" int pkv_prefill_attention(
                 "prefill_attention: a token stride must hold its heads and be a multiple of 8 elements");
   if (k_stride > (1 << 23) || v_stride > (1 << 23))  // a tile's rows lie within 2 GiB
     return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: token strides of K and V up to 2^23 elements");
-  const int64_t slots = (int64_t)tokens * group / kRows + batch;
-  if ((int64_t)tokens * group > INT32_MAX || slots * num_kv_heads > INT32_MAX)
+  auto slots = [&](int rows) { return ((int64_t)tokens * group / rows + batch) * num_kv_heads; };
+  if ((int64_t)tokens * group > INT32_MAX || slots(kWaveRows) > INT32_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: too many tokens");
   if (batch == 0 || tokens == 0) return pkv::ok();
   if (!q || !k || !v || !token_offsets || !output)
@@ -486,9 +536,12 @@ extern "C" int pkv_prefill_attention(
   const PrefillArgs a{(const uint8_t*)q, (const uint8_t*)k, (const uint8_t*)v, token_offsets,
                       (uint8_t*)output, 2 * q_stride, 2 * k_stride, 2 * v_stride,
                       batch, tokens, num_q_heads, num_kv_heads, group, 1.0f / (float)group};
-  const dim3 grid((unsigned)(slots * num_kv_heads)), threads(kWaves * 64);
-  if (dtype == PKV_DTYPE_BF16) prefill_kernel<BFloat><<<grid, threads, 0, (hipStream_t)stream>>>(a);
-  else prefill_kernel<Half><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+  // Blocks of 128 rows that leave more than half of the CUs without one become blocks of 64
+  // rows whose tiles two pairs of waves share.
+  const bool split = slots(kWaves * kWaveRows) <= compute_units() / 2, bf16 = dtype == PKV_DTYPE_BF16;
+  auto* const kernel = split ? (bf16 ? prefill_kernel<BFloat, 2> : prefill_kernel<Half, 2>)
+                             : (bf16 ? prefill_kernel<BFloat, 1> : prefill_kernel<Half, 1>);
+  kernel<<<dim3((unsigned)slots(kWaves * kWaveRows / (split ? 2 : 1))), dim3(kWaves * 64), 0, (hipStream_t)stream>>>(a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? pkv::ok()
                          : fail(PKV_ERR_LAUNCH, "prefill_attention launch: %s", hipGetErrorString(e));

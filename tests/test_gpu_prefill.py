@@ -53,6 +53,16 @@ def test_head_layouts(ext, gpu, hq, hkv, dtype):
     _check(ext, gpu, qkv, off, hq, hkv, f"Hq {hq} Hkv {hkv}")
 
 
+@pytest.mark.parametrize("lengths", [[1], [64, 33], [500], [130, 257, 5], [1000, 17]], ids=str)
+@pytest.mark.parametrize("hq,hkv,empty,dtype", [(8, 2, 150, F16), (3, 3, 60, BF16), (16, 16, 12, F16), (32, 16, 20, BF16)])
+def test_blocks_for_every_cu(ext, gpu, lengths, hq, hkv, empty, dtype):
+    """Sequences without tokens count as blocks, so that the launch has more blocks of 128 rows
+    than half the CUs and its waves do not share rows' tiles out; with up to 64 sequences and
+    with more."""
+    qkv, off = packed_inputs([0] * (empty // 2) + lengths + [0] * (empty - empty // 2), hq, hkv, dtype, seed=sum(lengths) + empty)
+    _check(ext, gpu, qkv, off, hq, hkv, f"{lengths} and {empty} empty")
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_tokens_outside_every_sequence(ext, gpu, dtype):
     """Tokens before the first and behind the last sequence hold NaN: nothing reads them, and
@@ -64,9 +74,9 @@ def test_tokens_outside_every_sequence(ext, gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("hq,hkv", [(8, 2), (2, 2), (16, 1)])
-def test_nonfinite_values_reach_later_tokens_only(ext, gpu, dtype, hq, hkv):
-    qkv, off = packed_inputs([100, 150, 64], hq, hkv, dtype, seed=4)
+@pytest.mark.parametrize("hq,hkv,empty", [(8, 2, 0), (2, 2, 0), (16, 1, 0), (8, 2, 90), (2, 2, 90), (16, 1, 190)])
+def test_nonfinite_values_reach_later_tokens_only(ext, gpu, dtype, hq, hkv, empty):
+    qkv, off = packed_inputs([100, 150, 64] + [0] * empty, hq, hkv, dtype, seed=4)
     k, v = qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
     inf, nan = float("inf"), float("nan")
     v[70, 0, 3], v[90, 0, 3], v[40, 0, 127], v[99, hkv - 1, 0] = inf, -inf, nan, nan

@@ -82,11 +82,15 @@ __device__ inline uint32_t finite_max(uint32_t m, u32x4 x) {
   for (int i = 0; i < 4; ++i) m = max2(m, finite_order<BF16>(x[i]));
   return m;
 }
-// The largest finite magnitude of a wave's values, from its lanes' finite_max.
 template <bool BF16>
-__device__ inline float wave_amax(uint32_t m) {
+__device__ inline uint32_t wave_max(uint32_t m) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) m = max2(m, __shfl_xor(m, d));
+  return m;
+}
+// The largest finite magnitude, from the largest of its finite_order.
+template <bool BF16>
+__device__ inline float finite_value(uint32_t m) {
   const uint32_t z = max(m & 0xffffu, m >> 16), one = BF16 ? 0x80u : 0x400u;
   return pkv::half_bits_to_float<BF16>(z > one ? z - one : 0u);
 }
@@ -127,9 +131,10 @@ __device__ inline float mul_odd(float x, float r) {
   return __uint_as_float((err > 0.f) == (p > 0.f) ? b + 1 : b - 1);
 }
 
-// The stored rows [0, rows) of one (page, head) block, times r (at most 1), rounded again.
-__device__ inline void rescale_rows(uint8_t* block, int rows, float r, int lane) {
-  for (int t = lane >> 4; t < rows; t += 4) {
+// The stored rows first, first + step, ... below `rows` of one (page, head) block, times r (at
+// most 1), rounded again; lane c % 16 takes dims 8 c ... of each.
+__device__ inline void rescale_rows(uint8_t* block, int first, int step, int rows, float r, int lane) {
+  for (int t = first; t < rows; t += step) {
     u32x2* const p = (u32x2*)(block + (long)t * kD + (lane & 15) * 8);
     u32x2 x = *p;
 #pragma unroll
@@ -143,23 +148,25 @@ __device__ inline void rescale_rows(uint8_t* block, int rows, float r, int lane)
   }
 }
 
-// One wave writes one run: `count` tokens from t0 on, in consecutive slots of one page.  Up to
-// 16 * CHUNKS tokens stay in registers between the search for the largest magnitude and the
-// rounding (all of their loads are in flight at once); those of longer runs are read again.
-template <bool BF16, int CHUNKS>
-__device__ void write_run(const WriteArgs& a, int t0, int count, int page, int off, int h, int lane) {
-  constexpr int kRows = 4 * CHUNKS;  // registers' rows of four tokens
+// WAVES waves write one run: `count` tokens from t0 on, in consecutive slots of one page.  Up to
+// 4 * WAVES * ROWS tokens stay in registers between the search for the largest magnitude and
+// the rounding (all of their loads are in flight at once); those of longer runs are read again.
+// `lds`: 2 * WAVES + 2 words.
+template <bool BF16, int WAVES, int ROWS>
+__device__ void write_run(const WriteArgs& a, int t0, int count, int page, int off, int h, int wave, int lane,
+                          uint32_t* lds) {
+  constexpr int kStep = 4 * WAVES;  // tokens that the waves take at once, four each
   const long block = (long)page * a.hkv + h;
   float* const scales = a.kv_scales + 2 * block;
-  const int sub = lane >> 4;
+  const int sub = 4 * wave + (lane >> 4);
   const uint8_t* const kn = a.k_new + t0 * a.k_stride + (long)h * kRowBytes + (lane & 15) * 16;
   const uint8_t* const vn = a.v_new + t0 * a.v_stride + (long)h * kRowBytes + (lane & 15) * 16;
   f32x2 old = {1.f, 1.f};
-  if (off > 0) old = *(const f32x2*)scales;
-  u32x4 k[kRows], v[kRows];
+  if (off > 0 && wave == 0) old = *(const f32x2*)scales;
+  u32x4 k[ROWS], v[ROWS];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int t = 4 * i + sub;
+  for (int i = 0; i < ROWS; ++i) {
+    const int t = kStep * i + sub;
     if (t < count) {
       k[i] = *(const u32x4*)(kn + t * a.k_stride);
       v[i] = *(const u32x4*)(vn + t * a.v_stride);
@@ -169,12 +176,25 @@ __device__ void write_run(const WriteArgs& a, int t0, int count, int page, int o
   }
   uint32_t mk = 0, mv = 0;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) mk = finite_max<BF16>(mk, k[i]), mv = finite_max<BF16>(mv, v[i]);
-  for (int t = 4 * kRows + sub; t < count; t += 4) {
+  for (int i = 0; i < ROWS; ++i) mk = finite_max<BF16>(mk, k[i]), mv = finite_max<BF16>(mv, v[i]);
+  for (int t = kStep * ROWS + sub; t < count; t += kStep) {
     mk = finite_max<BF16>(mk, *(const u32x4*)(kn + t * a.k_stride));
     mv = finite_max<BF16>(mv, *(const u32x4*)(vn + t * a.v_stride));
   }
-  int ek = scale_exponent(wave_amax<BF16>(mk)), ev = scale_exponent(wave_amax<BF16>(mv));
+  mk = wave_max<BF16>(mk), mv = wave_max<BF16>(mv);
+  if constexpr (WAVES > 1) {  // the old scales too: read before, and written after, the barrier
+    __syncthreads();          // the run before is done with `lds`
+    if (lane == 0) lds[2 * wave] = mk, lds[2 * wave + 1] = mv;
+    if (wave == 0 && lane == 0) {
+      lds[2 * WAVES] = __float_as_uint(old[0]);
+      lds[2 * WAVES + 1] = __float_as_uint(old[1]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) mk = max2(mk, lds[2 * w]), mv = max2(mv, lds[2 * w + 1]);
+    old = f32x2{__uint_as_float(lds[2 * WAVES]), __uint_as_float(lds[2 * WAVES + 1])};
+  }
+  int ek = scale_exponent(finite_value<BF16>(mk)), ev = scale_exponent(finite_value<BF16>(mv));
   uint8_t* const kb = a.k_pages + block * a.page_size * kD;
   uint8_t* const vb = a.v_pages + block * a.page_size * kD;
   if (off > 0) {  // earlier tokens share the block: its scales can only grow
@@ -182,34 +202,37 @@ __device__ void write_run(const WriteArgs& a, int t0, int count, int page, int o
     const float ks = fminf(fmaxf(old[0], lo), hi), vs = fminf(fmaxf(old[1], lo), hi);
     ek = max(ek, old_exponent(ks));
     ev = max(ev, old_exponent(vs));
-    if (ks != pow2(ek)) rescale_rows(kb, off, ks * pow2(-ek), lane);
-    if (vs != pow2(ev)) rescale_rows(vb, off, vs * pow2(-ev), lane);
+    if (ks != pow2(ek)) rescale_rows(kb, sub, kStep, off, ks * pow2(-ek), lane);
+    if (vs != pow2(ev)) rescale_rows(vb, sub, kStep, off, vs * pow2(-ev), lane);
   }
   const float ik = pow2(-ek), iv = pow2(-ev);
   const long to = (long)off * kD + (lane & 15) * 8;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int t = 4 * i + sub;
+  for (int i = 0; i < ROWS; ++i) {
+    const int t = kStep * i + sub;
     if (t < count) {
-      *(u32x2*)(kb + to + t * kD) = encode8<BF16>(k[i], ik);
-      *(u32x2*)(vb + to + t * kD) = encode8<BF16>(v[i], iv);
+      *(u32x2*)(kb + to + (long)t * kD) = encode8<BF16>(k[i], ik);
+      *(u32x2*)(vb + to + (long)t * kD) = encode8<BF16>(v[i], iv);
     }
   }
-  for (int t = 4 * kRows + sub; t < count; t += 4) {
+  for (int t = kStep * ROWS + sub; t < count; t += kStep) {
     *(u32x2*)(kb + to + (long)t * kD) = encode8<BF16>(*(const u32x4*)(kn + t * a.k_stride), ik);
     *(u32x2*)(vb + to + (long)t * kD) = encode8<BF16>(*(const u32x4*)(vn + t * a.v_stride), iv);
   }
-  if (lane == 0) *(f32x2*)scales = f32x2{pow2(ek), pow2(ev)};
+  if (wave == 0 && lane == 0) *(f32x2*)scales = f32x2{pow2(ek), pow2(ev)};
 }
 
-// A wave takes the runs that begin in its `window` (at most 16) tokens, for one head.  Its
-// lanes hold the slots of 64 tokens from the one before the window on.
-template <bool BF16, int CHUNKS>
+// WAVES waves take the runs that begin in their `window` (at most 32) tokens, for one head.
+// Every wave's lanes hold the slots of 64 tokens from the one before the window on.  With pages
+// of 16 a run is 8 KB, enough for one wave; longer pages' runs are shared by the workgroup (one
+// wave alone took 25 us for the longest of a few pages of 128) unless they are short.
+template <bool BF16, int WAVES, int ROWS>
 __global__ __launch_bounds__(256) void write_block_kernel(WriteArgs a, int window) {
-  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane((int)(id / a.hkv));
-  const int h = __builtin_amdgcn_readfirstlane((int)(id - (long)w * a.hkv));
+  __shared__ uint32_t lds[2 * WAVES + 2];
+  const int id = blockIdx.x * (4 / WAVES) + (WAVES == 1 ? threadIdx.x >> 6 : 0);
+  const int wave = WAVES == 1 ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(id / a.hkv);
+  const int h = __builtin_amdgcn_readfirstlane(id - w * a.hkv);
   const int first = (int)min((long)w * window, (long)a.tokens);
   const int t = first - 1 + lane;
   const int slot = t >= 0 && t < a.tokens ? a.slots[t] : -1;
@@ -220,14 +243,14 @@ __global__ __launch_bounds__(256) void write_block_kernel(WriteArgs a, int windo
   const uint64_t joined = __builtin_amdgcn_ballot_w64(follows);
   const uint64_t mine = ((1ull << window) - 1) << 1;  // lanes of the window's tokens
   uint64_t starts = __builtin_amdgcn_ballot_w64(valid && !follows) & mine;
+  int turn = 0;
   while (starts) {
     const int i = __builtin_ctzll(starts);
     starts &= starts - 1;
     const int s0 = __builtin_amdgcn_readlane(slot, i), t0 = first - 1 + i;
     const int p0 = __builtin_amdgcn_readlane(page, i), o0 = __builtin_amdgcn_readlane(off, i);
-    // 1 + the lanes behind lane i that follow one another; past lane 63, token by token.
-    const uint64_t after = i < 63 ? ~(joined >> (i + 1)) : 1;
-    int count = 1 + min(__builtin_ctzll(after | 1ull << (63 - i)), 63 - i);
+    // 1 + the lanes behind lane i that follow one another; past lane 63, 64 tokens at a time.
+    int count = 1 + min(__builtin_ctzll(~(joined >> (i + 1)) | 1ull << (63 - i)), 63 - i);
     if (i + count == 64) {
       const int most = min(a.page_size - o0, a.tokens - t0);
       for (bool more = true; more && count < most;) {
@@ -238,7 +261,11 @@ __global__ __launch_bounds__(256) void write_block_kernel(WriteArgs a, int windo
         more = n == 64;
       }
     }
-    write_run<BF16, CHUNKS>(a, t0, count, p0, o0, h, lane);
+    if (WAVES > 1 && window > 1 && count <= 16) {  // short runs: a wave each, in turn
+      if (turn++ % WAVES == wave) write_run<BF16, 1, 4>(a, t0, count, p0, o0, h, 0, lane, lds);
+    } else {
+      write_run<BF16, WAVES, ROWS>(a, t0, count, p0, o0, h, wave, lane, lds);
+    }
   }
 }
 
@@ -252,7 +279,7 @@ int check_write(const char* op, const WriteArgs& a, int32_t head_dim, int32_t nu
     return fail(PKV_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", op, dtype);
   if ((long)num_pages * a.page_size > INT32_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "%s: num_pages * page_size does not fit in int32", op);
-  if ((long)a.tokens * a.hkv > (1L << 32))
+  if ((long)a.tokens * a.hkv > (1L << 31) - 64)
     return fail(PKV_ERR_UNSUPPORTED, "%s: tokens * num_kv_heads too large", op);
   if (a.k_stride < (long)a.hkv * kRowBytes || a.v_stride < (long)a.hkv * kRowBytes ||
       a.k_stride % 16 || a.v_stride % 16)
@@ -301,15 +328,16 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
   if (st != PKV_OK || tokens == 0) return st == PKV_OK ? pkv::ok() : st;
   if (!kv_scales || ((uintptr_t)kv_scales & 7))
     return pkv::fail(PKV_ERR_INVALID_ARGUMENT, "write_kv_fp8_block: kv_scales null or not 8-byte aligned");
-  const int window = (long)tokens * num_kv_heads <= 16384 ? 1 : 16;
-  const long waves = (long)((tokens + window - 1) / window) * num_kv_heads;
-  const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
-  const bool bf16 = dtype == PKV_DTYPE_BF16;
-  const int chunks = page_size <= 16 || window == 1 ? 1 : page_size <= 32 ? 2 : 4;
-  auto* const kernel = chunks == 1 ? (bf16 ? write_block_kernel<true, 1> : write_block_kernel<false, 1>)
-                     : chunks == 2 ? (bf16 ? write_block_kernel<true, 2> : write_block_kernel<false, 2>)
-                                   : (bf16 ? write_block_kernel<true, 4> : write_block_kernel<false, 4>);
-  kernel<<<grid, block, 0, (hipStream_t)stream>>>(a, window);
+  // Few tokens: a window each, so that runs that lie next to one another (a decode step's) are
+  // not written one after another; else windows of about a page, most with one start or two
+  // (a workgroup without one still costs 2 us of a CU's place).
+  const bool bf16 = dtype == PKV_DTYPE_BF16, shared = page_size > 16;
+  const int window = (long)tokens * num_kv_heads <= 4096 ? 1 : shared ? 32 : 16;
+  const long units = (long)((tokens + window - 1) / window) * num_kv_heads;
+  auto* const kernel = !shared         ? (bf16 ? write_block_kernel<true, 1, 4> : write_block_kernel<false, 1, 4>)
+                       : page_size <= 64 ? (bf16 ? write_block_kernel<true, 4, 4> : write_block_kernel<false, 4, 4>)
+                                         : (bf16 ? write_block_kernel<true, 4, 8> : write_block_kernel<false, 4, 8>);
+  kernel<<<dim3((unsigned)(shared ? units : (units + 3) / 4)), dim3(256), 0, (hipStream_t)stream>>>(a, window);
   return launched("write_kv_fp8_block");
 }
 

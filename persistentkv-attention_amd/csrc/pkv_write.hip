@@ -148,91 +148,83 @@ __device__ inline void rescale_rows(uint8_t* block, int first, int step, int row
   }
 }
 
-// WAVES waves write one run: `count` tokens from t0 on, in consecutive slots of one page.  Up to
-// 4 * WAVES * ROWS tokens stay in registers between the search for the largest magnitude and
-// the rounding (all of their loads are in flight at once); those of longer runs are read again.
-// `lds`: 2 * WAVES + 2 words.
+// One of K and V: the run's tensor, and its page's block.
+struct Run {
+  const uint8_t* from;  // the run's first token
+  long stride;          // bytes between tokens
+  uint8_t* block;       // [ps, 128] e4m3
+  float* scale;
+  int count, off;       // tokens, and the slot of the first in its page
+};
+
+// WAVES waves write one run.  Up to 4 * WAVES * ROWS tokens stay in registers between the search
+// for the largest magnitude and the rounding (all of their loads are in flight at once); those
+// of longer runs are read again.  `lds`: WAVES + 1 words.
 template <bool BF16, int WAVES, int ROWS>
-__device__ void write_run(const WriteArgs& a, int t0, int count, int page, int off, int h, int wave, int lane,
-                          uint32_t* lds) {
+__device__ void write_run(const Run& r, int wave, int lane, uint32_t* lds) {
   constexpr int kStep = 4 * WAVES;  // tokens that the waves take at once, four each
-  const long block = (long)page * a.hkv + h;
-  float* const scales = a.kv_scales + 2 * block;
   const int sub = 4 * wave + (lane >> 4);
-  const uint8_t* const kn = a.k_new + t0 * a.k_stride + (long)h * kRowBytes + (lane & 15) * 16;
-  const uint8_t* const vn = a.v_new + t0 * a.v_stride + (long)h * kRowBytes + (lane & 15) * 16;
-  f32x2 old = {1.f, 1.f};
-  if (off > 0 && wave == 0) old = *(const f32x2*)scales;
-  u32x4 k[ROWS], v[ROWS];
+  const uint8_t* const from = r.from + (lane & 15) * 16;
+  float old = 1.f;
+  if (r.off > 0 && wave == 0) old = *r.scale;
+  u32x4 x[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int t = kStep * i + sub;
-    if (t < count) {
-      k[i] = *(const u32x4*)(kn + t * a.k_stride);
-      v[i] = *(const u32x4*)(vn + t * a.v_stride);
-    } else {
-      k[i] = v[i] = u32x4{0, 0, 0, 0};
-    }
+    x[i] = t < r.count ? *(const u32x4*)(from + t * r.stride) : u32x4{0, 0, 0, 0};
   }
-  uint32_t mk = 0, mv = 0;
+  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) mk = finite_max<BF16>(mk, k[i]), mv = finite_max<BF16>(mv, v[i]);
-  for (int t = kStep * ROWS + sub; t < count; t += kStep) {
-    mk = finite_max<BF16>(mk, *(const u32x4*)(kn + t * a.k_stride));
-    mv = finite_max<BF16>(mv, *(const u32x4*)(vn + t * a.v_stride));
-  }
-  mk = wave_max<BF16>(mk), mv = wave_max<BF16>(mv);
-  if constexpr (WAVES > 1) {  // the old scales too: read before, and written after, the barrier
+  for (int i = 0; i < ROWS; ++i) m = finite_max<BF16>(m, x[i]);
+  for (int t = kStep * ROWS + sub; t < r.count; t += kStep)
+    m = finite_max<BF16>(m, *(const u32x4*)(from + t * r.stride));
+  m = wave_max<BF16>(m);
+  if constexpr (WAVES > 1) {  // the old scale too: read before, and written after, the barrier
     __syncthreads();          // the run before is done with `lds`
-    if (lane == 0) lds[2 * wave] = mk, lds[2 * wave + 1] = mv;
-    if (wave == 0 && lane == 0) {
-      lds[2 * WAVES] = __float_as_uint(old[0]);
-      lds[2 * WAVES + 1] = __float_as_uint(old[1]);
-    }
+    if (lane == 0) lds[wave] = m;
+    if (wave == 0 && lane == 0) lds[WAVES] = __float_as_uint(old);
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) mk = max2(mk, lds[2 * w]), mv = max2(mv, lds[2 * w + 1]);
-    old = f32x2{__uint_as_float(lds[2 * WAVES]), __uint_as_float(lds[2 * WAVES + 1])};
+    for (int w = 0; w < WAVES; ++w) m = max2(m, lds[w]);
+    old = __uint_as_float(lds[WAVES]);
   }
-  int ek = scale_exponent(finite_value<BF16>(mk)), ev = scale_exponent(finite_value<BF16>(mv));
-  uint8_t* const kb = a.k_pages + block * a.page_size * kD;
-  uint8_t* const vb = a.v_pages + block * a.page_size * kD;
-  if (off > 0) {  // earlier tokens share the block: its scales can only grow
-    const float lo = pow2(-kScaleExp), hi = pow2(kScaleExp);
-    const float ks = fminf(fmaxf(old[0], lo), hi), vs = fminf(fmaxf(old[1], lo), hi);
-    ek = max(ek, old_exponent(ks));
-    ev = max(ev, old_exponent(vs));
-    if (ks != pow2(ek)) rescale_rows(kb, sub, kStep, off, ks * pow2(-ek), lane);
-    if (vs != pow2(ev)) rescale_rows(vb, sub, kStep, off, vs * pow2(-ev), lane);
+  int e = scale_exponent(finite_value<BF16>(m));
+  if (r.off > 0) {  // earlier tokens share the block: its scale can only grow
+    old = fminf(fmaxf(old, pow2(-kScaleExp)), pow2(kScaleExp));
+    e = max(e, old_exponent(old));
+    if (old != pow2(e)) rescale_rows(r.block, sub, kStep, r.off, old * pow2(-e), lane);
   }
-  const float ik = pow2(-ek), iv = pow2(-ev);
-  const long to = (long)off * kD + (lane & 15) * 8;
+  const float inv = pow2(-e);
+  uint8_t* const to = r.block + (long)r.off * kD + (lane & 15) * 8;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int t = kStep * i + sub;
-    if (t < count) {
-      *(u32x2*)(kb + to + (long)t * kD) = encode8<BF16>(k[i], ik);
-      *(u32x2*)(vb + to + (long)t * kD) = encode8<BF16>(v[i], iv);
-    }
+    if (t < r.count) *(u32x2*)(to + (long)t * kD) = encode8<BF16>(x[i], inv);
   }
-  for (int t = kStep * ROWS + sub; t < count; t += kStep) {
-    *(u32x2*)(kb + to + (long)t * kD) = encode8<BF16>(*(const u32x4*)(kn + t * a.k_stride), ik);
-    *(u32x2*)(vb + to + (long)t * kD) = encode8<BF16>(*(const u32x4*)(vn + t * a.v_stride), iv);
-  }
-  if (wave == 0 && lane == 0) *(f32x2*)scales = f32x2{pow2(ek), pow2(ev)};
+  for (int t = kStep * ROWS + sub; t < r.count; t += kStep)
+    *(u32x2*)(to + (long)t * kD) = encode8<BF16>(*(const u32x4*)(from + t * r.stride), inv);
+  if (wave == 0 && lane == 0) *r.scale = pow2(e);
 }
 
-// WAVES waves take the runs that begin in their `window` (at most 32) tokens, for one head.
-// Every wave's lanes hold the slots of 64 tokens from the one before the window on.  With pages
-// of 16 a run is 8 KB, enough for one wave; longer pages' runs are shared by the workgroup (one
-// wave alone took 25 us for the longest of a few pages of 128) unless they are short.
+// WAVES waves take the runs that begin in their `window` (at most 32) tokens, for one head and
+// K or V.  Heads vary fastest, K's before V's: a token's lie next to one another in memory, and
+// are read at about the same time.  Every wave's lanes hold the slots of 64 tokens from the one
+// before the window on.  A run of up to 64 tokens is one wave's, in its registers; the runs of
+// longer pages are shared by the workgroup (one wave took 25 us for the longest of two rows of
+// 8270 tokens in pages of 128, four take 9.6) unless they are short.
+//
+// Bound by memory: 46257 tokens, 8 heads, some continuing a page, 284 MB: 59.7 us in pages of 16
+// (4.8 TB/s, where a copy reaches 5.1), 59 of 32, 76 of 64, 115 of 128 (a token's heads are read
+// further apart in time).  Four waves a run from pages of 32 on: 95 us of 32, 107 of 64.
 template <bool BF16, int WAVES, int ROWS>
 __global__ __launch_bounds__(256) void write_block_kernel(WriteArgs a, int window) {
-  __shared__ uint32_t lds[2 * WAVES + 2];
+  __shared__ uint32_t lds[WAVES + 1];
   const int id = blockIdx.x * (4 / WAVES) + (WAVES == 1 ? threadIdx.x >> 6 : 0);
   const int wave = WAVES == 1 ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane(id / a.hkv);
-  const int h = __builtin_amdgcn_readfirstlane(id - w * a.hkv);
+  const int w = __builtin_amdgcn_readfirstlane(id / (2 * a.hkv));
+  const int part = __builtin_amdgcn_readfirstlane(id - w * (2 * a.hkv));
+  const bool is_v = part >= a.hkv;
+  const int h = is_v ? part - a.hkv : part;
   const int first = (int)min((long)w * window, (long)a.tokens);
   const int t = first - 1 + lane;
   const int slot = t >= 0 && t < a.tokens ? a.slots[t] : -1;
@@ -261,10 +253,14 @@ __global__ __launch_bounds__(256) void write_block_kernel(WriteArgs a, int windo
         more = n == 64;
       }
     }
+    const long block = (long)p0 * a.hkv + h, stride = is_v ? a.v_stride : a.k_stride;
+    const Run run{(is_v ? a.v_new : a.k_new) + t0 * stride + (long)h * kRowBytes, stride,
+                  (is_v ? a.v_pages : a.k_pages) + block * a.page_size * kD,
+                  a.kv_scales + 2 * block + (is_v ? 1 : 0), count, o0};
     if (WAVES > 1 && window > 1 && count <= 16) {  // short runs: a wave each, in turn
-      if (turn++ % WAVES == wave) write_run<BF16, 1, 4>(a, t0, count, p0, o0, h, 0, lane, lds);
+      if (turn++ % WAVES == wave) write_run<BF16, 1, 4>(run, 0, lane, lds);
     } else {
-      write_run<BF16, WAVES, ROWS>(a, t0, count, p0, o0, h, wave, lane, lds);
+      write_run<BF16, WAVES, ROWS>(run, wave, lane, lds);
     }
   }
 }
@@ -279,7 +275,7 @@ int check_write(const char* op, const WriteArgs& a, int32_t head_dim, int32_t nu
     return fail(PKV_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", op, dtype);
   if ((long)num_pages * a.page_size > INT32_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "%s: num_pages * page_size does not fit in int32", op);
-  if ((long)a.tokens * a.hkv > (1L << 31) - 64)
+  if ((long)a.tokens * a.hkv > (1L << 30) - 64)
     return fail(PKV_ERR_UNSUPPORTED, "%s: tokens * num_kv_heads too large", op);
   if (a.k_stride < (long)a.hkv * kRowBytes || a.v_stride < (long)a.hkv * kRowBytes ||
       a.k_stride % 16 || a.v_stride % 16)
@@ -331,12 +327,13 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
   // Few tokens: a window each, so that runs that lie next to one another (a decode step's) are
   // not written one after another; else windows of about a page, most with one start or two
   // (a workgroup without one still costs 2 us of a CU's place).
-  const bool bf16 = dtype == PKV_DTYPE_BF16, shared = page_size > 16;
-  const int window = (long)tokens * num_kv_heads <= 4096 ? 1 : shared ? 32 : 16;
-  const long units = (long)((tokens + window - 1) / window) * num_kv_heads;
-  auto* const kernel = !shared         ? (bf16 ? write_block_kernel<true, 1, 4> : write_block_kernel<false, 1, 4>)
-                       : page_size <= 64 ? (bf16 ? write_block_kernel<true, 4, 4> : write_block_kernel<false, 4, 4>)
-                                         : (bf16 ? write_block_kernel<true, 4, 8> : write_block_kernel<false, 4, 8>);
+  const bool bf16 = dtype == PKV_DTYPE_BF16, shared = page_size > 64;
+  const int window = (long)tokens * num_kv_heads <= 4096 ? 1 : page_size > 16 ? 32 : 16;
+  const long units = (long)((tokens + window - 1) / window) * num_kv_heads * 2;
+  auto* const kernel = shared           ? (bf16 ? write_block_kernel<true, 4, 8> : write_block_kernel<false, 4, 8>)
+                       : page_size <= 16 ? (bf16 ? write_block_kernel<true, 1, 4> : write_block_kernel<false, 1, 4>)
+                       : page_size <= 32 ? (bf16 ? write_block_kernel<true, 1, 8> : write_block_kernel<false, 1, 8>)
+                                         : (bf16 ? write_block_kernel<true, 1, 16> : write_block_kernel<false, 1, 16>);
   kernel<<<dim3((unsigned)(shared ? units : (units + 3) / 4)), dim3(256), 0, (hipStream_t)stream>>>(a, window);
   return launched("write_kv_fp8_block");
 }

@@ -359,8 +359,10 @@ int pkv_build_block_tables(
 /* Causal attention over whole prompts: sequence b is the tokens [token_offsets[b],
  * token_offsets[b + 1]) of q [tokens, num_q_heads, 128] and of k, v [tokens, num_kv_heads,
  * 128]; its token i attends to its tokens 0 ... i.  output [tokens, num_q_heads, 128],
- * contiguous; rows outside every sequence are left as they are.  Offsets must not decrease and
- * count as clamped to [0, tokens].  G = num_q_heads / num_kv_heads in [1, 32]. */
+ * contiguous; rows outside every sequence are left as they are.  It may be q itself, but must
+ * not overlap k or v.  Offsets must not decrease and count as clamped to [0, tokens].
+ * G = num_q_heads / num_kv_heads in [1, 32].  An infinity or NaN in K or V reaches the tokens
+ * from its own on, and no other. */
 int pkv_prefill_attention(
     const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
     int64_t v_stride, const int32_t* token_offsets, void* output, int32_t batch, int32_t tokens,
@@ -396,7 +398,7 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
  * multiple of 16; rows of length 0 give zeros; lengths are clamped to the table, page ids
  * into the pool.  At most 16000 rows.  The workspace is required:
  * pkv_fp8_block_workspace_bytes on the same device, for any lengths; it holds nothing
- * between calls. */
+ * between calls, and calls that may overlap need one each.  output may be q itself. */
 int pkv_paged_attention_fp8_block(
     const void* q, const void* k_pages, const void* v_pages, const float* kv_scales,
     const int32_t* block_table, const int32_t* seq_lens, void* output, void* workspace,

@@ -20,6 +20,7 @@
 //   from row-major V in LDS through the transposing reads (ds_read_b64_tr_b16).
 
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void prefill_kern
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
       if constexpr (kFirst) {
         m = fmaxf(mx, __shfl_xor(mx, 32));
-        if constexpr (GROUPS > 1) m = fmaxf(m, -1e30f);  // finite where a row sees no key of the tile
+        if (GROUPS > 1 && m == -INFINITY) m = -FLT_MAX;  // finite where a row sees no key of the tile
         l = 0.f;
       } else if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
         mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void prefill_kern
     landed<0>();
     __syncthreads();
     if constexpr (GROUPS > 1) {  // a wave without a key: weight 0
-      m = -1e30f, l = 0.f;
+      m = -FLT_MAX, l = 0.f;
 #pragma unroll
       for (int db = 0; db < 4; ++db) o[db] = f32x16{};
     }
@@ -533,6 +534,8 @@ extern "C" int pkv_prefill_attention(
     return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: null pointer");
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)output) & 15)
     return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: tensors must be 16-byte aligned");
+  if (output == k || output == v)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: output must not be k or v");
   const PrefillArgs a{(const uint8_t*)q, (const uint8_t*)k, (const uint8_t*)v, token_offsets,
                       (uint8_t*)output, 2 * q_stride, 2 * k_stride, 2 * v_stride,
                       batch, tokens, num_q_heads, num_kv_heads, group, 1.0f / (float)group};

@@ -102,6 +102,42 @@ def test_growing_and_peaked_scores(ext, gpu, dtype):
     _check(ext, gpu, qkv, off, 4, 1, "one peak")
 
 
+@pytest.mark.parametrize("empty", [0, 90])
+def test_scores_at_the_ends_of_the_range(ext, gpu, empty):
+    """bf16 scores around -1e36 in every token (their differences decide), and rows of -inf."""
+    qkv, off = packed_inputs([90, 40] + [0] * empty, 2, 1, BF16, seed=11)
+    qkv[:, :2] = 0.0
+    qkv[:, 2] = 0.0
+    qkv[:90, :2, 0] = 2.0 ** 60
+    steps = torch.arange(90) % 3
+    qkv[:90, 2, 0] = (-(2.0 ** 60) * (1 + steps / 4)).to(BF16)
+    out = torch.zeros(130, 2, 128, dtype=BF16, device=gpu)
+    ext.prefill_attention(*split_qkv(qkv.to(gpu), 2, 1), off.to(gpu), out)
+    v = qkv[:90, 3].double()
+    for i in range(90):  # the tokens with the largest score share all the weight
+        want = v[:i + 1][steps[:i + 1] == 0].mean(0)
+        assert (out[i].cpu().double() - want).abs().max() <= 2.0 ** -7 * want.abs().max() + 1e-4
+    qkv[90:, :2, 0] = float("inf")
+    qkv[90:, 2, 0] = -1.0
+    ext.prefill_attention(*split_qkv(qkv.to(gpu), 2, 1), off.to(gpu), out)
+    assert torch.isnan(out[90:]).all() and torch.isfinite(out[:90]).all()
+
+
+def test_token_strides_at_their_limit(ext, gpu):
+    """2^23 elements between the tokens of K: 300 of them pass 2^32 bytes."""
+    qkv, off = packed_inputs([10, 290], 4, 2, F16, seed=12)
+    q, k, v = (x.contiguous().to(gpu) for x in split_qkv(qkv, 4, 2))
+    far = torch.empty(299 * 2 ** 23 + 256, dtype=F16, device=gpu).as_strided((300, 2, 128), (2 ** 23, 128, 1))
+    far.copy_(k)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    ext.prefill_attention(q, k, v, off.to(gpu), a)
+    ext.prefill_attention(q, far, v, off.to(gpu), b)
+    assert torch.equal(a, b)
+    far.copy_(v)
+    ext.prefill_attention(q, k, far, off.to(gpu), b)
+    assert torch.equal(a, b)
+
+
 def test_contiguous_and_offset_inputs(ext, gpu):
     qkv, off = packed_inputs([150, 33], 8, 2, F16, seed=8)
     ref = _check(ext, gpu, qkv, off, 8, 2)

@@ -128,3 +128,40 @@ def test_write_nothing(ext, gpu):
     p8, s = pool.to(F8), torch.ones(3, 2, 2, device=gpu)
     ext.write_kv_fp8_block(k, k, p8, p8.clone(), s, none)
     assert (s == 1).all()
+
+
+def test_pools_past_32_bits(ext, gpu):
+    """Pages at the end of pools of more than 2^32 bytes (and 2^31 elements)."""
+    pages, hkv, ps = 2 ** 21 + 8, 1, 16
+    near = [3, 0, 5]
+    slots = {d: torch.tensor([(p + d) * ps + i for p in near for i in range(ps)], dtype=torch.int32, device=gpu)
+             for d in (0, pages - 8)}
+    k, v = (x.contiguous().to(gpu) for x in _new(48, hkv, F16, seed=15))
+    small = [torch.zeros(8, hkv, ps, 128, dtype=F16, device=gpu) for _ in range(2)]
+    ext.write_kv(k, v, *small, slots[0])
+    big = [torch.empty(pages, hkv, ps, 128, dtype=F16, device=gpu) for _ in range(2)]
+    for x in big:
+        x[-8:] = 0
+    ext.write_kv(k, v, *big, slots[pages - 8])
+    assert all(torch.equal(b[-8:], s) for b, s in zip(big, small))
+    del big
+    small = [x.to(F8) for x in small]
+    s0, s1 = torch.ones(8, hkv, 2, device=gpu), torch.ones(pages, hkv, 2, device=gpu)
+    ext.write_kv_fp8_block(k, v, *small, s0, slots[0])
+    big = [torch.empty(pages, hkv, ps, 128, dtype=F8, device=gpu) for _ in range(2)]
+    for x in big:
+        x.view(torch.uint8)[-8:] = 0
+    ext.write_kv_fp8_block(k, v, *big, s1, slots[pages - 8])
+    assert torch.equal(s1[-8:], s0)
+    sel = torch.tensor(near, device=gpu)
+    for b, s in zip(big, small):
+        assert torch.equal(b.view(torch.uint8)[-8:][sel], s.view(torch.uint8)[sel])
+    # and decode over them
+    q = torch.randn(1, 4, 128, device=gpu).to(F16)
+    table = torch.tensor([near], dtype=torch.int32, device=gpu)
+    lens = torch.tensor([40], dtype=torch.int32, device=gpu)
+    ws = torch.empty(ext.fp8_block_workspace_floats(1, 4, 1), device=gpu)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    ext.paged_attention_fp8_block(q, *small, s0, table, lens, a, ws, ps)
+    ext.paged_attention_fp8_block(q, *big, s1, table + (pages - 8), lens, b, ws, ps)
+    assert torch.equal(a, b) and torch.isfinite(a).all()

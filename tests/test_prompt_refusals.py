@@ -11,6 +11,9 @@ F16, F8, I32 = torch.float16, torch.float8_e4m3fn, torch.int32
 FAKE = ctypes.c_void_p(0x1000)  # never dereferenced: validation fails first
 
 
+OUT = ctypes.c_void_p(0x8000)
+
+
 def _call(name, args):
     f = getattr(pkv_native.lib(), name)
     f.restype = ctypes.c_int
@@ -27,7 +30,7 @@ def _tables(**o):
 
 
 def _prefill(**o):
-    a = dict(q=FAKE, qs=1024, k=FAKE, ks=256, v=FAKE, vs=256, off=FAKE, out=FAKE, batch=1, tokens=4, hq=8, hkv=2, d=128, dtype=0)
+    a = dict(q=FAKE, qs=1024, k=FAKE, ks=256, v=FAKE, vs=256, off=FAKE, out=OUT, batch=1, tokens=4, hq=8, hkv=2, d=128, dtype=0)
     a.update(o)
     for s in ("qs", "ks", "vs"):
         a[s] = ("i64", a[s])
@@ -60,7 +63,7 @@ def _decode(**o):
     (_prefill, dict(qs=1016), 1, "stride"), (_prefill, dict(ks=252), 1, "stride"), (_prefill, dict(vs=260), 1, "stride"),
     (_prefill, dict(ks=1 << 24), 2, "2^23"), (_prefill, dict(dtype=5), 2, "dtype"), (_prefill, dict(tokens=-1), 1, "tokens"),
     (_prefill, dict(tokens=1 << 30, hq=8), 2, "too many"), (_prefill, dict(out=None), 1, "null"),
-    (_prefill, dict(k=ctypes.c_void_p(0x1008)), 1, "aligned"),
+    (_prefill, dict(k=ctypes.c_void_p(0x1008)), 1, "aligned"), (_prefill, dict(out=FAKE), 1, "must not be k or v"),
     (_write, dict(d=64), 2, "head_dim"), (_write, dict(ps=0), 1, "page_size"), (_write, dict(ks=128), 1, "stride"),
     (_write, dict(vs=260), 1, "stride"), (_write, dict(dtype=9), 1, "dtype"), (_write, dict(slots=None), 1, "null"),
     (_write, dict(pages=1 << 30), 2, "int32"), (_write, dict(tokens=-2), 1, "tokens"), (_write, dict(k=ctypes.c_void_p(0x1008)), 1, "aligned"),

@@ -20,7 +20,10 @@
 //
 // Per wave and tile: K and V straight from the pages into registers (16- and 8-byte buffer
 // loads whose descriptor ends with the row's last token), S^T = K Q^T and O^T += V^T P^T on
-// v_mfma_f32_16x16x32, heads padded to 16 a block.
+// v_mfma_f32_16x16x32, heads padded to 16 a block.  Two tiles (16 KB) in flight in each of a CU's
+// four waves keep HBM busy: 64 Zipf rows (bf16, G = 8, 600 MB) 97-99 us, 6.1 TB/s; 8 bimodal
+// rows (fp16, G = 4, 95 MB) 19.5 us, 4.9 TB/s, of which about 3 us pass before the first bytes;
+// then 4 to 6 us of merge.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_block_kernel(BlockArgs a) 
 // Joins the partial states of one (pair, head); an empty row's output is zero.  Every wave
 // computes the states' weights 2^(m - M) for itself, a state a lane; then half a wave reads one
 // state's 512 bytes of sums, so that a workgroup has 8 states in flight in each of kUnroll steps.
-// (One wave a head, a state after another, took 10 to 22 us where this takes 3 to 5.)
+// (One wave a head, a state after another, took 10 to 22 us where this takes 4 to 6.)
 template <class Elem>
 __global__ __launch_bounds__(kMergeWaves * 64) void merge_block_kernel(BlockArgs a) {
   constexpr int kUnroll = 4, kHalves = 2 * kMergeWaves;

@@ -30,6 +30,7 @@
 #include <stdint.h>
 
 #include "pkv.h"
+#include "pkv_device.h"
 
 namespace pkv {
 int fail(int status, const char* fmt, ...);  // pkv_decode.hip: sets pkv_last_error()
@@ -475,16 +476,8 @@ __global__ __launch_bounds__(kMergeWaves * 64) void merge_block_kernel(BlockArgs
   }
 }
 
-int compute_units() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-    return 256;
-  return n;
-}
-
 size_t workspace_bytes(int64_t batch, int64_t hkv, int64_t group) {
-  const size_t states = 2 * (size_t)compute_units() * kWaves * group * kStateFloats * sizeof(float);
+  const size_t states = 2 * (size_t)pkv::compute_units() * kWaves * group * kStateFloats * sizeof(float);
   return states + (size_t)batch * hkv * sizeof(int2);
 }
 
@@ -544,7 +537,7 @@ int pkv_paged_attention_fp8_block(
   if (!workspace || workspace_size < need)
     return fail(PKV_ERR_WORKSPACE_TOO_SMALL, "paged_attention_fp8_block: workspace of %zu bytes, %zu needed",
                 workspace_size, need);
-  const int waves = compute_units() * kWaves;
+  const int waves = pkv::compute_units() * kWaves;
   BlockArgs a{};
   a.q = (const uint8_t*)q;
   a.k_pages = (const uint8_t*)k_pages;

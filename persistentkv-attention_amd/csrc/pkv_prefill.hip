@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "pkv.h"
+#include "pkv_device.h"
 
 namespace pkv {
 int fail(int status, const char* fmt, ...);  // pkv_decode.hip: sets pkv_last_error()
@@ -503,14 +504,6 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void prefill_kern
   }
 }
 
-int compute_units() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-    return 256;
-  return n;
-}
-
 }  // namespace
 
 extern "C" int pkv_prefill_attention(
@@ -550,7 +543,7 @@ extern "C" int pkv_prefill_attention(
                       batch, tokens, num_q_heads, num_kv_heads, group, 1.0f / (float)group};
   // Blocks of 128 rows that leave more than half of the CUs without one become blocks of 64
   // rows whose tiles two pairs of waves share.
-  const bool split = slots(kWaves * kWaveRows) <= compute_units() / 2, bf16 = dtype == PKV_DTYPE_BF16;
+  const bool split = slots(kWaves * kWaveRows) <= pkv::compute_units() / 2, bf16 = dtype == PKV_DTYPE_BF16;
   auto* const kernel = split ? (bf16 ? prefill_kernel<BFloat, 2> : prefill_kernel<Half, 2>)
                              : (bf16 ? prefill_kernel<BFloat, 1> : prefill_kernel<Half, 1>);
   kernel<<<dim3((unsigned)slots(kWaves * kWaveRows / (split ? 2 : 1))), dim3(kWaves * 64), 0, (hipStream_t)stream>>>(a);

@@ -118,13 +118,12 @@ __device__ inline int load_scalar(const int32_t* p) {
   return uniform(*(const __attribute__((address_space(4))) int32_t*)p);
 }
 
-// Tokens of a row, at most what its table row can address.
-__device__ inline int row_length(const BlockArgs& a, int row) {
-  const long cap = (long)a.max_pages * a.page_size;
-  return (int)min((long)max(a.seq_lens[row], 0), cap);
+// Tokens of a row, at most what its table row can address (below 2^31, see the launch).
+__device__ inline int clamp_length(const BlockArgs& a, int n) {
+  return min(max(n, 0), a.max_pages * a.page_size);
 }
 __device__ inline int row_positions(const BlockArgs& a, int row) {
-  const int n = row_length(a, row);
+  const int n = clamp_length(a, a.seq_lens[row]);
   return n ? (n + kTile - 1) / kTile + kPieceCost : 0;
 }
 
@@ -281,9 +280,9 @@ __device__ inline u32x4 pack8(const f32x4 (&o)[8], int i, float f) {
 template <class Elem, int HB>
 __device__ void piece(const BlockArgs& a, int row, int kvh, int t0, int t1, int state, int lane) {
   const int c = lane & 15, g = lane >> 4;
-  const int len = uniform(row_length(a, row));
-  const Stream stream{a, a.block_table + (long)row * a.max_pages, kvh, min(len, t1 * kTile), lane};
+  Stream stream{a, a.block_table + (long)row * a.max_pages, kvh, 0, lane};
   Pages pa = stream.lookup(t0), pb = stream.lookup(t0 + 1);
+  stream.len = min(clamp_length(a, load_scalar(a.seq_lens + row)), t1 * kTile);
   u32x4 q[HB][4];
 #pragma unroll
   for (int hb = 0; hb < HB; ++hb) {
@@ -338,6 +337,19 @@ __device__ void piece(const BlockArgs& a, int row, int kvh, int t0, int t1, int 
   }
 }
 
+template <int CTRL, int ROW_MASK>
+__device__ inline uint32_t dpp_add(uint32_t x) {
+  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ inline uint32_t wave_scan(uint32_t x) {  // inclusive sums
+  x = dpp_add<0x111, 0xf>(x);                       // row_shr 1, 2, 4, 8: within 16 lanes
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);                       // row_bcast 15, 31
+  return dpp_add<0x143, 0xc>(x);
+}
+
 template <class Elem, int HB>
 __global__ __launch_bounds__(kWaves * 64) void decode_block_kernel(BlockArgs a) {
   extern __shared__ uint32_t prefix[];  // [B + 1] exclusive prefix of the rows' positions, then sums
@@ -347,11 +359,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_block_kernel(BlockArgs a) 
   for (int base = 0; base < a.batch; base += kWaves * 64) {
     const int row = base + tid;
     uint32_t x = row < a.batch ? (uint32_t)row_positions(a, row) : 0;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t u = __shfl_up(x, d);
-      if (lane >= d) x += u;
-    }
+    x = wave_scan(x);
     if (lane == 63) sums[wave] = x;
     __syncthreads();
 #pragma unroll

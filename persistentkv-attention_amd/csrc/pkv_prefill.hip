@@ -215,7 +215,7 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 // 64 x 16 bytes from a buffer straight to LDS, lane l's to `lds` + 16 l.  In assembly because the
 // compiler lets every LDS read wait for every such load in flight, the next tile's among them;
 // landed() is the wait, before the barrier behind which the tile is read.  No registers are
-// written.
+// written but m0, which nothing else in these kernels uses.
 __device__ inline void load_to_lds(uint32_t lds, i32x4 rsrc, uint32_t offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(lds), "v"(offset), "s"(rsrc) : "memory");

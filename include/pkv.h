@@ -361,8 +361,8 @@ int pkv_build_block_tables(
  * 128]; its token i attends to its tokens 0 ... i.  output [tokens, num_q_heads, 128],
  * contiguous; rows outside every sequence are left as they are.  It may be q itself, but must
  * not overlap k or v.  Offsets must not decrease and count as clamped to [0, tokens].
- * G = num_q_heads / num_kv_heads in [1, 32].  An infinity or NaN in K or V reaches the tokens
- * from its own on, and no other. */
+ * G = num_q_heads / num_kv_heads in [1, 32]; (tokens * G / 128 + batch) * num_kv_heads must be
+ * below 2^24.  An infinity or NaN in K or V reaches the tokens from its own on, and no other. */
 int pkv_prefill_attention(
     const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
     int64_t v_stride, const int32_t* token_offsets, void* output, int32_t batch, int32_t tokens,
@@ -371,7 +371,7 @@ int pkv_prefill_attention(
 /* Writes k_new[t] and v_new[t] ([num_kv_heads, 128], dtype f16 or bf16) to slot
  * slot_mapping[t] (page * page_size + offset) of the pools [num_pages, num_kv_heads,
  * page_size, 128] of the same dtype.  Slots outside the pools are skipped; a slot may occur
- * only once in a call. */
+ * only once in a call.  tokens * num_kv_heads must be below 2^28. */
 int pkv_write_kv(const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride,
                  void* k_pages, void* v_pages, const int32_t* slot_mapping, int32_t tokens,
                  int32_t num_kv_heads, int32_t head_dim, int32_t num_pages, int32_t page_size,
@@ -396,7 +396,8 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
  * V = kv_scales[p, h, 1] * v8 for every page p and KV head h.  Scales count as clamped to
  * [2^-60, 2^60] (NaN as the lower end) and need not be powers of two.  page_size must be a
  * multiple of 16; rows of length 0 give zeros; lengths are clamped to the table, page ids
- * into the pool.  At most 16000 rows.  The workspace is required:
+ * into the pool.  At most 16000 rows, and fewer than 2^24 output rows (batch * num_q_heads).
+ * The workspace is required:
  * pkv_fp8_block_workspace_bytes on the same device, for any lengths; it holds nothing
  * between calls, and calls that may overlap need one each.  output may be q itself. */
 int pkv_paged_attention_fp8_block(

@@ -532,9 +532,10 @@ int pkv_paged_attention_fp8_block(
     return fail(PKV_ERR_UNSUPPORTED, "paged_attention_fp8_block: batch %d (at most %d)", batch, kMaxRows);
   const int64_t tokens = (int64_t)max_pages * page_size;
   const int64_t capacity = tokens < INT32_MAX ? tokens : INT32_MAX;
-  if (tokens > INT32_MAX - 256 || (capacity / kTile + 1 + kPieceCost) * batch * num_kv_heads > INT32_MAX ||
-      (int64_t)batch * num_q_heads > INT32_MAX / 2)
+  if (tokens > INT32_MAX - 256 || (capacity / kTile + 1 + kPieceCost) * batch * num_kv_heads > INT32_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "paged_attention_fp8_block: the block table addresses too many tokens");
+  if (!pkv::fits_grid((int64_t)batch * num_q_heads, kMergeWaves * 64))
+    return fail(PKV_ERR_UNSUPPORTED, "paged_attention_fp8_block: batch * num_q_heads too large (below 2^24)");
   if (batch == 0) return pkv::ok();
   if (!q || !k_pages || !v_pages || !kv_scales || !block_table || !seq_lens || !output)
     return fail(PKV_ERR_INVALID_ARGUMENT, "paged_attention_fp8_block: null pointer");

@@ -3,6 +3,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <stdint.h>
+
 #include <atomic>
 
 namespace pkv {
@@ -19,5 +21,8 @@ inline int compute_units() {
   }
   return n;
 }
+
+// Whether a launch of `blocks` in one dimension is possible: its threads must count in 32 bits.
+inline bool fits_grid(int64_t blocks, int threads) { return blocks * threads <= (int64_t)UINT32_MAX; }
 
 }  // namespace pkv

@@ -529,8 +529,8 @@ extern "C" int pkv_prefill_attention(
   if (k_stride > (1 << 23) || v_stride > (1 << 23))  // a tile's rows lie within 2 GiB
     return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: token strides of K and V up to 2^23 elements");
   auto slots = [&](int rows) { return ((int64_t)tokens * group / rows + batch) * num_kv_heads; };
-  if ((int64_t)tokens * group > INT32_MAX || slots(kWaveRows) > INT32_MAX)
-    return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: too many tokens");
+  if ((int64_t)tokens * group > INT32_MAX || !pkv::fits_grid(slots(kWaves * kWaveRows), kWaves * 64))
+    return fail(PKV_ERR_UNSUPPORTED, "prefill_attention: too many tokens or sequences");
   if (batch == 0 || tokens == 0) return pkv::ok();
   if (!q || !k || !v || !token_offsets || !output)
     return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: null pointer");

@@ -16,6 +16,7 @@
 #include <stdint.h>
 
 #include "pkv.h"
+#include "pkv_device.h"
 #include "pkv_e4m3.h"
 
 namespace pkv {
@@ -309,7 +310,10 @@ int pkv_write_kv(const void* k_new, int64_t k_stride, const void* v_new, int64_t
   const int st = check_write("write_kv", a, head_dim, num_pages, dtype);
   if (st != PKV_OK || tokens == 0) return st == PKV_OK ? pkv::ok() : st;
   const long lanes = (long)tokens * num_kv_heads * 16;
-  write_kernel<<<dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, (hipStream_t)stream>>>(a);
+  const long groups = (lanes + 255) / 256;
+  if (!pkv::fits_grid(groups, 256))
+    return pkv::fail(PKV_ERR_UNSUPPORTED, "write_kv: tokens * num_kv_heads too large (below 2^28)");
+  write_kernel<<<dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream>>>(a);
   return launched("write_kv");
 }
 
@@ -331,11 +335,14 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
   const bool bf16 = dtype == PKV_DTYPE_BF16, shared = page_size > 64;
   const int window = (long)tokens * num_kv_heads <= 4096 ? 1 : page_size > 16 ? 32 : 16;
   const long units = (long)((tokens + window - 1) / window) * num_kv_heads * 2;
+  const long groups = shared ? units : (units + 3) / 4;
+  if (!pkv::fits_grid(groups, 256))
+    return pkv::fail(PKV_ERR_UNSUPPORTED, "write_kv_fp8_block: tokens * num_kv_heads too large (below 2^28)");
   auto* const kernel = shared           ? (bf16 ? write_block_kernel<true, 4, 8> : write_block_kernel<false, 4, 8>)
                        : page_size <= 16 ? (bf16 ? write_block_kernel<true, 1, 4> : write_block_kernel<false, 1, 4>)
                        : page_size <= 32 ? (bf16 ? write_block_kernel<true, 1, 8> : write_block_kernel<false, 1, 8>)
                                          : (bf16 ? write_block_kernel<true, 1, 16> : write_block_kernel<false, 1, 16>);
-  kernel<<<dim3((unsigned)(shared ? units : (units + 3) / 4)), dim3(256), 0, (hipStream_t)stream>>>(a, window);
+  kernel<<<dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream>>>(a, window);
   return launched("write_kv_fp8_block");
 }
 

@@ -79,6 +79,19 @@ def test_c_abi_refusals(call, overrides, status, text):
     assert text in pkv_native.last_error()
 
 
+@pytest.mark.parametrize("call,overrides,status,text", [
+    # Launches of 2^32 threads and more, which HIP does not take.
+    (_prefill, dict(batch=1 << 23, tokens=1, hkv=2), 2, "too many"),
+    (_prefill, dict(batch=1, tokens=(1 << 30) - 1, hq=2, qs=256, hkv=2), 2, "too many"),
+    (_write, dict(tokens=1 << 28, hkv=1), 2, "2^28"), (_write, dict(tokens=1 << 27, hkv=2), 2, "2^28"),
+    (_write, dict(block=True, ps=128, tokens=1 << 28, hkv=1), 2, "2^28"),
+    (_decode, dict(batch=1 << 13, hq=1 << 11, hkv=1 << 11), 2, "2^24"),
+])
+def test_c_abi_refuses_launches_past_the_grid(call, overrides, status, text):
+    assert call(**overrides) == status
+    assert text in pkv_native.last_error()
+
+
 def test_c_abi_empty_calls_are_no_ops():
     assert _prefill(tokens=0) == 0 and _prefill(batch=0) == 0
     assert _write(tokens=0) == 0 and _write(block=True, tokens=0) == 0

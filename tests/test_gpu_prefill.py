@@ -149,6 +149,13 @@ def test_contiguous_and_offset_inputs(ext, gpu):
     assert torch.equal(q, ref)
 
 
+def test_thousands_of_sequences(ext, gpu):
+    """More sequences than two rounds of the search for a block's tell apart (63^2)."""
+    lengths = [(7 * i) % 3 for i in range(4100)] + [200, 1]
+    qkv, off = packed_inputs(lengths, 4, 2, F16, seed=21)
+    _check(ext, gpu, qkv, off, 4, 2)
+
+
 def test_bad_offsets_stay_inside(ext, gpu):
     """Offsets past the tokens, or negative, count as clamped."""
     qkv, _ = packed_inputs([200], 4, 2, F16, seed=9)

@@ -95,3 +95,62 @@ def test_prompts_then_decode_steps(ext, gpu, dtype, block_scaled):
     assert counts[0].item() == pages - used
     ids = torch.cat([table[b, :-(-(n + 19) // ps)] for b, n in enumerate(lengths)])
     assert len(set(ids.tolist())) == used  # no page twice
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_captured_decode_step(ext, gpu, dtype):
+    """One captured graph of a whole step (pages and slots, the write, attention, lengths one
+    further), replayed 40 times with new tokens: as the same calls made one by one."""
+    hq, hkv, ps, columns, lengths, pages = 8, 2, 16, 12, [33, 1, 127, 16], 40
+    rows, gen = len(lengths), torch.Generator().manual_seed(17)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu)
+    free = torch.randperm(pages, generator=gen).to(torch.int32).to(gpu)
+    prompts = [torch.randn(sum(lengths), hkv, 128, generator=gen).to(dtype).to(gpu) for _ in range(2)]
+
+    class Loop:
+        def __init__(self):
+            self.pools = [torch.zeros(pages, hkv, ps, 128, device=gpu).to(F8) for _ in range(2)]
+            self.scales = torch.ones(pages, hkv, 2, device=gpu)
+            self.table = torch.full((rows, columns), -1, dtype=torch.int32, device=gpu)
+            self.cached, self.lens, self.num_free, self.left = i32([0] * rows), i32(lengths), i32([pages]), i32([0])
+            self.offsets = i32([0] * (rows + 1))
+            self.qkv = torch.zeros(rows, hq + 2 * hkv, 128, dtype=dtype, device=gpu)
+            self.out = torch.zeros(rows, hq, 128, dtype=dtype, device=gpu)
+            self.workspace = torch.empty(ext.fp8_block_workspace_floats(rows, hq, hkv), device=gpu)
+            self.admit(*prompts)
+
+        def admit(self, k, v):
+            slots = i32([0] * k.shape[0])
+            ext.build_block_tables(self.cached, self.lens, free, self.num_free, self.table, self.offsets, slots, self.left, ps)
+            ext.write_kv_fp8_block(k, v, *self.pools, self.scales, slots)
+            self.slots = i32([0] * rows)
+            self.further()
+
+        def further(self):
+            self.num_free.copy_(self.left)
+            self.cached.copy_(self.lens)
+            self.lens.add_(1)
+
+        def step(self):
+            ext.build_block_tables(self.cached, self.lens, free, self.num_free, self.table, self.offsets, self.slots, self.left, ps)
+            ext.write_kv_fp8_block(self.qkv[:, hq:hq + hkv], self.qkv[:, hq + hkv:], *self.pools, self.scales, self.slots)
+            ext.paged_attention_fp8_block(self.qkv[:, :hq].contiguous(), *self.pools, self.scales, self.table, self.lens,
+                                          self.out, self.workspace, ps)
+            self.further()
+
+    eager, captured = Loop(), Loop()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # records, and runs nothing
+        captured.step()
+    for n in range(40):
+        new = torch.randn(rows, hq + 2 * hkv, 128, generator=gen).to(dtype) * (1 + n % 7)
+        for x in (eager, captured):
+            x.qkv.copy_(new)
+        eager.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured.out, eager.out) and torch.isfinite(eager.out).all(), n
+        assert torch.equal(captured.table, eager.table) and torch.equal(captured.num_free, eager.num_free)
+        assert torch.equal(captured.scales, eager.scales)
+    assert captured.num_free.item() == pages - sum(-(-(n + 40) // ps) for n in lengths)

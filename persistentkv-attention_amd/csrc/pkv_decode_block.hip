@@ -16,7 +16,8 @@
 // once.  Every workgroup computes the cut from the lengths (a scan in LDS), so nothing is
 // planned on the host and the call can be captured for lengths that change.  A pair inside one
 // share is written to the output, the others as partial states, at most two a wave, and
-// joined by the merge kernel.
+// joined by the merge kernel.  Tables of few tokens take one launch instead, a workgroup a pair
+// (short_block_kernel).
 //
 // Per wave and tile: K and V straight from the pages into registers (16- and 8-byte buffer
 // loads whose descriptor ends with the row's last token), S^T = K Q^T and O^T += V^T P^T on
@@ -47,6 +48,8 @@ constexpr int kMinShare = 2;         // positions of a share
 constexpr int kMaxRows = 16000;      // an LDS prefix of 4 bytes a row
 constexpr int kStateFloats = kD + 2; // acc, m, l
 constexpr int kMergeWaves = 4;
+constexpr int kShortWaves = 8;       // of a workgroup that takes a (row, KV head) of a short table,
+constexpr int kShortTokens = 512;    // which addresses at most this many tokens (see there)
 constexpr int kKvLoadPolicy = 2;     // non-temporal: K/V bytes are read once
 constexpr uint32_t kRsrcWord3 = 0x00020000u;  // raw buffer, 32-bit data format (gfx9 family)
 constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
@@ -276,9 +279,11 @@ __device__ inline u32x4 pack8(const f32x4 (&o)[8], int i, float f) {
                Elem::pack2(o[4][i] * f, o[5][i] * f), Elem::pack2(o[6][i] * f, o[7][i] * f)};
 }
 
-// Tiles [t0, t1) of (row, kvh).  `state` < 0: the whole pair, written to the output.
+// Tiles [t0, t1) of (row, kvh).  `state` < 0: the whole pair, written to the output; else that
+// place in `states` and `ml`.
 template <class Elem, int HB>
-__device__ void piece(const BlockArgs& a, int row, int kvh, int t0, int t1, int state, int lane) {
+__device__ void piece(const BlockArgs& a, int row, int kvh, int t0, int t1, int state, float* states,
+                      f32x2* ml, int lane) {
   const int c = lane & 15, g = lane >> 4;
   Stream stream{a, a.block_table + (long)row * a.max_pages, kvh, 0, lane};
   Pages pa = stream.lookup(t0), pb = stream.lookup(t0 + 1);
@@ -326,8 +331,8 @@ __device__ void piece(const BlockArgs& a, int row, int kvh, int t0, int t1, int 
       for (int i = 0; i < 4; ++i) out[i] = pack8<Elem>(st.o[hb], i, inv);
     } else {
       const long at = (long)state * a.group + head;
-      if (g == 0) a.ml[at] = f32x2{st.m[hb], l};
-      f32x4* acc = (f32x4*)(a.acc + at * kD + g * 32);
+      if (g == 0) ml[at] = f32x2{st.m[hb], l};
+      f32x4* acc = (f32x4*)(states + at * kD + g * 32);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -410,7 +415,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_block_kernel(BlockArgs a) 
     const int t0 = max((int)(x - at) - kPieceCost, 0), t1 = (int)(stop - at) - kPieceCost;
     if (t1 > t0) {
       const bool first = at + kPieceCost >= w * share, last = stop == at + n;
-      piece<Elem, HB>(a, row, (int)h, t0, t1, first && last ? -1 : (int)(2 * w + (first ? 1 : 0)), lane);
+      piece<Elem, HB>(a, row, (int)h, t0, t1, first && last ? -1 : (int)(2 * w + (first ? 1 : 0)), a.acc, a.ml, lane);
     }
     x = stop;
   }
@@ -484,6 +489,44 @@ __global__ __launch_bounds__(kMergeWaves * 64) void merge_block_kernel(BlockArgs
   }
 }
 
+// Tables of few tokens: a workgroup takes a (row, KV head), its waves the tiles in equal parts,
+// and joins their states in LDS.  One launch, no cut and no plan (32 / 8 heads, fp16, 1 row: 64
+// tokens 3.8 us where the cut takes 6.6, 512 tokens 7.1 and 8.4; 32 rows: 4.1 and 7.0, 9.1 and
+// 14.2; 64 rows of 512: 16.3 and 20.1).  A CU by itself gets 34 GB/s, so 1024 tokens of one row
+// take 10.9 where the cut over all CUs takes 8.9; only pairs for every CU make up for that (32
+// rows of 1024: 14.0 and 19.2, of 1-1024: 12.6 and 14.7; 40 rows, the worst: 23.3 and 22.1).  Past two
+// pairs a CU the starts count: 128 rows of 512 take 30.1 and 26.3.
+template <class Elem>
+__global__ __launch_bounds__(kShortWaves * 64) void short_block_kernel(BlockArgs a) {
+  __shared__ __attribute__((aligned(16))) float states[kShortWaves * 16 * kD];  // [wave, head, 128]
+  __shared__ f32x2 ml[kShortWaves * 16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int row = uniform((int)(blockIdx.x / (unsigned)a.hkv)), kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
+  const int tiles = (clamp_length(a, load_scalar(a.seq_lens + row)) + kTile - 1) / kTile;
+  const int n = min(tiles, kShortWaves);
+  if (wave < n)
+    piece<Elem, 1>(a, row, kvh, wave * tiles / n, (wave + 1) * tiles / n, n == 1 ? -1 : wave, states, ml, lane);
+  if (n == 1) return;
+  __syncthreads();
+  uint8_t* const out = a.output + (long)blockIdx.x * a.group * (2 * kD);
+  for (int i = tid; i < a.group * (kD / 4); i += kShortWaves * 64) {
+    const int head = i / (kD / 4);
+    float m = -INFINITY, l = 0.f;
+    for (int w = 0; w < n; ++w) m = fmaxf(m, ml[w * a.group + head][0]);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < n; ++w) {
+      const f32x2 y = ml[w * a.group + head];
+      const float f = __builtin_amdgcn_exp2f(y[0] - m);
+      const f32x4 x = *(const f32x4*)(states + w * a.group * kD + 4 * i);
+      l = __builtin_fmaf(y[1], f, l);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(x[j], f, sum[j]);
+    }
+    const float inv = n ? 1.0f / l : 0.f;  // no token: zero
+    *(u32x2*)(out + i * 8) = u32x2{Elem::pack2(sum[0] * inv, sum[1] * inv), Elem::pack2(sum[2] * inv, sum[3] * inv)};
+  }
+}
+
 size_t workspace_bytes(int64_t batch, int64_t hkv, int64_t group) {
   const size_t states = 2 * (size_t)pkv::compute_units() * kWaves * group * kStateFloats * sizeof(float);
   return states + (size_t)batch * hkv * sizeof(int2);
@@ -491,6 +534,13 @@ size_t workspace_bytes(int64_t batch, int64_t hkv, int64_t group) {
 
 template <class Elem, int HB>
 void launch(const BlockArgs& a, hipStream_t s) {
+  if constexpr (HB == 1) {
+    const int pairs = a.batch * a.hkv, cus = a.waves / kWaves;
+    if (a.max_pages * a.page_size <= (pairs < cus ? kShortTokens : 2 * kShortTokens) && pairs <= 2 * cus) {
+      short_block_kernel<Elem><<<dim3((unsigned)(a.batch * a.hkv)), dim3(kShortWaves * 64), 0, s>>>(a);
+      return;
+    }
+  }
   const size_t lds = (size_t)(a.batch + 1 + kWaves) * sizeof(uint32_t);
   decode_block_kernel<Elem, HB><<<dim3((unsigned)(a.waves / kWaves)), dim3(kWaves * 64), lds, s>>>(a);
   const long heads = (long)a.batch * a.hkv * a.group;

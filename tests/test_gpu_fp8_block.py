@@ -62,6 +62,53 @@ def test_lengths(ext, gpu, lengths, page_size, dtype):
     _check(ext, gpu, _case(lengths, 8, 2, page_size, dtype, seed=sum(lengths)), f"{lengths[:5]} pages of {page_size}")
 
 
+@pytest.mark.parametrize("lengths", [[1], [15, 16, 17], [31, 32, 33, 0, 1], [500], [0, 0], [512, 3, 64, 65, 130], [33] * 90], ids=str)
+@pytest.mark.parametrize("columns", [32, 33, 400])
+@pytest.mark.parametrize("hq,hkv,dtype", [(8, 2, F16), (16, 1, BF16), (17, 1, F16), (3, 3, BF16)])
+def test_lengths_under_short_and_wide_tables(ext, gpu, lengths, columns, hq, hkv, dtype):
+    """Tables of 512 tokens, a page more, and many: each way to share the work out."""
+    _check(ext, gpu, _case(lengths, hq, hkv, 16, dtype, seed=columns + len(lengths), columns=columns), f"{lengths[:5]} of {16 * columns}")
+
+
+@pytest.mark.parametrize("rows,columns,longest", [(512, 16, 300), (513, 16, 300), (255, 32, 200), (256, 32, 1024), (300, 33, 200)])
+def test_rows_of_short_tables(ext, gpu, rows, columns, longest):
+    """About a row and two rows a CU, between which a table of up to 1024 tokens is short too."""
+    rng = np.random.default_rng(rows)
+    lengths = rng.integers(0, 60, rows)
+    lengths[::9] = rng.integers(0, longest + 1, len(lengths[::9]))
+    _check(ext, gpu, _case(lengths.tolist(), 2, 1, 32, BF16, seed=rows, columns=columns), f"{rows} rows")
+
+
+def test_scales_far_apart_in_a_wide_table(ext, gpu):
+    """Pages whose V is 2^40 larger than others', through the cut over all CUs."""
+    case = _case([200, 65, 400], 4, 2, 16, F16, seed=3, columns=64)
+    scales = case[3]
+    scales[:, :, 0] = 2.0 ** -8
+    scales[::2, :, 1] = 2.0 ** -40
+    _check(ext, gpu, case, "2^40 apart")
+
+
+def test_short_tables_in_place_and_replayed(ext, gpu):
+    cases = [_case([300, 33, 0, 512], 8, 2, 16, F16, seed=s, columns=32) for s in (31, 32)]
+    refs = [_check(ext, gpu, c) for c in cases]
+    dev = [[x.to(gpu) for x in c] for c in cases]
+    q = dev[0][0].clone()
+    ws = torch.empty(ext.fp8_block_workspace_floats(4, 8, 2), device=gpu)
+    ext.paged_attention_fp8_block(q, *dev[0][1:], q, ws, 16)  # output over q
+    assert torch.equal(q, refs[0])
+    ins, out = [x.clone() for x in dev[0]], torch.zeros_like(refs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ext.paged_attention_fp8_block(*ins, out, ws, 16)
+    for i in (0, 1, 0, 1):
+        for x, y in zip(ins, dev[i]):
+            x.view(torch.uint8).copy_(y.view(torch.uint8))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, refs[i])
+
+
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (2, 1), (3, 1), (5, 1), (8, 1), (10, 2), (16, 1), (17, 1), (31, 1), (32, 1), (40, 2), (12, 12)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_head_layouts(ext, gpu, hq, hkv, dtype):

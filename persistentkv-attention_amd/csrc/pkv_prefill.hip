@@ -214,10 +214,13 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
 // 64 x 16 bytes from a buffer straight to LDS, lane l's to `lds` + 16 l.  In assembly because the
 // compiler lets every LDS read wait for every such load in flight, the next tile's among them;
-// landed() is the wait, before the barrier behind which the tile is read.  No registers are
-// written but m0, which nothing else in these kernels uses.
+// landed() is the wait, before the barrier behind which the tile is read.  The compiler keeps no
+// distances to instructions in assembly, so this text carries them: a scalar register written by a
+// vector instruction (the descriptor's, by readfirstlane or as a spilled one brought back) must
+// lie five wait states before the load that reads it (s_mov, and four of s_nop 3), m0 one.  No
+// registers are written but m0, which nothing else in these kernels uses.
 __device__ inline void load_to_lds(uint32_t lds, i32x4 rsrc, uint32_t offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(lds), "v"(offset), "s"(rsrc) : "memory");
 }
 // Waits until at most N of the wave's loads are in flight.

@@ -390,8 +390,8 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void prefill_kern
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
       if constexpr (kFirst) {
-        m = fmaxf(mx, __shfl_xor(mx, 32));
-        if (GROUPS > 1 && m == -INFINITY) m = -FLT_MAX;  // finite where a row sees no key of the tile
+        // Finite where a row sees no key of the tile, or none but of score -inf: weights 0, not NaN.
+        m = fmaxf(fmaxf(mx, __shfl_xor(mx, 32)), -FLT_MAX);
         l = 0.f;
       } else if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
         mx = fmaxf(mx, __shfl_xor(mx, 32));

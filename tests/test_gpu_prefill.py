@@ -123,6 +123,24 @@ def test_scores_at_the_ends_of_the_range(ext, gpu, empty):
     assert torch.isnan(out[90:]).all() and torch.isfinite(out[:90]).all()
 
 
+@pytest.mark.parametrize("empty", [0, 90])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hidden", [31, 32, 40, 64, 70])
+def test_keys_of_minus_infinity(ext, gpu, dtype, hidden, empty):
+    """Keys whose scores are -inf have no weight: a row that sees none but such is NaN, and the
+    later ones are as if the sequence began behind them, whole tiles of them or not."""
+    qkv, off = packed_inputs([200] + [0] * empty, 4, 2, dtype, seed=hidden)
+    qkv[:, :4, 0] = 1.0
+    qkv[:hidden, 4:6, 0] = -float("inf")
+    out = torch.zeros(200, 4, 128, dtype=dtype, device=gpu)
+    ext.prefill_attention(*split_qkv(qkv.to(gpu), 4, 2), off.to(gpu), out)
+    assert torch.isnan(out[:hidden]).all()
+    q, k, v = (x[hidden:].double() for x in split_qkv(qkv, 4, 2))
+    want, weight, vmax, score = prompt.prefill(q, k, v, [0, 200 - hidden])
+    tiny = 200 * 2.0 ** -25 * vmax if dtype == F16 else 0.0
+    assert_within(out[hidden:], want, attention_tolerance(want, weight, score, 200, dtype, U[dtype], tiny), f"behind {hidden}")
+
+
 def test_token_strides_at_their_limit(ext, gpu):
     """2^23 elements between the tokens of K: 300 of them pass 2^32 bytes."""
     qkv, off = packed_inputs([10, 290], 4, 2, F16, seed=12)

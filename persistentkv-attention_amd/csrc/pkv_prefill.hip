@@ -57,6 +57,10 @@ constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // log
 // The running maximum is replaced only when a score passes it by more than 2^8 in weight:
 // the output is rescaled in few tiles, and weights stay below 2^8, far inside fp16's range.
 constexpr float kSlack = 8.0f / kScaleLog2;
+// Weights are 2^(s c - M c), c = kScaleLog2, in one multiply-add.  M c is rounded: a factor that all
+// of a row's weights share, within 2^-13 of 1 for |M| below 2^14 but of any size for larger ones
+// (2^32 at |M| = 2^32: past fp16's range, or below it).  From 2^14 on it is (s - M) c.
+constexpr float kLargeScore = 0x1p14f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -334,6 +338,7 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void prefill_kern
 
   f32x16 o[4];
   float m, l;
+  bool large = false;  // a row of the wave has a large maximum
   const uint8_t* kat[8];
   const uint8_t* vat[4];
 #pragma unroll
@@ -393,18 +398,25 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void prefill_kern
         // Finite where a row sees no key of the tile, or none but of score -inf: weights 0, not NaN.
         m = fmaxf(fmaxf(mx, __shfl_xor(mx, 32)), -FLT_MAX);
         l = 0.f;
+        large = __builtin_amdgcn_ballot_w64(fabsf(m) >= kLargeScore) != 0;
       } else if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float mn = fmaxf(m, mx);
         const float c = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2);
         m = mn;
+        large = __builtin_amdgcn_ballot_w64(fabsf(m) >= kLargeScore) != 0;
         l *= c;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[db][i] *= c;
       }
-      const float ms = m * kScaleLog2;
+      float ms = m * kScaleLog2;
+      if (large) {
+        ms = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] -= m;
+      }
       u32x4 p[2];
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {

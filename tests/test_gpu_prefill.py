@@ -124,6 +124,34 @@ def test_scores_at_the_ends_of_the_range(ext, gpu, empty):
 
 
 @pytest.mark.parametrize("empty", [0, 90])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_large_scores(ext, gpu, dtype, sign, empty):
+    """Scores that are exact in 32 bits, about 2^32 (fp16) and 2^100 (bf16), and no powers of two:
+    their scaled value is rounded by tens of units and more, and the weights must not show it.
+    The tokens with the largest score share all the weight, 1 each, so that only the mean's own
+    arithmetic and the output's rounding are left."""
+    qkv, off = packed_inputs([90, 40] + [0] * empty, 2, 1, dtype, seed=13)
+    qkv[:, :3] = 0.0
+    steps = torch.arange(130) % 3
+    if dtype == F16:  # four products of 22 bits
+        qkv[:, :2, :4] = 16.0 * 2047
+        qkv[:, 2, :4] = (sign * 16.0 * ((2039 if sign > 0 else 2037) - sign * steps))[:, None].to(dtype)
+    else:
+        qkv[:, :2, 0] = 255.0 * 2.0 ** 42
+        qkv[:, 2, 0] = (sign * 2.0 ** 42 * (249 - sign * steps)).to(dtype)
+    out = torch.zeros(130, 2, 128, dtype=dtype, device=gpu)
+    ext.prefill_attention(*split_qkv(qkv.to(gpu), 2, 1), off.to(gpu), out)
+    for first, last in ((0, 90), (90, 130)):
+        v, s = qkv[first:last, 3].double(), steps[first:last]
+        for i in range(last - first):
+            tied = s[:i + 1] == s[:i + 1].min()
+            want, most = v[:i + 1][tied].mean(0), v[:i + 1][tied].abs().max()
+            bound = U[dtype] * want.abs() + 200 * 2.0 ** -24 * most + 2.0 ** -25
+            assert ((out[first + i].cpu().double() - want).abs() <= bound).all(), (first, i)
+
+
+@pytest.mark.parametrize("empty", [0, 90])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("hidden", [31, 32, 40, 64, 70])
 def test_keys_of_minus_infinity(ext, gpu, dtype, hidden, empty):

@@ -169,6 +169,20 @@ def test_keys_of_minus_infinity(ext, gpu, dtype, hidden, empty):
     assert_within(out[hidden:], want, attention_tolerance(want, weight, score, 200, dtype, U[dtype], tiny), f"behind {hidden}")
 
 
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 3)])
+@pytest.mark.parametrize("nats", [10.0, 10.4, 11.0])
+def test_many_weights_below_the_normal_range(ext, gpu, hq, hkv, nats):
+    """One key ahead of 4999 equal ones by so much that their fp16 weights, 2^-14.4 to 2^-15.9, are
+    subnormal, and 0.08 to 0.23 of the sum together; V of one sign.  With rows' tiles shared out
+    over two pairs of waves (one KV head) and not."""
+    qkv, off = packed_inputs([5000], hq, hkv, F16, seed=14)
+    qkv[:, :hq] = 1.0
+    qkv[:, hq:hq + hkv] = 0.0
+    qkv[0, hq:hq + hkv] = nats * 128 ** 0.5 / 128
+    qkv[:, hq + hkv:] = 1.0 + qkv[:, hq + hkv:].abs()
+    _check(ext, gpu, qkv, off, hq, hkv, f"{nats} nats ahead")
+
+
 def test_token_strides_at_their_limit(ext, gpu):
     """2^23 elements between the tokens of K: 300 of them pass 2^32 bytes."""
     qkv, off = packed_inputs([10, 290], 4, 2, F16, seed=12)

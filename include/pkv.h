@@ -359,8 +359,9 @@ int pkv_build_block_tables(
 /* Causal attention over whole prompts: sequence b is the tokens [token_offsets[b],
  * token_offsets[b + 1]) of q [tokens, num_q_heads, 128] and of k, v [tokens, num_kv_heads,
  * 128]; its token i attends to its tokens 0 ... i.  output [tokens, num_q_heads, 128],
- * contiguous; rows outside every sequence are left as they are.  It may be q itself, but must
- * not overlap k or v.  Offsets must not decrease and count as clamped to [0, tokens].
+ * contiguous; rows outside every sequence are left as they are.  It may be q itself if q is
+ * contiguous too (q_stride = num_q_heads * 128, or one token); otherwise it must not overlap q,
+ * and never k or v (refused).  Offsets must not decrease and count as clamped to [0, tokens].
  * G = num_q_heads / num_kv_heads in [1, 32]; (tokens * G / 128 + batch) * num_kv_heads must be
  * below 2^24.  An infinity or NaN in K or V reaches the tokens from its own on, and no other. */
 int pkv_prefill_attention(

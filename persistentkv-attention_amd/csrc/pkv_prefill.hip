@@ -551,8 +551,16 @@ extern "C" int pkv_prefill_attention(
     return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: null pointer");
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)output) & 15)
     return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: tensors must be 16-byte aligned");
-  if (output == k || output == v)
-    return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: output must not be k or v");
+  // Blocks read K and V, and other blocks' rows of q, until the last one ends: only a q whose rows
+  // are the output's own may be written over.
+  const int64_t row = (int64_t)num_q_heads * kRowBytes, kv_row = (int64_t)num_kv_heads * kRowBytes;
+  if (pkv::meets_rows(output, tokens * row, k, tokens, 2 * k_stride, kv_row) ||
+      pkv::meets_rows(output, tokens * row, v, tokens, 2 * v_stride, kv_row))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "prefill_attention: output must not be k or v, nor overlap them");
+  if (!(output == q && (tokens == 1 || 2 * q_stride == row)) &&
+      pkv::meets_rows(output, tokens * row, q, tokens, 2 * q_stride, row))
+    return fail(PKV_ERR_INVALID_ARGUMENT,
+                "prefill_attention: output must be a contiguous q itself, or not overlap q");
   const PrefillArgs a{(const uint8_t*)q, (const uint8_t*)k, (const uint8_t*)v, token_offsets,
                       (uint8_t*)output, 2 * q_stride, 2 * k_stride, 2 * v_stride,
                       batch, tokens, num_q_heads, num_kv_heads, group, 1.0f / (float)group};

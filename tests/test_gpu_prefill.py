@@ -209,6 +209,38 @@ def test_contiguous_and_offset_inputs(ext, gpu):
     assert torch.equal(q, ref)
 
 
+def test_outputs_over_and_beside_the_inputs(ext, gpu):
+    """A fused projection whose rows lie apart may not be written over, but for one token; memory
+    that ends where an input begins, and lies between an input's rows, may be."""
+    qkv, off = packed_inputs([40, 25], 8, 2, F16, seed=15)
+    ref = _check(ext, gpu, qkv, off, 8, 2)
+    fused = qkv.to(gpu)
+    parts = split_qkv(fused, 8, 2)
+    over = fused.view(-1)[:65 * 8 * 128].view(65, 8, 128)
+    for out, message in ((over, "must not be k or v"), (fused.view(-1)[128:65 * 8 * 128 + 128].view(65, 8, 128), "must not be k or v")):
+        with pytest.raises(RuntimeError, match=message):
+            ext.prefill_attention(*parts, off.to(gpu), out)
+    with pytest.raises(RuntimeError, match="not overlap q"):
+        ext.prefill_attention(parts[0], *(x.contiguous() for x in parts[1:]), off.to(gpu), over)
+    assert torch.equal(fused.cpu(), qkv)
+    one, one_off = packed_inputs([1], 8, 2, F16, seed=16)
+    want = _check(ext, gpu, one, one_off, 8, 2)
+    fused = one.to(gpu)
+    q, k, v = split_qkv(fused, 8, 2)
+    ext.prefill_attention(q, k, v, one_off.to(gpu), q)
+    assert torch.equal(fused[:, :8], want) and torch.equal(fused[:, 8:].cpu(), one[:, 8:])
+    wide = torch.zeros(2 * 65 * 12 * 128, dtype=F16, device=gpu)  # the inputs, and the output right behind them
+    wide[:65 * 12 * 128].view(65, 12, 128).copy_(qkv)
+    out = wide[65 * 12 * 128:][:65 * 8 * 128].view(65, 8, 128)
+    ext.prefill_attention(*split_qkv(wide[:65 * 12 * 128].view(65, 12, 128), 8, 2), off.to(gpu), out)
+    assert torch.equal(out, ref)
+    apart = torch.zeros(65, 12 + 65 * 8, 128, dtype=F16, device=gpu)  # and between the first two rows
+    apart[:, :12].copy_(qkv)
+    out = apart[0, 12:]
+    ext.prefill_attention(*split_qkv(apart[:, :12], 8, 2), off.to(gpu), out.view(65, 8, 128))
+    assert torch.equal(out.view(65, 8, 128), ref)
+
+
 def test_thousands_of_sequences(ext, gpu):
     """More sequences than two rounds of the search for a block's tell apart (63^2)."""
     lengths = [(7 * i) % 3 for i in range(4100)] + [200, 1]

@@ -92,6 +92,24 @@ def test_c_abi_refuses_launches_past_the_grid(call, overrides, status, text):
     assert text in pkv_native.last_error()
 
 
+FUSED = dict(qs=1536, ks=1536, vs=1536, k=ctypes.c_void_p(0x10800), v=ctypes.c_void_p(0x10a00), q=ctypes.c_void_p(0x10000))
+
+
+@pytest.mark.parametrize("overrides,text", [
+    # q, k, v: column ranges of four rows of 0xc00 bytes from 0x10000 on; the output takes 0x2000 bytes
+    (dict(**FUSED, out=ctypes.c_void_p(0x10000)), "must not be k or v"),            # over the first rows
+    (dict(**FUSED, out=ctypes.c_void_p(0x12ff0)), "must not be k or v"),            # the last 16 bytes of v
+    (dict(**FUSED, out=ctypes.c_void_p(0xe010)), "not overlap q"),                  # the first 16 bytes of q
+    (dict(**{**FUSED, "k": FAKE, "v": FAKE}, out=ctypes.c_void_p(0x10000)), "not overlap q"),  # at q, whose rows lie apart
+    (dict(q=ctypes.c_void_p(0x10000), out=ctypes.c_void_p(0x10800)), "not overlap q"),   # a contiguous q, one row on
+    (dict(q=ctypes.c_void_p(0x10800), out=ctypes.c_void_p(0x10000)), "not overlap q"),   # and one row before
+    (dict(v=ctypes.c_void_p(0x9ff0)), "must not be k or v"), (dict(k=ctypes.c_void_p(0x7810)), "must not be k or v"),
+])
+def test_prefill_refuses_outputs_over_its_inputs(overrides, text):
+    assert _prefill(**overrides) == 1
+    assert text in pkv_native.last_error()
+
+
 def test_c_abi_empty_calls_are_no_ops():
     assert _prefill(tokens=0) == 0 and _prefill(batch=0) == 0
     assert _write(tokens=0) == 0 and _write(block=True, tokens=0) == 0

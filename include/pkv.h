@@ -400,7 +400,8 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
  * into the pool.  At most 16000 rows, and fewer than 2^24 output rows (batch * num_q_heads).
  * The workspace is required:
  * pkv_fp8_block_workspace_bytes on the same device, for any lengths; it holds nothing
- * between calls, and calls that may overlap need one each.  output may be q itself. */
+ * between calls, and calls that may overlap need one each.  output may be q itself, but must not
+ * overlap it otherwise (refused). */
 int pkv_paged_attention_fp8_block(
     const void* q, const void* k_pages, const void* v_pages, const float* kv_scales,
     const int32_t* block_table, const int32_t* seq_lens, void* output, void* workspace,

@@ -592,6 +592,9 @@ int pkv_paged_attention_fp8_block(
   if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)output | (uintptr_t)workspace) & 15 ||
       (uintptr_t)kv_scales & 7)
     return fail(PKV_ERR_INVALID_ARGUMENT, "paged_attention_fp8_block: tensors must be 16-byte aligned");
+  const int64_t bytes = (int64_t)batch * num_q_heads * (2 * kD);
+  if (output != q && pkv::meets_rows(output, bytes, q, 1, bytes, bytes))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "paged_attention_fp8_block: output must be q itself, or not overlap q");
   const size_t need = workspace_bytes(batch, num_kv_heads, group);
   if (!workspace || workspace_size < need)
     return fail(PKV_ERR_WORKSPACE_TOO_SMALL, "paged_attention_fp8_block: workspace of %zu bytes, %zu needed",

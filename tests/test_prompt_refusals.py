@@ -110,6 +110,12 @@ def test_prefill_refuses_outputs_over_its_inputs(overrides, text):
     assert text in pkv_native.last_error()
 
 
+@pytest.mark.parametrize("out", [0x1100, 0x17f0, 0x810])
+def test_decode_refuses_outputs_over_a_part_of_q(out):
+    assert _decode(out=ctypes.c_void_p(out)) == 1
+    assert "not overlap q" in pkv_native.last_error()
+
+
 def test_c_abi_empty_calls_are_no_ops():
     assert _prefill(tokens=0) == 0 and _prefill(batch=0) == 0
     assert _write(tokens=0) == 0 and _write(block=True, tokens=0) == 0

@@ -385,8 +385,9 @@ int pkv_write_kv(const void* k_new, int64_t k_stride, const void* v_new, int64_t
  * written offset is 0 starts anew.  Otherwise the tokens before it stay: the scale is at
  * least the old one (rounded up to a power of two), and where it grows, those tokens are
  * stored again under it (exact but for subnormals).  The tokens of one page must follow one
- * another in slot_mapping in ascending slots, and a slot may occur only once in a call; a
- * call that breaks this leaves the pages concerned with unspecified values. */
+ * another in slot_mapping, each in the slot behind its predecessor's, without gaps; a call that
+ * breaks this (slots 5 and 7 of a page, a page's tokens in two places, a slot twice) leaves the
+ * pages concerned with unspecified values. */
 int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_new,
                            int64_t v_stride, void* k_pages, void* v_pages, float* kv_scales,
                            const int32_t* slot_mapping, int32_t tokens, int32_t num_kv_heads,

@@ -110,7 +110,8 @@ def clamp_scale(s):
 
 def write_kv_fp8_block(pages, scales, new, slots):
     """(pool values, scales) of one tensor (K or V) after the new tokens: ``pages``
-    [pages, hkv, ps, 128] e4m3 values as float64, ``scales`` [pages, hkv]."""
+    [pages, hkv, ps, 128] e4m3 values as float64, ``scales`` [pages, hkv].  A page's tokens
+    must be one run of consecutive slots: anything else has no defined result."""
     pages, scales = np.array(pages, dtype=np.float64), np.array(scales, dtype=np.float64)
     new = np.asarray(new, dtype=np.float64)
     ps = pages.shape[2]
@@ -120,6 +121,8 @@ def write_kv_fp8_block(pages, scales, new, slots):
             runs.setdefault(int(slot) // ps, []).append((int(slot) % ps, t))
     for page, run in runs.items():
         first = run[0][0]
+        if any(b[0] != a[0] + 1 or b[1] != a[1] + 1 for a, b in zip(run, run[1:])):
+            raise ValueError(f"page {page}: tokens that are not one run of consecutive slots")
         for h in range(pages.shape[1]):
             x = np.stack([new[t, h] for _, t in run])
             amax = np.abs(np.where(np.isfinite(x), x, 0.0)).max()

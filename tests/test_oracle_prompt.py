@@ -75,6 +75,14 @@ def test_block_write_grows_a_scale():
     assert got[1, 0, 1, 0] == 224.0  # 224.5 to a step of 16
 
 
+@pytest.mark.parametrize("slots", [[5, 7], [7, 6], [3, 20, 4], [3, -1, 4], [3, 3]], ids=str)
+def test_block_write_takes_a_page_as_one_run(slots):
+    """Without gaps, in order and in one place: what the operator's header asks for."""
+    with pytest.raises(ValueError, match="one run of consecutive slots"):
+        prompt.write_kv_fp8_block(np.zeros((2, 1, 16, 128)), np.ones((2, 1)), np.ones((len(slots), 1, 128)), slots)
+    prompt.write_kv_fp8_block(np.zeros((2, 1, 16, 128)), np.ones((2, 1)), np.ones((5, 1, 128)), [14, 15, -1, 16, 17])
+
+
 def test_block_decode_matches_the_decode_oracle():
     rng = np.random.default_rng(2)
     k, v = (prompt.e4m3_round(rng.standard_normal((5, 2, 16, 128)) * 50) for _ in range(2))

@@ -348,6 +348,10 @@ int pkv_workqueue_decode_fp8(
  *   num_free_out  [1]  num_free less the pages taken; negative when that many were missing
  *                 (the entries concerned are -1).  It must not be num_free: the inputs
  *                 stay as they are, and a repeated call gives the same result.
+ * A step with a negative num_free_out must not be used: tokens without a page have no slot, and
+ * the entries of -1 would count as pages held once cached_lens has moved on.  With cached_lens
+ * and num_free as they were, and pages returned to the list or rows left out (seq_lens =
+ * cached_lens), the same call builds it again.
  * num_free [1] counts as clamped to [0, free_capacity].  At most 8000 rows, and 2^31 - 1 new
  * tokens.  Returning pages is the caller's: entries copied to the end of free_pages. */
 int pkv_build_block_tables(

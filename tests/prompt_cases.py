@@ -54,3 +54,33 @@ def assert_within(got, want, bound, what=""):
     worst = float(ratio.max()) if ratio.size else 0.0
     print(f"{what}: at most {worst:.3f} of the bound")
     assert worst <= 1.0, (what, worst)
+
+
+def shortage_and_retry(build):
+    """The documented answer to a list that runs out: the step is not used, rows are left out or
+    pages returned, and it is built again from the same lengths and table.  `build(cached, lens,
+    free, num_free, table, slots, page_size)` gives (table, offsets, slots, num_free_out) as lists."""
+    ps, columns, free = 16, 6, [7, 3, 9, 4, 1, 8] + [-99] * 6  # 3 are held by row 0, 5 and 6 by row 1
+    table = [[0, 2, 11, -1, -1, -1], [5, 6, -1, -1, -1, -1], [-1] * columns]
+    cached, lens = [45, 20, 0], [50, 70, 33]  # 1 + 3 + 3 pages, and 6 are free
+
+    def step(table, lens, free, num_free):
+        new = [max(n - c, 0) for n, c in zip(lens, cached)]
+        table, offsets, slots, left = build(cached, lens, free, num_free, table, sum(new), ps)
+        assert offsets == [sum(new[:i]) for i in range(4)]
+        return table, slots, left
+
+    table, slots, left = step(table, lens, free, 6)
+    assert left == -1 and slots[-1] == -1
+    # row 1 waits: the others have their pages, and its own are untouched
+    t1, slots, left = step(table, [50, 20, 33], free, 6)
+    held = [t1[0][:4], t1[1][:2], t1[2][:3]]
+    assert left == 2 and min(slots) >= 0 and held == [[0, 2, 11, 8], [5, 6], [1, 4, 9]]
+    # or two pages come back, at free_pages[num_free] on: everything fits, each page once
+    free[6:8] = [20, 21]
+    t2, slots, left = step(table, lens, free, 8)
+    held = t2[0][:4] + t2[1][:5] + t2[2][:3]
+    assert left == 1 and min(slots) >= 0 and len(set(held)) == len(held) and min(held) >= 0
+    assert t2[0][:3] == [0, 2, 11] and t2[1][:2] == [5, 6]
+    want = [t2[b][p // ps] * ps + p % ps for b in range(3) for p in range(cached[b], lens[b])]
+    assert slots == want

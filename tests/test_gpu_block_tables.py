@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from oracle import prompt
+from prompt_cases import shortage_and_retry
 
 pytestmark = pytest.mark.gpu
 
@@ -56,6 +57,15 @@ def test_the_list_runs_out(ext, gpu):
     _check(ext, gpu, [0, 5, 0], [20, 50, 90], [3, 1, 2, 9, 8], 4, np.full((3, 8), 6), 160, 16)
     _check(ext, gpu, [0], [20], [3, 1], -3, np.full((1, 8), 6), 20, 16)   # counts as none
     _check(ext, gpu, [0], [50], [3, 1], 99, np.full((1, 8), 6), 50, 16)   # at most the list
+
+
+def test_a_step_is_built_again_after_a_shortage(ext, gpu):
+    def build(cached, lens, free, num_free, table, slots, page_size):
+        t, out, off, left = _i32(table, gpu), _i32([77] * slots, gpu), _i32([77] * (len(cached) + 1), gpu), _i32([77], gpu)
+        ext.build_block_tables(_i32(cached, gpu), _i32(lens, gpu), _i32(free, gpu), _i32([num_free], gpu), t, off, out, left, page_size)
+        return t.tolist(), off.tolist(), out.tolist(), left.item()
+
+    shortage_and_retry(build)
 
 
 def test_shrinking_negative_and_unassigned_rows(ext, gpu):

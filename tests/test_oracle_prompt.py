@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from oracle import attention, prompt
+from prompt_cases import shortage_and_retry
 
 
 def test_tables_by_hand():
@@ -24,6 +25,10 @@ def test_tables_run_out():
     t, _, slots, left = prompt.build_block_tables([0, 0], [4, 9], [3, 4], 2, [[-7] * 3] * 2, 13, 4)
     assert t.tolist() == [[4, -7, -7], [3, -1, -1]] and left == -2
     assert slots.tolist() == [16, 17, 18, 19, 12, 13, 14, 15] + [-1] * 5
+
+
+def test_tables_after_a_shortage():
+    shortage_and_retry(lambda *a: [x.tolist() if hasattr(x, "tolist") else x for x in prompt.build_block_tables(*a)])
 
 
 @pytest.mark.parametrize("lengths,hq,hkv", [([1, 5, 33], 4, 2), ([7], 3, 1)])

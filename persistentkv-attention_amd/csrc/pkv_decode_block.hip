@@ -67,8 +67,15 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // P enters the PV product in the activation type; bf16 keeps 8 bits, so its P is split into
 // two terms (two products), as the framework's other decode kernels split it.
+//
+// kLift: the state's m lies this far below the maximum of y, so that the largest weights are
+// 2^kLift.  Where pages' scales of V are 2^120 apart, a token of a small-scaled page that counts
+// in the sum has a weight next to 2^-126, the end of fp32's range (v_exp gives 0 below it); with
+// 2^30 in hand what is lost there is below 2^-36 of the largest token's share.  fp16's weights
+// have no such room, and scales of V so far apart have no output in fp16.
 struct Half {
   static constexpr int kPasses = 1;
+  static constexpr float kLift = 0.f;
   __device__ static inline f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -83,6 +90,7 @@ struct Half {
 };
 struct BFloat {
   static constexpr int kPasses = 2;
+  static constexpr float kLift = 30.f;
   __device__ static inline f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -195,6 +203,10 @@ struct State {
   f32x4 o[HB][8];       // o[hb][jj][i]: dim 8 (4 (lane / 16) + i) + jj of head 16 hb + lane % 16
 };
 
+// The square root of 2^x.  A state's l is a sum of weights over scales of V, up to 2^60 and more
+// times its weights: 2^x, taken by itself, may be below fp32's range where l 2^x is not.
+__device__ inline float half_weight(float x) { return __builtin_amdgcn_exp2f(0.5f * x); }
+
 template <class Elem, int HB>
 __device__ inline void compute(State<HB>& st, const Tile& r, const u32x4 (&q)[HB][4], int tile,
                                int len, int lane) {
@@ -242,12 +254,12 @@ __device__ inline void compute(State<HB>& st, const Tile& r, const u32x4 (&q)[HB
     float mx = y[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) mx = fmaxf(mx, y[j]);
-    if (__builtin_amdgcn_ballot_w64(mx > st.m[hb] + kSlack) != 0) {
+    if (__builtin_amdgcn_ballot_w64(mx > st.m[hb] + (Elem::kLift + kSlack)) != 0) {
       mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(st.m[hb], fmaxf(mx, __shfl_xor(mx, 32)));
-      const float c = __builtin_amdgcn_exp2f(st.m[hb] - mx);
+      mx = fmaxf(st.m[hb], fmaxf(mx, __shfl_xor(mx, 32)) - Elem::kLift);
+      const float root = half_weight(st.m[hb] - mx), c = root * root;
       st.m[hb] = mx;
-      st.l[hb] *= c;
+      st.l[hb] = st.l[hb] * root * root;
 #pragma unroll
       for (int jj = 0; jj < 8; ++jj) st.o[hb][jj] *= c;
     }
@@ -459,10 +471,12 @@ __global__ __launch_bounds__(kMergeWaves * 64) void merge_block_kernel(BlockArgs
   m = fmaxf(m, own[0]);
 #pragma unroll
   for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  float l = own[1] * __builtin_amdgcn_exp2f(own[0] - m);
+  const float root = half_weight(own[0] - m);
+  float l = own[1] * root * root;
   for (int i = lane + 64; i < n; i += 64) {
     const f32x2 y = a.ml[state(i)];
-    l = __builtin_fmaf(y[1], __builtin_amdgcn_exp2f(y[0] - m), l);
+    const float r = half_weight(y[0] - m);
+    l = __builtin_fmaf(y[1] * r, r, l);
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
@@ -516,9 +530,9 @@ __global__ __launch_bounds__(kShortWaves * 64) void short_block_kernel(BlockArgs
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     for (int w = 0; w < n; ++w) {
       const f32x2 y = ml[w * a.group + head];
-      const float f = __builtin_amdgcn_exp2f(y[0] - m);
+      const float root = half_weight(y[0] - m), f = root * root;
       const f32x4 x = *(const f32x4*)(states + w * a.group * kD + 4 * i);
-      l = __builtin_fmaf(y[1], f, l);
+      l = __builtin_fmaf(y[1] * root, root, l);
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(x[j], f, sum[j]);
     }

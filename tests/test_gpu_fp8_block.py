@@ -150,6 +150,20 @@ def test_scales_far_apart(ext, gpu, dtype):
     _check(ext, gpu, (q, k8.to(F8), v8.to(F8), scales, table, lens), "large V without weight")
 
 
+@pytest.mark.parametrize("tokens,columns", [(400, 32), (400, 64), (4112, 257)])
+def test_scales_at_both_ends(ext, gpu, tokens, columns):
+    """bf16: one page whose V is 2^120 larger than the others', and whose tokens weigh 2^7.1 times as
+    much each.  Next to weight times V's scale the others' are below fp32's range, but they are
+    0.15 to 0.65 of the sum that divides."""
+    q, k8, v8, scales, table, lens = _case([tokens], 4, 2, 16, BF16, seed=10, columns=columns)
+    q[:] = 1.0
+    k8, big = torch.zeros_like(k8.float()), table[0, 3].item()
+    k8[big, :, :, 0] = 56.0
+    scales[:, :, 0], scales[:, :, 1] = 1.0, 2.0 ** -60
+    scales[big, :, 1] = 2.0 ** 60
+    _check(ext, gpu, (q, k8.to(F8), v8, scales, table, lens), f"{tokens} tokens")
+
+
 def test_scales_that_are_no_powers_of_two(ext, gpu):
     case = _case([300, 20], 8, 2, 16, F16, seed=4)
     scales = case[3] * (1 + torch.rand(case[3].shape, generator=torch.Generator().manual_seed(5)))

@@ -107,6 +107,19 @@ def lib():
         _PI32, _PI32, _I32, _PI32, _PI32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
         _PI32, _PI32, _PI32, _PI32, _PI32, _PI32, _PI32, _PI32, _PI32, ctypes.c_int64, _PI64]
     so.pkv_build_buckets.restype = ctypes.c_int
+    # From a prompt to the cache: device pointers, token strides and sizes in 64 bits.
+    ptr, i64, size = ctypes.c_void_p, ctypes.c_int64, ctypes.c_size_t
+    token_major = [ptr, i64, ptr, i64]  # two tensors, each with the stride of its tokens
+    so.pkv_build_block_tables.argtypes = [ptr] * 8 + [_I32] * 5 + [ptr]
+    so.pkv_prefill_attention.argtypes = [ptr, i64] + token_major + [ptr, ptr] + [_I32] * 6 + [ptr]
+    so.pkv_write_kv.argtypes = token_major + [ptr] * 3 + [_I32] * 6 + [ptr]
+    so.pkv_write_kv_fp8_block.argtypes = token_major + [ptr] * 4 + [_I32] * 6 + [ptr]
+    so.pkv_paged_attention_fp8_block.argtypes = [ptr] * 8 + [size] + [_I32] * 8 + [ptr]
+    for f in (so.pkv_build_block_tables, so.pkv_prefill_attention, so.pkv_write_kv,
+              so.pkv_write_kv_fp8_block, so.pkv_paged_attention_fp8_block):
+        f.restype = ctypes.c_int
+    so.pkv_fp8_block_workspace_bytes.argtypes = [_I32] * 3
+    so.pkv_fp8_block_workspace_bytes.restype = size
     _lib = so
     return so
 

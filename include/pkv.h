@@ -367,7 +367,10 @@ int pkv_build_block_tables(
  * contiguous too (q_stride = num_q_heads * 128, or one token); otherwise it must not overlap q,
  * and never k or v (refused).  Offsets must not decrease and count as clamped to [0, tokens].
  * G = num_q_heads / num_kv_heads in [1, 32]; (tokens * G / 128 + batch) * num_kv_heads must be
- * below 2^24.  An infinity or NaN in K or V reaches the tokens from its own on, and no other. */
+ * below 2^24.  An infinity or NaN in K or V reaches the tokens from its own on, and no other (a
+ * key of score -inf has weight 0).  K and V of the call are all that is attended to: tokens that
+ * the cache holds already are not, so a row that continues a cached prefix (cached_lens > 0 in
+ * pkv_build_block_tables) must not go in for its new tokens alone. */
 int pkv_prefill_attention(
     const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
     int64_t v_stride, const int32_t* token_offsets, void* output, int32_t batch, int32_t tokens,
@@ -385,7 +388,9 @@ int pkv_write_kv(const void* k_new, int64_t k_stride, const void* v_new, int64_t
 /* pkv_write_kv into fp8 (OCP e4m3) pools with kv_scales [num_pages, num_kv_heads, 2] (K's
  * scale, V's scale; 8-byte aligned).  Scales are powers of two in [2^-60, 2^60], the smallest
  * with amax <= 448 scale over the finite values the block receives; elements are stored as
- * e4m3(clamp(x / scale, -448, 448)), rounded to nearest even, NaN as NaN.  A page whose first
+ * e4m3(clamp(x / scale, -448, 448)), rounded to nearest even, NaN as NaN.  An infinity is so
+ * stored as 448 scale: the largest value that its block can hold, and 448 * 2^-60 where all of
+ * the block's finite values are zero.  A page whose first
  * written offset is 0 starts anew.  Otherwise the tokens before it stay: the scale is at
  * least the old one (rounded up to a power of two), and where it grows, those tokens are
  * stored again under it (exact but for subnormals).  The tokens of one page must follow one

@@ -24,7 +24,9 @@
 // v_mfma_f32_16x16x32, heads padded to 16 a block.  Two tiles (16 KB) in flight in each of a CU's
 // four waves keep HBM busy: 64 Zipf rows (bf16, G = 8, 600 MB) 97-99 us, 6.1 TB/s; 8 bimodal
 // rows (fp16, G = 4, 95 MB) 19.5 us, 4.9 TB/s, of which about 3 us pass before the first bytes;
-// then 4 to 6 us of merge.
+// then 4 to 6 us of merge.  For G above 16 a wave holds two blocks of heads in 254 registers and
+// takes twice the products a tile: 128 rows of 8192, 32 / 1 heads (268 MB), 62 us and 4.3 TB/s, 64 / 2
+// heads (537 MB) 119 us and 4.5, where 32 rows of 8192 at 32 / 8 (537 MB) take 91 us and 5.9.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -509,7 +511,9 @@ __global__ __launch_bounds__(kMergeWaves * 64) void merge_block_kernel(BlockArgs
 // 14.2; 64 rows of 512: 16.3 and 20.1).  A CU by itself gets 34 GB/s, so 1024 tokens of one row
 // take 10.9 where the cut over all CUs takes 8.9; only pairs for every CU make up for that (32
 // rows of 1024: 14.0 and 19.2, of 1-1024: 12.6 and 14.7; 40 rows, the worst: 23.3 and 22.1).  Past two
-// pairs a CU the starts count: 128 rows of 512 take 30.1 and 26.3.
+// pairs a CU the starts count: 128 rows of 512 take 30.1 and 26.3.  For G up to 16 only: the states of
+// 32 heads would take 128 KB of LDS; larger groups go through the cut (1 row of 400 tokens, 32 / 1
+// heads: 10.4 us).
 template <class Elem>
 __global__ __launch_bounds__(kShortWaves * 64) void short_block_kernel(BlockArgs a) {
   __shared__ __attribute__((aligned(16))) float states[kShortWaves * 16 * kD];  // [wave, head, 128]

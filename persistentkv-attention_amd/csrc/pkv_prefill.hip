@@ -19,14 +19,21 @@
 //   (the k order of a product is free as long as both operands agree), V^T's A operand comes
 //   from row-major V in LDS through the transposing reads (ds_read_b64_tr_b16).
 // P is rounded to the activation type (half a step of it, as the operand must be), and the sum
-// that divides is that of the rounded weights; scores, sums and outputs are in 32 bits.
+// that divides is that of the rounded weights; scores, sums and outputs are in 32 bits.  The
+// decode kernels add a second bf16 term of P: they wait for memory, and its products cost
+// little.  Here products are what bounds it, and a second term is half as many again: bf16
+// outputs are 1.9e-3 to 2.0e-3 from the exact ones (relative 2-norm), where 32-bit weights give
+// 1.5e-3 to 1.6e-3, the output's own rounding.
 //
 // Three workgroups run on a CU (168 registers, 48 KB of LDS each), so that one's softmax and
 // waits lie under another's products; K/V pass from memory to LDS without registers, two tiles
-// ahead.  Two prompts of 8192 (Hq 32, Hkv 8, bf16): 0.95-0.975 ms, 1.13-1.16 PFLOP/s, 0.9 of
-// what a library product of 8192^3 reaches; bounded by power (1.55-1.7 GHz with the matrix units
-// busy 62-64 % of the cycles; the products alone take 0.815 ms).  32 prompts of 16-1024: 125 us,
-// 640 TFLOP/s, a third of it the start and end of each workgroup.
+// ahead.  The compiler spills 4 (fp16) or 6 (bf16) vector registers to 20 bytes of scratch and 43
+// scalars to lanes of vector registers, and brings them back before the first tile, right
+// behind its scores or after the last one; the kernel for few blocks spills 55 scalars.  Two
+// prompts of 8192 (Hq 32, Hkv 8, bf16): 0.965-0.98 ms, 1.12-1.14 PFLOP/s, 0.9 of what a library
+// product of 8192^3 reaches; bounded by power (1.55-1.7 GHz with the matrix units busy 62-64 %
+// of the cycles; the products alone take 0.815 ms).  32 prompts of 16-1024: 126 us, 630 TFLOP/s,
+// a third of it the start and end of each workgroup.
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -250,7 +257,7 @@ __device__ inline uint32_t drop_nonfinite(uint32_t x2) {
 // GROUPS = 2: two waves for 64 rows' even tiles and two for their odd ones, whose states are
 // joined at the end.  A step takes about 0.65 us however little the GPU has to do, so where
 // blocks are few, half the steps on twice the CUs count for more than the second reading of
-// K/V: one prompt of 500 tokens (8 KV heads) 15.2 -> 12.4 us, 4000 (1 KV head) 82 -> 52 us; with
+// K/V: one prompt of 500 tokens (8 KV heads) 15.2 -> 12.7 us, 4000 (1 KV head) 82 -> 52 us; with
 // blocks for every CU it is no faster.
 template <class Elem, int GROUPS>
 __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void prefill_kernel(PrefillArgs a) {

@@ -330,8 +330,9 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
   if (!kv_scales || ((uintptr_t)kv_scales & 7))
     return pkv::fail(PKV_ERR_INVALID_ARGUMENT, "write_kv_fp8_block: kv_scales null or not 8-byte aligned");
   // Few tokens: a window each, so that runs that lie next to one another (a decode step's) are
-  // not written one after another; else windows of about a page, most with one start or two
-  // (a workgroup without one still costs 2 us of a CU's place).
+  // not written one after another; else windows of 16 tokens for pages of up to 16, a start or
+  // two each, and of 32 for larger ones.  Of long prompts in pages of 64 and 128 every second
+  // window and three of four hold no start, and one without still costs 2 us of a CU's place.
   const bool bf16 = dtype == PKV_DTYPE_BF16, shared = page_size > 64;
   const int window = (long)tokens * num_kv_heads <= 4096 ? 1 : page_size > 16 ? 32 : 16;
   const long units = (long)((tokens + window - 1) / window) * num_kv_heads * 2;

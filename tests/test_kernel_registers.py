@@ -45,3 +45,11 @@ def test_two_workgroups_of_fp8_queue_items_per_cu(registers, elem):
             if n.startswith(f"_ZN3pkv13decode_kernelINS_{elem}ELi1ELi3ELi2ELi8E")}
     assert len(ours) == 4, sorted(ours)
     assert max(ours.values()) <= 128, ours
+
+
+@pytest.mark.parametrize("elem", ["4Half", "6BFloat"])
+def test_three_workgroups_of_prompt_attention_per_cu(registers, elem):
+    # prefill_kernel<elem, 1 group of four waves>: a wave of each workgroup on a SIMD
+    ours = {n: r for n, r in registers.items() if n.startswith(f"_ZN12_GLOBAL__N_114prefill_kernelINS_{elem}ELi1E")}
+    assert len(ours) == 1, sorted(ours)
+    assert max(ours.values()) <= 168, ours

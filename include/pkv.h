@@ -421,6 +421,125 @@ int pkv_paged_attention_fp8_block(
 size_t pkv_fp8_block_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads);
 
 /* ---------------------------------------------------------------------------------
+ * A further turn over rows that are cached.  No counterpart in the reference.
+ * ------------------------------------------------------------------------------- */
+
+/* The norm of every head of q [tokens, num_q_heads, 128] and k [tokens, num_kv_heads, 128] and its
+ * rotation by position, in 32 bits, rounded once:
+ *   y = x * (mean(x^2) + eps)^(-1/2) * weight       (weight null: y = x)
+ *   a' = a cos - b sin,  b' = b cos + a sin          for the pairs (a, b) of the first rotary_dim dims
+ * Pairs are dims (i, i + rotary_dim / 2), or with `interleaved` (2 i, 2 i + 1).  Weights are fp32
+ * [128] (*_weight_heads = 1) or one row a head ([heads, 128], *_weight_heads = heads).  cos_sin is
+ * fp32 [max_positions, rotary_dim]: the cosines of the rotary_dim / 2 angles, then their sines.
+ * rotary_dim is a multiple of 16 up to 128, eps (where a weight is given) in [2^-100, 2^100].
+ * positions [tokens] count as clamped to the table.  An output is its own input (same pointer and
+ * stride), or overlaps neither the inputs nor the other output (refused).  The same number of
+ * elements from token to token as for the inputs above, for outputs too. */
+int pkv_norm_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                  const float* q_weight, int32_t q_weight_heads, const float* k_weight,
+                  int32_t k_weight_heads, const float* cos_sin, const int32_t* positions, void* q_out,
+                  int64_t q_out_stride, void* k_out, int64_t k_out_stride, int32_t tokens,
+                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                  int32_t max_positions, int32_t interleaved, float eps, int32_t dtype, void* stream);
+
+/* pkv_norm_rope and pkv_write_kv in one pass: k goes, normed and rotated, and v, as it is, to slot
+ * slot_mapping[t] of the pools (which no other tensor of the call may overlap); slots outside them
+ * are skipped, and a slot may occur only once.  q_out as above. */
+int pkv_norm_rope_write_kv(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                           const void* v, int64_t v_stride, const float* q_weight,
+                           int32_t q_weight_heads, const float* k_weight, int32_t k_weight_heads,
+                           const float* cos_sin, const int32_t* positions, void* q_out,
+                           int64_t q_out_stride, void* k_pages, void* v_pages,
+                           const int32_t* slot_mapping, int32_t tokens, int32_t num_q_heads,
+                           int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                           int32_t max_positions, int32_t interleaved, float eps, int32_t num_pages,
+                           int32_t page_size, int32_t dtype, void* stream);
+
+/* Pages that several rows hold.  page_shares [num_pages] counts the holders of a page beyond the
+ * first: 0 for a page that one row holds and for a free one, so pages that pkv_build_block_tables
+ * hands out need nothing done.  All zero at the start; only these three operators write it.
+ *
+ * Forks: row children[i] of the table becomes a copy of row parents[i], for i < num_forks (at most
+ * 8000).  Of the parent's lens[parent] tokens, full pages are shared (entries copied, page_shares one
+ * more); a part-filled last page is the child's own: taken from the end of the list free_pages[0,
+ * num_free) in the order of i, entered in its table row, and named in copy_src[i], copy_dst[i]
+ * (the parent's page and the child's; -1, -1 where there is none) for pkv_copy_pages, once for every
+ * layer's pools.  num_free_out is num_free less the pages taken; negative when that many were
+ * missing: then nothing else is written but -1 to the copy lists, and the call can be repeated.
+ * Lengths are the caller's: the children's are set by it.  Pairs whose rows are outside the table,
+ * or the same, are skipped; a row must not be a child twice, nor a child and a parent in one call
+ * (unspecified entries and counts, nothing outside the tables).  num_free counts as clamped to [0,
+ * free_capacity], lengths to the table.  num_free_out must not be num_free. */
+int pkv_fork_rows(const int32_t* parents, const int32_t* children, const int32_t* lens,
+                  int32_t* block_table, int32_t* page_shares, const int32_t* free_pages,
+                  const int32_t* num_free, int32_t* num_free_out, int32_t* copy_src, int32_t* copy_dst,
+                  int32_t num_forks, int32_t batch, int32_t max_pages, int32_t num_pages,
+                  int32_t free_capacity, int32_t page_size, void* stream);
+
+/* Rows that end: every page that holds tokens of the rows `rows` [num_rows] (at most 8000) loses one
+ * holder, and pages that had no other go, in ascending order, to free_pages[num_free] and behind;
+ * num_free_out is the new count.  A row listed twice counts once; rows outside the table are
+ * skipped.  Table and lengths stay as they are (the caller sets the rows' lengths to 0).  The list
+ * must have a place for every page (free_capacity >= num_pages).  The workspace, of
+ * pkv_page_workspace_bytes(num_pages), holds nothing between calls; calls that may overlap need one
+ * each, and must not share lists. */
+int pkv_free_rows(const int32_t* rows, const int32_t* lens, const int32_t* block_table,
+                  int32_t* page_shares, int32_t* free_pages, const int32_t* num_free,
+                  int32_t* num_free_out, void* workspace, size_t workspace_size, int32_t num_rows,
+                  int32_t batch, int32_t max_pages, int32_t num_pages, int32_t free_capacity,
+                  int32_t page_size, void* stream);
+
+/* Pages moved to the front of the pool, so that those in use (the ones that free_pages[0, num_free)
+ * does not name; U of them) are 0 ... U - 1 and the rest can be given back.  A page below U stays; the
+ * used page of the highest id goes to the lowest free id, and so on:
+ *   page_map [num_pages]        every used page's new id; -1 for free ones
+ *   block_table_out             the table [batch, max_pages] with its ids mapped (free pages' as -1;
+ *                               entries that are no ids stay); it may be block_table itself
+ *   page_shares_out             the counts at the new ids, 0 behind; not page_shares itself
+ *   free_pages_out              num_pages - 1 down to U, so that the lowest is taken first; it may be
+ *                               free_pages itself (both have free_capacity >= num_pages places)
+ *   num_free_out [1]            num_pages - U; not num_free itself
+ *   copy_src, copy_dst          [num_copies >= num_pages / 2] the moves, for pkv_copy_pages, once for
+ *                               every layer's pools; -1 behind them
+ * The inputs stay as they are but where outputs are said to lie over them.  Workspace as above. */
+int pkv_compact_pages(const int32_t* block_table, const int32_t* page_shares, const int32_t* free_pages,
+                      const int32_t* num_free, int32_t* page_map, int32_t* block_table_out,
+                      int32_t* page_shares_out, int32_t* free_pages_out, int32_t* num_free_out,
+                      int32_t* copy_src, int32_t* copy_dst, void* workspace, size_t workspace_size,
+                      int32_t batch, int32_t max_pages, int32_t num_pages, int32_t free_capacity,
+                      int32_t num_copies, void* stream);
+size_t pkv_page_workspace_bytes(int32_t num_pages);
+
+/* Page copy_dst[i] of the pools [num_pages, num_kv_heads, page_size, 128] (elements of 1 or 2 bytes)
+ * becomes page copy_src[i], and its kv_scales [num_pages, num_kv_heads, 2] too (or null).  Entries
+ * that are not ids of the pool, and copies of a page to itself, are skipped.  No page may be written
+ * twice, nor written and read, in one call. */
+int pkv_copy_pages(const int32_t* copy_src, const int32_t* copy_dst, void* k_pages, void* v_pages,
+                   float* kv_scales, int32_t num_copies, int32_t num_pages, int32_t num_kv_heads,
+                   int32_t page_size, int32_t head_dim, int32_t element_bytes, void* stream);
+
+/* Attention of the newest tokens of every row over its pages, which hold them already (2-byte
+ * pools).  Row b has seq_lens[b] tokens; the n of the call are q's tokens [token_offsets[b],
+ * token_offsets[b + 1]), at positions seq_lens[b] - n ... seq_lens[b] - 1, and each attends to the
+ * row's tokens up to its own: a second turn over a cached prefix, a piece of a prompt, one token,
+ * or none.  A token at a negative position (more new tokens than the row has) sees nothing: 0.
+ * output [tokens, num_q_heads, 128], contiguous; rows outside every sequence are left as they are;
+ * it may be a contiguous q itself, otherwise it must not overlap q (refused), nor the pools.  Any
+ * page_size; G = num_q_heads / num_kv_heads in [1, 32].  Lengths count as clamped to the table, page ids
+ * into the pool, offsets (which must not decrease) to [0, tokens].  Page slots past a row's length are
+ * not read.  An infinity or NaN in K or V reaches the tokens that see its key, and no other.
+ * (tokens * G / 128 + batch) * num_kv_heads must be below 2^24 less the number of the GPU's compute
+ * units times 8.  The workspace is required: pkv_paged_prefill_workspace_bytes on the same device, for
+ * any lengths; it holds nothing between calls, and calls that may overlap need one each. */
+int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                                const int32_t* block_table, const int32_t* seq_lens,
+                                const int32_t* token_offsets, void* output, void* workspace,
+                                size_t workspace_size, int32_t batch, int32_t tokens, int32_t num_q_heads,
+                                int32_t num_kv_heads, int32_t head_dim, int32_t num_pages,
+                                int32_t page_size, int32_t max_pages, int32_t dtype, void* stream);
+size_t pkv_paged_prefill_workspace_bytes(int32_t batch, int32_t tokens, int32_t num_q_heads, int32_t num_kv_heads);
+
+/* ---------------------------------------------------------------------------------
  * Contiguous-layout decode: K and V are [batch, num_kv_heads, context, 128] (every row
  * holds `context` tokens) and q / output are [batch, num_q_heads, 128].
  * ------------------------------------------------------------------------------- */

@@ -1,0 +1,680 @@
+// pkv_chunk.hip — attention of the newest tokens of every row over the row's pages, which hold
+// them already: a second turn over a cached prefix, a piece of a long prompt, guessed tokens that
+// are checked at once, single tokens among them (the reference has one token a row only,
+// cuh:294-459).
+//
+//   o[i] = sum_{j <= p_i, j < L} softmax_j(q[i] k[j] / sqrt(128)) v[j],  p_i = L - n + i
+//
+// for the n newest of a row's L tokens; a token that sees no key gives 0.
+//
+// The products are those of the prompt attention (pkv_prefill.hip): rows of work are the (token,
+// head of the group) pairs of a KV head, S^T = K Q^T and O^T += V^T P^T on 32x32x16 tiles, K/V
+// tiles of 32 keys straight to LDS in a ring of three.  What is new:
+//
+// Pages.  A tile's keys lie in any pages: every lane computes its key's place, a 64-bit address from
+// the page's id in LDS (a window of the row's table, renewed every few hundred keys), and loads 16
+// bytes of it.  Keys past the row's end read its last key again; their weights are 0.
+//
+// Splits.  Rows differ in length by orders of magnitude and a call may have very few rows, so work
+// is cut by keys as well: with W tiles in all blocks of the call (as if every block saw all keys)
+// and P parts wanted, no workgroup takes more than C = max(kMinTiles, W / P) tiles.  All
+// workgroups compute C and their own part from the lengths on the GPU.  The parts of a block
+// leave their sums in the workspace, and a second kernel joins them.
+
+#include <hip/hip_runtime.h>
+#include <float.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "pkv.h"
+#include "pkv_attention_tile.h"
+#include "pkv_device.h"
+
+namespace pkv {
+int fail(int status, const char* fmt, ...);  // pkv_decode.hip: sets pkv_last_error()
+int ok();
+}  // namespace pkv
+
+namespace {
+
+constexpr int kIds = 512;      // page ids in LDS
+constexpr int kMinTiles = 4;
+constexpr int kSmallBatch = 64;  // rows of a table whose plan every wave makes for itself
+constexpr int kStateFloats = kD + 2;  // of one row: its sums, maximum and sum of weights
+
+struct ChunkArgs {
+  const uint8_t* q;  // token t, head h at q + t * q_stride + h * 256 (bytes)
+  const uint8_t* k_pages;  // [num_pages, Hkv, ps, 128]
+  const uint8_t* v_pages;
+  const int32_t* block_table;    // [B, max_pages]
+  const int32_t* seq_lens;       // [B]
+  const int32_t* token_offsets;  // [B + 1]
+  uint8_t* output;               // [T, Hq, 128]
+  int32_t* plan;                 // of more than kSmallBatch rows
+  float* sums;                   // [state rows, Hkv, 128]
+  float* tops;                   // [state rows, Hkv, 2]: maximum, sum of weights
+  long q_stride, page_bytes;
+  int32_t batch, tokens, hq, hkv, group, num_pages, max_pages, page_size, parts;
+  uint32_t page_magic, page_shift;  // key / page_size = mulhi(2 key, magic) >> shift, key < 2^31
+  float inv_group;
+};
+
+// A row of the table: its n tokens of the call from `start` on, the first at position `before`
+// (negative where more tokens are called new than the row has), and the keys that it has.
+struct Seq {
+  int start, n, before, len;
+};
+__device__ inline int offset_of(const ChunkArgs& a, int b) { return min(max(a.token_offsets[b], 0), a.tokens); }
+__device__ inline Seq seq_of(const ChunkArgs& a, int b) {
+  const int start = offset_of(a, b), n = max(offset_of(a, b + 1) - start, 0), total = max(a.seq_lens[b], 0);
+  return {start, n, total - n, min(total, a.max_pages * a.page_size)};
+}
+__device__ inline int tiles_of(int len) { return (int)(((uint32_t)len + kKeys - 1) / kKeys); }
+template <int ROWS>
+__device__ inline int blocks_of(const ChunkArgs& a, int n) { return (int)(((uint32_t)(n * a.group) + ROWS - 1) / ROWS); }
+
+__device__ inline double wave_sum(double x) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  return x;
+}
+// `tiles`: blocks times tiles of all rows, whole and so the same in any order (below 2^53).
+__device__ inline int part_tiles(const ChunkArgs& a, double tiles) {
+  return max(kMinTiles, (int)fmin(ceil(tiles * a.hkv / a.parts), 1e9));
+}
+__device__ inline int parts_of(int tiles, int each) { return max((int)(((uint32_t)tiles + each - 1) / each), 1); }
+
+// What a row adds to the plan's three running sums: units of work (blocks by parts), rows of states
+// in the workspace, and rows to join.
+struct Share {
+  int units, states, joins;
+};
+template <int ROWS>
+__device__ inline Share share_of(const ChunkArgs& a, const Seq& s, int each) {
+  const int parts = parts_of(tiles_of(s.len), each), rows = parts > 1 ? s.n * a.group : 0;
+  return {blocks_of<ROWS>(a, s.n) * parts, rows * parts, rows};
+}
+
+// The plan in memory: C, 0, then for every row of the table, and behind the last, the sums before it.
+__device__ inline int32_t* units_before(const ChunkArgs& a) { return a.plan + 2; }
+__device__ inline int32_t* states_before(const ChunkArgs& a) { return a.plan + 2 + (a.batch + 1); }
+__device__ inline int32_t* joins_before(const ChunkArgs& a) { return a.plan + 2 + 2 * (a.batch + 1); }
+
+constexpr int kPlanThreads = 1024;
+template <int ROWS>
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
+  constexpr int kPlanWaves = kPlanThreads / 64;
+  __shared__ double total[kPlanWaves];
+  __shared__ int sums[3][kPlanWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  double tiles = 0;
+  for (int b = tid; b < a.batch; b += kPlanThreads) {
+    const Seq s = seq_of(a, b);
+    tiles += (double)blocks_of<ROWS>(a, s.n) * tiles_of(s.len);
+  }
+  tiles = wave_sum(tiles);
+  if (lane == 0) total[wave] = tiles;
+  __syncthreads();
+  tiles = 0;
+  for (int w = 0; w < kPlanWaves; ++w) tiles += total[w];
+  const int each = part_tiles(a, tiles);
+  int before[3] = {0, 0, 0};
+  int32_t* const to[3] = {units_before(a), states_before(a), joins_before(a)};
+  for (int base = 0; base <= a.batch; base += kPlanThreads) {
+    const int b = base + tid;
+    Share x{0, 0, 0};
+    if (b < a.batch) x = share_of<ROWS>(a, seq_of(a, b), each);
+    const int mine[3] = {x.units, x.states, x.joins};
+    int sum[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      sum[i] = wave_scan(mine[i]);
+      if (lane == 63) sums[i][wave] = sum[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      int at = before[i] + sum[i] - mine[i];
+      for (int w = 0; w < kPlanWaves; ++w) {
+        if (w < wave) at += sums[i][w];
+        before[i] += sums[i][w];
+      }
+      if (b <= a.batch) to[i][b] = at;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) a.plan[0] = each;
+}
+
+// A unit of work: part `part` of block `block` of a row of the table.  block < 0: none.
+struct Unit {
+  Seq seq;
+  int row, block, part, each, states;
+};
+
+__device__ inline Seq seq_from(const Seq& s, int lane) {
+  return {__builtin_amdgcn_readlane(s.start, lane), __builtin_amdgcn_readlane(s.n, lane),
+          __builtin_amdgcn_readlane(s.before, lane), __builtin_amdgcn_readlane(s.len, lane)};
+}
+
+// Units go through the rows of the table, part by part, a part's last block first: the blocks at
+// work at one time share their keys in L2.
+template <int ROWS>
+__device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
+  Unit u;
+  int unit;
+  if (a.batch <= kSmallBatch) {
+    Seq s{0, 0, 0, 0};
+    if (lane < a.batch) s = seq_of(a, lane);
+    u.each = uniform(part_tiles(a, wave_sum((double)blocks_of<ROWS>(a, s.n) * tiles_of(s.len))));
+    const Share x = share_of<ROWS>(a, s, u.each);
+    const int units = wave_scan(x.units), states = wave_scan(x.states);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(units > slot);
+    u.block = -1;
+    if (!past) return u;
+    u.row = __builtin_ctzll(past);
+    u.seq = seq_from(s, u.row);
+    u.states = __builtin_amdgcn_readlane(states - x.states, u.row);
+    unit = slot - __builtin_amdgcn_readlane(units - x.units, u.row);
+  } else {
+    // The last row whose first unit is at most `slot` (rows without units share the next one's),
+    // found among 64 candidates at a time.
+    const int32_t* const first = units_before(a);
+    u.each = uniform(a.plan[0]);
+    u.block = -1;
+    if (slot >= uniform(first[a.batch])) return u;
+    int b = 0, n = a.batch;
+    while (n > 1) {
+      const int stride = (n + 63) / 64, at = b + lane * stride;
+      const uint64_t fits = __builtin_amdgcn_ballot_w64(lane * stride < n && first[min(at, a.batch)] <= slot);
+      const int found = 63 - __builtin_clzll(fits);  // the first candidate always fits
+      n = min(stride, n - found * stride);
+      b += found * stride;
+    }
+    u.row = uniform(b);
+    u.seq = seq_of(a, u.row);
+    u.states = uniform(states_before(a)[u.row]);
+    unit = slot - uniform(first[u.row]);
+  }
+  const int blocks = blocks_of<ROWS>(a, u.seq.n);
+  u.part = unit / blocks;
+  u.block = blocks - 1 - (unit - u.part * blocks);
+  return u;
+}
+
+// The last key that token i of a row sees; -1: none.
+__device__ inline int last_key(const Seq& s, int i) { return max(min(s.before + i, s.len - 1), -1); }
+
+__device__ inline int page_index(const ChunkArgs& a, int key) {
+  return (int)(__umulhi(2 * (uint32_t)key, a.page_magic) >> a.page_shift);
+}
+
+// 64 x 16 bytes straight to LDS, lane l's to `lds` + 16 l.  In assembly because the compiler lets
+// every LDS read wait for every such load in flight; landed() is the wait.  m0 must be one wait
+// state old.
+__device__ inline void load_to_lds(uint32_t lds, const uint8_t* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(from) : "memory");
+}
+
+// GROUPS = 1: four waves of 32 rows each.  2: two pairs of waves share 64 rows' tiles, the even
+// ones and the odd ones, and join their sums.
+template <class Elem, int GROUPS>
+__global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel(ChunkArgs a) {
+  constexpr int kGroupWaves = kWaves / GROUPS, kRows = kGroupWaves * kWaveRows;
+  constexpr int kGroupBytes = kBuffers * 2 * kTileBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t all_lds[GROUPS * kGroupBytes];
+  __shared__ int ids[kIds];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int group = GROUPS == 1 ? 0 : uniform(tid >> 6) / kGroupWaves, wave = (tid >> 6) - group * kGroupWaves;
+  uint8_t* const lds = all_lds + group * kGroupBytes;  // K and V of the group's tiles
+  const int col = lane & 31, half = lane >> 5;
+  const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
+  const Unit u = unit_of<kRows>(a, uniform((int)(blockIdx.x / (unsigned)a.hkv)), lane);
+  if (u.block < 0) return;
+  const int start = uniform(u.seq.start), n = uniform(u.seq.n), len = uniform(u.seq.len);
+  const Seq seq{start, n, uniform(u.seq.before), len};
+  const int block = uniform(u.block), rows = n * a.group;
+
+  // Row row0 + r of the wave is token tok0 + (rem + r) / G: a quotient of numbers below 64, which
+  // the product with 1 / G in 32 bits gives exactly (it is off by less than 1 / (2 G)).
+  const int row0 = uniform(min(block * kRows + wave * kWaveRows, rows));
+  const int tok0 = row0 / a.group, rem = row0 - tok0 * a.group, live = rows - row0;  // may be 0
+  auto token_of = [&](int r) { return (int)(((float)(rem + r) + 0.5f) * a.inv_group); };
+  const int last_row = max(min(kWaveRows, live) - 1, 0);
+  const int r = min(col, last_row), dt = token_of(r);
+  const int tok = min(tok0 + dt, n - 1);  // a wave past the last row takes the last token's
+  const int see = last_key(seq, tok);
+  const int wave_first = last_key(seq, min(tok0, n - 1));
+  const int wave_last = live > 0 ? last_key(seq, tok0 + uniform(token_of(last_row))) : -1;
+  const int block_tiles = tiles_of(last_key(seq, (min((block + 1) * kRows, rows) - 1) / a.group) + 1);
+  const int part = uniform(u.part), tile0 = part * uniform(u.each);
+  if (part > 0 && tile0 >= block_tiles) return;
+  const int end = min(block_tiles, tile0 + uniform(u.each));
+  const bool whole = block_tiles <= u.each;
+  const int tiles = (end - tile0 - group + GROUPS - 1) / GROUPS;  // the group's: tile0 + GROUPS i + group
+  const int steps = (end - tile0 + GROUPS - 1) / GROUPS;
+
+  // A wave moves rows kMoved wave + 4 i + lane / 16 of a tile, 256 bytes a row.  16-byte chunk p of
+  // row r in LDS is chunk p ^ r of K's row (p ^ 4 r of V's), so that reads of one chunk column
+  // (K) or of 64 bytes of four rows (V) spread over all banks.
+  constexpr int kMoved = kKeys / kGroupWaves;
+  constexpr int kLoads = kMoved / 4;  // per wave and tile of K, and of V
+  const int srow = wave * kMoved + (lane >> 4), chunk = lane & 15;
+  const uint32_t lds0 = (uint32_t)uniform((int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds +
+                                                (uint32_t)(wave * kMoved * kRowBytes)));
+  const uint32_t head = (uint32_t)(kvh * a.page_size) * kRowBytes;
+  const uint32_t kchunk = (chunk ^ (srow & 15)) << 4, vchunk = (chunk ^ ((srow & 3) << 2)) << 4;
+  const int32_t* const table = a.block_table + (long)u.row * a.max_pages;
+  // ids[] holds the pages from `first_id` on, of the tiles before `id_end`.
+  const int window = (int)min((long)(kIds - 1) * a.page_size / kKeys, 1L << 26);
+  int first_id = 0, id_end = 0;
+  auto renew_ids = [&](int tile) __attribute__((always_inline)) {
+    first_id = uniform(page_index(a, tile * kKeys));
+    id_end = tile + window;
+    const int last = page_index(a, len - 1);
+    for (int i = tid; i < kIds && first_id + i <= last; i += kWaves * 64)
+      ids[i] = min(max(table[first_id + i], 0), a.num_pages - 1);
+    __syncthreads();
+  };
+  auto fetch = [&](int i, int buf) __attribute__((always_inline)) {  // the group's i-th tile
+    const uint32_t to = (uint32_t)uniform((int)(lds0 + buf * 2 * kTileBytes));
+    const int key0 = (tile0 + GROUPS * i + group) * kKeys + srow;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int key = min(key0 + 4 * j, len - 1), page = page_index(a, key);
+      const uint64_t at = (uint64_t)(uint32_t)ids[page - first_id] * (uint64_t)a.page_bytes +
+                          (head + (uint32_t)(key - page * a.page_size) * kRowBytes);
+      load_to_lds(to + j * 4 * kRowBytes, a.k_pages + at + (kchunk ^ (j << 6)));
+      load_to_lds(to + kTileBytes + j * 4 * kRowBytes, a.v_pages + at + vchunk);
+    }
+  };
+  auto begin = [&]() __attribute__((always_inline)) {
+    if (steps > 0) renew_ids(tile0);
+    if (tiles > 0) fetch(0, 0);
+    if (tiles > 1) fetch(1, 1);
+  };
+  begin();
+
+  u32x4 q[8];
+  const uint8_t* qp = a.q + (start + (long)tok) * a.q_stride +
+                      (long)(kvh * a.group + rem + r - dt * a.group) * kRowBytes + half * 16;
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) q[kk] = *(const u32x4*)(qp + kk * 32);
+
+  // Reads: lane's K row (key col), chunk 2 kk + half; V rows 4 half + (lane % 16) / 4, four
+  // dims from 32 db + 16 (lane / 16 % 2) + 4 (lane % 4) on.
+  const uint32_t ksrc = col * kRowBytes + ((half ^ (col & 15)) << 4);
+  const int vr = (lane >> 2) & 3;
+  const uint32_t vsrc = (4 * half + vr) * kRowBytes + (vr << 6) + ((lane & 16) << 1) + ((lane & 3) << 3);
+
+  f32x16 o[4];
+  float m, l;
+  bool large = false;  // a row of the wave has a large maximum
+  const uint8_t* kat[8];
+  const uint8_t* vat[4];
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) kat[kk] = lds + (ksrc ^ (kk << 5));
+#pragma unroll
+  for (int db = 0; db < 4; ++db) vat[db] = lds + kTileBytes + (vsrc ^ (db << 6));
+
+  // A masked weight is 0, and 0 times an infinity or NaN in V is NaN.  So where a row comes out
+  // not finite, its workgroup computes once more, `careful`: such values are taken out of the tiles
+  // that a row of it masks in part, those of the steps from `masked` on (the keys read twice past
+  // the end among them), and put back at the end for the rows that see their token.
+  bool careful = false;
+  const int masked = max((last_key(seq, block * kRows / a.group) + 1) / kKeys - tile0, 0) / GROUPS;
+  auto clean = [&](int buf) {
+    u32x4* const v = (u32x4*)(lds + buf * 2 * kTileBytes + kTileBytes) + wave * 64 + lane;
+    for (int i = 0; i < kTileBytes / 16; i += kGroupWaves * 64) {
+      u32x4 x = v[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = drop_nonfinite<Elem>(x[j]);
+      v[i] = x;
+    }
+    __syncthreads();
+  };
+
+  // The group's i-th tile, which lies in buffer `buf`.
+  auto step = [&](int i, int buf) __attribute__((always_inline)) {
+    const int at = buf * 2 * kTileBytes;
+    if (careful && i >= masked) clean(buf);
+    if (GROUPS * (i + 3) > id_end - tile0 && GROUPS * (i + 2) < end - tile0) {
+      __syncthreads();  // the old ids have been read
+      renew_ids(tile0 + GROUPS * (i + 2));
+    }
+    if (i + 2 < tiles) fetch(i + 2, buf >= 1 ? buf - 1 : buf + 2);
+    const int k0 = (tile0 + GROUPS * i + group) * kKeys;
+    if (k0 <= wave_last && (GROUPS == 1 || i < tiles)) {
+      f32x16 s = {};
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) s = Elem::mma(*(const u32x4*)(kat[kk] + at), q[kk], s);
+      auto value = [&](int c, int db) __attribute__((always_inline)) {  // keys 16 c ..., dims 32 db + lane % 32
+        typedef __attribute__((address_space(3))) s16x4* Lds;
+        const uint8_t* v = vat[db] + at + c * 16 * kRowBytes;
+        const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)v));
+        const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v + 8 * kRowBytes)));
+        return u32x4{v0[0], v0[1], v1[0], v1[1]};
+      };
+      u32x4 v0[4];
+#pragma unroll
+      for (int db = 0; db < 4; ++db) v0[db] = value(0, db);
+      if (k0 + kKeys - 1 > wave_first) {
+        const int visible = see - k0 - 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i >> 2) + (i & 3) > visible) s[i] = -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float mn = fmaxf(m, mx);
+        const float c = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2);
+        m = mn;
+        large = __builtin_amdgcn_ballot_w64(fabsf(m) >= kLargeScore) != 0;
+        l *= c;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[db][i] *= c;
+      }
+      float ms = m * kScaleLog2;
+      if (large) {
+        ms = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] -= m;
+      }
+      u32x4 p[2];
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t x = Elem::pack2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kScaleLog2, -ms)),
+                                       __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], kScaleLog2, -ms)));
+        p[i >> 3][(i & 7) >> 1] = x;
+        l = Elem::sum2(x, l);
+      }
+      u32x4 v1[4];
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        v1[db] = value(1, db);
+        o[db] = Elem::mma(v0[db], p[0], o[db]);
+      }
+#pragma unroll
+      for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v1[db], p[1], o[db]);
+    }
+    // The next tile has landed, and behind the barrier this one's place is free.
+    if (i + 2 < tiles) landed<2 * kLoads>();
+    else landed<0>();
+    __syncthreads();
+  };
+  u32x2 out[16];
+  for (;;) {
+    landed<0>();
+    __syncthreads();
+    m = -FLT_MAX, l = 0.f;  // finite where a row sees no key, or none but of score -inf
+    large = true;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) o[db] = f32x16{};
+    for (int i = 0; i < steps; i += kBuffers) {  // LDS places known at compile time
+      step(i, 0);
+      if (i + 1 >= steps) break;
+      step(i + 1, 1);
+      if (i + 2 >= steps) break;
+      step(i + 2, 2);
+    }
+    if constexpr (GROUPS > 1) {  // the second group's sums to the first's waves
+      float* const at = (float*)all_lds + wave * 66 * 64 + lane;
+      if (group == 1) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) at[j * 64] = o[j >> 4][j & 15];
+        at[64 * 64] = m, at[65 * 64] = l;
+      }
+      __syncthreads();
+      if (group == 0) {
+        const float m1 = at[64 * 64], l1 = at[65 * 64], mn = fmaxf(m, m1);
+        const float c0 = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2), c1 = __builtin_amdgcn_exp2f((m1 - mn) * kScaleLog2);
+        m = mn, l = l * c0 + l1 * c1;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) o[j >> 4][j & 15] = o[j >> 4][j & 15] * c0 + at[j * 64] * c1;
+      }
+      __syncthreads();  // the places are free
+    }
+    if (careful) {
+      const int stop = min(see, end * kKeys - 1);
+      for (int key = (tile0 + masked * GROUPS) * kKeys; key <= stop; ++key) {
+        const int page = page_index(a, key), id = min(max(table[page], 0), a.num_pages - 1);
+        const u32x2* const x = (const u32x2*)(a.v_pages + (uint64_t)(uint32_t)id * (uint64_t)a.page_bytes +
+                                              (head + (uint32_t)(key - page * a.page_size) * kRowBytes)) + half;
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float y = Elem::widen(x[2 * c][i >> 1], i & 1);
+            o[c >> 2][4 * (c & 3) + i] += __builtin_isfinite(y) ? 0.f : y;
+          }
+      }
+    }
+    // `zero` turns NaN where a value is not finite.
+    const float sum = l + __shfl_xor(l, 32);
+    float zero = 0.f;
+    if (whole) {  // the rows in the output's type; 0 for a token that sees no key
+      const float inv = see < 0 ? 0.f : 1.0f / sum;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const uint32_t x = Elem::pack2(o[db][i] * inv, o[db][i + 1] * inv);
+          out[4 * db + (i >> 2)][(i >> 1) & 1] = x;
+          zero = Elem::times0(x, zero);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) zero = __builtin_fmaf(o[j >> 4][j & 15], 0.f, zero);
+    }
+    l = sum;
+    if (careful || !__syncthreads_or(group == 0 && live > 0 && zero != 0.f)) break;
+    careful = true;
+    begin();
+  }
+
+  if (group != 0) return;
+  if (!whole) {
+    if (col < live) {
+      const long state = ((long)u.states + (long)part * rows + row0 + col) * a.hkv + kvh;
+      float* const to = a.sums + state * kD + 4 * half;
+      typedef float f32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        *(f32x4*)(to + 8 * c) = f32x4{o[c >> 2][4 * (c & 3)], o[c >> 2][4 * (c & 3) + 1], o[c >> 2][4 * (c & 3) + 2],
+                                      o[c >> 2][4 * (c & 3) + 3]};
+      if (half == 0) *(f32x2*)(a.tops + 2 * state) = f32x2{m, l};
+    }
+    return;
+  }
+  // The wave's 32 rows pass through LDS, so that 16 lanes write one row of 256 bytes; 16-byte
+  // chunks lie under an exclusive or with the row.
+  uint8_t* const mine = lds + wave * kWaveRows * kRowBytes;
+#pragma unroll
+  for (int c = 0; c < 16; ++c) *(u32x2*)(mine + col * kRowBytes + ((c ^ (col & 15)) << 4) + 8 * half) = out[c];
+  // Row R of the (sequence, KV head), a row of its token t, is row R + t (Hq - G) of the output.
+  uint8_t* const to = a.output + ((long)start * a.hq + kvh * a.group + row0 + (long)tok0 * (a.hq - a.group)) * kRowBytes +
+                      (lane & 15) * 16;
+#pragma unroll
+  for (int i = 0; i < kWaveRows / 4; ++i) {
+    const int j = 4 * i + (lane >> 4);
+    if (j < live)
+      *(u32x4*)(to + (long)(j + token_of(j) * (a.hq - a.group)) * kRowBytes) =
+          *(const u32x4*)(mine + j * kRowBytes + (((lane & 15) ^ (j & 15)) << 4));
+  }
+}
+
+// Joins the parts of the rows that were cut: 32 lanes hold a row, four dims each, and kJoin of them
+// take its parts in turn.
+constexpr int kJoin = 8;
+template <class Elem, int ROWS>
+__global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  __shared__ f32x4 part_sums[kJoin][32];
+  __shared__ float part_m[kJoin], part_l[kJoin];
+  __shared__ int small_states[kSmallBatch + 1], small_joins[kSmallBatch + 1];
+  const int tid = threadIdx.x, lane = tid & 63, sub = tid >> 5, quad = tid & 31;
+  int each;
+  if (a.batch <= kSmallBatch) {
+    Seq s{0, 0, 0, 0};
+    if (lane < a.batch) s = seq_of(a, lane);
+    each = part_tiles(a, wave_sum((double)blocks_of<ROWS>(a, s.n) * tiles_of(s.len)));
+    const Share x = share_of<ROWS>(a, s, each);
+    const int states = wave_scan(x.states), joins = wave_scan(x.joins);
+    if (tid < 64) {
+      small_states[lane] = states - x.states, small_joins[lane] = joins - x.joins;
+      if (lane == 63) small_joins[64] = joins;
+    }
+    __syncthreads();
+  } else {
+    each = a.plan[0];
+  }
+  const bool small = a.batch <= kSmallBatch;
+  auto joins_at = [&](int b) { return small ? small_joins[b] : joins_before(a)[b]; };
+  const long total = (long)joins_at(a.batch) * a.hkv;
+  for (long i = blockIdx.x; i < total; i += gridDim.x) {
+    const int join = (int)(i / a.hkv), kvh = (int)(i - (long)join * a.hkv);
+    int b = 0;  // the last row of the table whose first join is at most `join`
+    for (int step = 1 << (31 - __builtin_clz(a.batch)); step; step >>= 1)
+      if (b + step < a.batch && joins_at(b + step) <= join) b += step;
+    const Seq s = seq_of(a, b);
+    const int row = join - joins_at(b), rows = s.n * a.group;
+    const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+    const int last = min((row / ROWS + 1) * ROWS, rows) - 1;
+    const int parts = parts_of(tiles_of(last_key(s, last / a.group) + 1), each);
+    if (parts == 1) continue;  // written by its only part
+    const long states = small ? small_states[b] : states_before(a)[b];
+    float m = -FLT_MAX, l = 0.f;
+    f32x4 o = {};
+    for (int p = sub; p < parts; p += kJoin) {
+      const long state = (states + (long)p * rows + row) * a.hkv + kvh;
+      const f32x2 top = *(const f32x2*)(a.tops + 2 * state);
+      const f32x4 x = *(const f32x4*)(a.sums + state * kD + 4 * quad);
+      const float mn = fmaxf(m, top[0]);
+      const float c0 = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2), c1 = __builtin_amdgcn_exp2f((top[0] - mn) * kScaleLog2);
+      m = mn, l = l * c0 + top[1] * c1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = o[j] * c0 + x[j] * c1;
+    }
+    __syncthreads();  // the row before has been read
+    part_sums[sub][quad] = o;
+    if (quad == 0) part_m[sub] = m, part_l[sub] = l;
+    __syncthreads();
+    if (sub == 0) {
+      for (int p = 1; p < kJoin; ++p) m = fmaxf(m, part_m[p]);
+      l = 0.f, o = f32x4{};
+      for (int p = 0; p < kJoin; ++p) {
+        const float c = __builtin_amdgcn_exp2f((part_m[p] - m) * kScaleLog2);
+        l += part_l[p] * c;
+        const f32x4 x = part_sums[p][quad];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += x[j] * c;
+      }
+      const float inv = last_key(s, tok) < 0 ? 0.f : 1.0f / l;
+      *(u32x2*)(a.output + (((long)s.start + tok) * a.hq + head) * kRowBytes + 8 * quad) =
+          u32x2{Elem::pack2(o[0] * inv, o[1] * inv), Elem::pack2(o[2] * inv, o[3] * inv)};
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// Host.
+// ---------------------------------------------------------------------------------
+int parts_wanted() { return 2 * pkv::compute_units(); }
+
+// The blocks of `rows` rows that a call can have, over all KV heads.
+int64_t blocks_at_most(int64_t batch, int64_t tokens, int64_t group, int64_t hkv, int rows) {
+  return (tokens * group / rows + batch) * hkv;
+}
+bool shares_keys(int64_t batch, int64_t tokens, int64_t group, int64_t hkv) {
+  return blocks_at_most(batch, tokens, group, hkv, kWaves * kWaveRows) <= pkv::compute_units() / 2;
+}
+size_t plan_bytes(int64_t batch) { return batch > kSmallBatch ? (size_t)((2 + 3 * (batch + 1)) * 4 + 15) / 16 * 16 : 0; }
+
+// Rows of states, over all KV heads: a row of the table is cut only where its tiles pass C >= W / P,
+// so that its parts are at most 2 tiles / C, and all rows' at most 2 P blocks' or calls' rows.
+int64_t states_at_most(int64_t tokens, int64_t group, int rows) {
+  const int64_t all = tokens * group;
+  return 2 * (int64_t)parts_wanted() * (all < rows ? all : rows);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pkv_paged_prefill_workspace_bytes(int32_t batch, int32_t tokens, int32_t num_q_heads, int32_t num_kv_heads) {
+  if (batch <= 0 || tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return 0;
+  const int64_t group = num_q_heads / num_kv_heads;
+  const int rows = kWaves * kWaveRows / (shares_keys(batch, tokens, group, num_kv_heads) ? 2 : 1);
+  return plan_bytes(batch) + (size_t)states_at_most(tokens, group, rows) * kStateFloats * sizeof(float);
+}
+
+int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                                const int32_t* block_table, const int32_t* seq_lens,
+                                const int32_t* token_offsets, void* output, void* workspace,
+                                size_t workspace_size, int32_t batch, int32_t tokens, int32_t num_q_heads,
+                                int32_t num_kv_heads, int32_t head_dim, int32_t num_pages,
+                                int32_t page_size, int32_t max_pages, int32_t dtype, void* stream) {
+  using pkv::fail;
+  const char* const op = "paged_prefill_attention";
+  if (batch < 0 || tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_pages <= 0 || page_size <= 0 || max_pages <= 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT,
+                "%s: batch %d, tokens %d, num_q_heads %d, num_kv_heads %d, num_pages %d, page_size %d, max_pages %d", op,
+                batch, tokens, num_q_heads, num_kv_heads, num_pages, page_size, max_pages);
+  if (head_dim != kD) return fail(PKV_ERR_UNSUPPORTED, "%s: head_dim %d (only 128)", op, head_dim);
+  if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16) return fail(PKV_ERR_UNSUPPORTED, "%s: unknown dtype %d", op, dtype);
+  if (num_q_heads % num_kv_heads) return fail(PKV_ERR_INVALID_ARGUMENT, "%s: Hq must be divisible by Hkv", op);
+  const int32_t group = num_q_heads / num_kv_heads;
+  if (group > PKV_MAX_GROUP) return fail(PKV_ERR_UNSUPPORTED, "%s: G=Hq/Hkv %d (at most %d)", op, group, PKV_MAX_GROUP);
+  if (q_stride < (int64_t)num_q_heads * kD || q_stride % 8)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "%s: the token stride must hold q's heads and be a multiple of 8 elements", op);
+  const int64_t page_bytes = (int64_t)num_kv_heads * page_size * kRowBytes;
+  if ((int64_t)max_pages * page_size > INT32_MAX - kKeys || page_bytes > INT32_MAX)
+    return fail(PKV_ERR_UNSUPPORTED, "%s: max_pages * page_size must be below 2^31 - 32, and a page below 2 GiB", op);
+  const bool split = shares_keys(batch, tokens, group, num_kv_heads);
+  const int rows = kWaves * kWaveRows / (split ? 2 : 1), parts = parts_wanted();
+  const int64_t groups = blocks_at_most(batch, tokens, group, num_kv_heads, rows) +
+                         (int64_t)((parts + num_kv_heads - 1) / num_kv_heads) * num_kv_heads;
+  if ((int64_t)tokens * group > INT32_MAX || !pkv::fits_grid(groups, kWaves * 64))
+    return fail(PKV_ERR_UNSUPPORTED, "%s: too many tokens or sequences", op);
+  if (batch == 0 || tokens == 0) return pkv::ok();
+  if (!q || !k_pages || !v_pages || !block_table || !seq_lens || !token_offsets || !output)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "%s: null pointer", op);
+  if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)output) & 15)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "%s: tensors must be 16-byte aligned", op);
+  const size_t need = pkv_paged_prefill_workspace_bytes(batch, tokens, num_q_heads, num_kv_heads);
+  if (!workspace || workspace_size < need || ((uintptr_t)workspace & 15))
+    return fail(PKV_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes is smaller than %zu, or misaligned", op,
+                workspace_size, need);
+  // Rows of q are read until the last part of their block ends, behind which the output of another
+  // may have been written: only a q whose rows are the output's own may be written over.
+  const int64_t row = (int64_t)num_q_heads * kRowBytes;
+  if (!(output == q && (tokens == 1 || 2 * q_stride == row)) &&
+      pkv::meets_rows(output, tokens * row, q, tokens, 2 * q_stride, row))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "%s: output must be a contiguous q itself, or not overlap q", op);
+  uint32_t log2 = 0;  // ceil(log2(page_size)); magic = ceil(2^(31 + log2) / page_size) is at most 2^32 - 1 but for powers of two
+  while ((1u << log2) < (uint32_t)page_size) ++log2;
+  const uint64_t magic = ((1ull << (31 + log2)) + page_size - 1) / page_size;
+  float* const states = (float*)((uint8_t*)workspace + plan_bytes(batch));
+  const ChunkArgs a{(const uint8_t*)q, (const uint8_t*)k_pages, (const uint8_t*)v_pages, block_table, seq_lens, token_offsets,
+                    (uint8_t*)output, (int32_t*)workspace, states, states + states_at_most(tokens, group, rows) * kD,
+                    2 * q_stride, page_bytes, batch, tokens, num_q_heads, num_kv_heads, group, num_pages, max_pages,
+                    page_size, parts, (uint32_t)magic, log2, 1.0f / (float)group};
+  const hipStream_t st = (hipStream_t)stream;
+  const bool bf16 = dtype == PKV_DTYPE_BF16;
+  if (batch > kSmallBatch) (split ? plan_kernel<64> : plan_kernel<128>)<<<1, kPlanThreads, 0, st>>>(a);
+  auto* const kernel = split ? (bf16 ? chunk_kernel<BFloat, 2> : chunk_kernel<Half, 2>)
+                             : (bf16 ? chunk_kernel<BFloat, 1> : chunk_kernel<Half, 1>);
+  kernel<<<dim3((unsigned)groups), dim3(kWaves * 64), 0, st>>>(a);
+  auto* const join = split ? (bf16 ? join_kernel<BFloat, 64> : join_kernel<Half, 64>)
+                           : (bf16 ? join_kernel<BFloat, 128> : join_kernel<Half, 128>);
+  join<<<dim3((unsigned)(4 * pkv::compute_units())), dim3(32 * kJoin), 0, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? pkv::ok() : fail(PKV_ERR_LAUNCH, "%s launch: %s", op, hipGetErrorString(e));
+}
+
+}  // extern "C"

@@ -12,7 +12,9 @@
 // (fp16 / bf16 / fp8 pools) that a serving loop runs before each decode step, alone or
 // fused into the indexed and work-queue ops (*_append); and the way from a prompt to the
 // cache: block tables and slots from lengths on the GPU, causal attention over packed
-// prompts, packed K/V writes, and decode over fp8 pools with a scale per (page, head).
+// prompts, packed K/V writes, and decode over fp8 pools with a scale per (page, head); and a
+// further turn over cached rows: norms and rotation of q and k, pages shared, freed, moved and
+// copied, and attention of several new tokens a row over its pages.
 // Work is enqueued on the current HIP stream of the tensors' device without a host sync,
 // so the ops can be captured in HIP graphs.
 
@@ -909,6 +911,259 @@ int64_t persistentkv_fp8_block_workspace_floats(int64_t batch, int64_t num_q_hea
                    sizeof(float));
 }
 
+namespace {
+
+// An fp32 norm weight, [128] or [heads, 128]; of no elements: no norm.
+struct Weight {
+  const float* data = nullptr;
+  int32_t heads = 1;
+};
+Weight weight_of(const torch::Tensor& t, const char* name, int64_t heads, const torch::Tensor& first) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  check_device(t, name, first);
+  TORCH_CHECK(t.scalar_type() == at::kFloat, name, " has wrong dtype");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  if (t.numel() == 0) return {};
+  const bool each = t.dim() == 2;
+  TORCH_CHECK((t.dim() == 1 || each) && t.size(-1) == PKV_HEAD_DIM && (!each || t.size(0) == 1 || t.size(0) == heads),
+              name, " must have shape [128] or [heads, 128]");
+  return {t.data_ptr<float>(), each ? (int32_t)t.size(0) : 1};
+}
+
+// norm_rope (k_out) and norm_rope_write_kv (v, pools and slots).
+void rope_op(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor* v, const torch::Tensor& q_weight,
+             const torch::Tensor& k_weight, const torch::Tensor& cos_sin, const torch::Tensor& positions,
+             torch::Tensor& q_out, torch::Tensor* k_out, torch::Tensor* k_pages, torch::Tensor* v_pages,
+             const torch::Tensor* slot_mapping, double eps, bool interleaved) {
+  const auto dt = activation_dtype(q, "q");
+  check_packed(q, "q", dt);
+  check_packed(k, "k", dt);
+  check_packed(q_out, "q_out", dt);
+  check_device(k, "k", q);
+  check_device(q_out, "q_out", q);
+  check_tensor(cos_sin, "cos_sin", at::kFloat, 2);
+  check_tensor(positions, "positions", at::kInt, 1);
+  check_device(cos_sin, "cos_sin", q);
+  check_device(positions, "positions", q);
+  const int64_t T = q.size(0);
+  TORCH_CHECK(k.size(0) == T, "k tokens mismatch");
+  TORCH_CHECK(q_out.sizes() == q.sizes(), "q_out shape must match q");
+  TORCH_CHECK(positions.size(0) == T, "positions must have one position a token");
+  const Weight qw = weight_of(q_weight, "q_weight", q.size(1), q), kw = weight_of(k_weight, "k_weight", k.size(1), q);
+  const int32_t tokens = i32(T, "q.size(0)"), Hq = i32(q.size(1), "q.size(1)"), Hkv = i32(k.size(1), "k.size(1)");
+  const int32_t rot = i32(cos_sin.size(1), "cos_sin.size(1)"), most = i32(cos_sin.size(0), "cos_sin.size(0)");
+  const c10::DeviceGuard guard(q.device());
+  if (!v) {
+    check_packed(*k_out, "k_out", dt);
+    check_device(*k_out, "k_out", q);
+    TORCH_CHECK(k_out->sizes() == k.sizes(), "k_out shape must match k");
+    raise_on(pkv_norm_rope(q.data_ptr(), token_stride(q), k.data_ptr(), token_stride(k), qw.data, qw.heads, kw.data,
+                           kw.heads, cos_sin.data_ptr<float>(), positions.data_ptr<int>(), q_out.data_ptr(),
+                           token_stride(q_out), k_out->data_ptr(), token_stride(*k_out), tokens, Hq, Hkv,
+                           PKV_HEAD_DIM, rot, most, interleaved ? 1 : 0, (float)eps, pkv_dtype_of(dt), stream_of(q)));
+    return;
+  }
+  check_packed(*v, "v", dt);
+  check_tensor(*k_pages, "k_pages", dt, 4);
+  check_tensor(*v_pages, "v_pages", dt, 4);
+  check_tensor(*slot_mapping, "slot_mapping", at::kInt, 1);
+  check_device(*v, "v", q);
+  check_device(*k_pages, "k_pages", q);
+  check_device(*v_pages, "v_pages", q);
+  check_device(*slot_mapping, "slot_mapping", q);
+  TORCH_CHECK(v->sizes() == k.sizes(), "v shape mismatch");
+  TORCH_CHECK(k_pages->size(1) == Hkv, "k_pages Hkv mismatch");
+  check_pages(*k_pages, *v_pages, k_pages->size(2), PKV_HEAD_DIM);
+  TORCH_CHECK(slot_mapping->size(0) == T, "slot_mapping must have one slot a token");
+  raise_on(pkv_norm_rope_write_kv(
+      q.data_ptr(), token_stride(q), k.data_ptr(), token_stride(k), v->data_ptr(), token_stride(*v), qw.data, qw.heads,
+      kw.data, kw.heads, cos_sin.data_ptr<float>(), positions.data_ptr<int>(), q_out.data_ptr(), token_stride(q_out),
+      k_pages->data_ptr(), v_pages->data_ptr(), slot_mapping->data_ptr<int>(), tokens, Hq, Hkv, PKV_HEAD_DIM, rot, most,
+      interleaved ? 1 : 0, (float)eps, i32(k_pages->size(0), "k_pages.size(0)"), i32(k_pages->size(2), "page_size"),
+      pkv_dtype_of(dt), stream_of(q)));
+}
+
+// An int32 tensor on the first one's device.
+void check_ints(const torch::Tensor& t, const char* name, int64_t dims, const torch::Tensor& first) {
+  check_tensor(t, name, at::kInt, dims);
+  check_device(t, name, first);
+}
+void check_counts(const torch::Tensor& num_free, const torch::Tensor& num_free_out) {
+  TORCH_CHECK(num_free.size(0) == 1 && num_free_out.size(0) == 1, "num_free must have one element");
+  TORCH_CHECK(num_free.data_ptr() != num_free_out.data_ptr(), "num_free_out must not be num_free");
+}
+
+}  // namespace
+
+void persistentkv_norm_rope(torch::Tensor q, torch::Tensor k, torch::Tensor q_weight, torch::Tensor k_weight,
+                            torch::Tensor cos_sin, torch::Tensor positions, torch::Tensor q_out,
+                            torch::Tensor k_out, double eps, bool interleaved) {
+  rope_op(q, k, nullptr, q_weight, k_weight, cos_sin, positions, q_out, &k_out, nullptr, nullptr, nullptr, eps, interleaved);
+}
+
+void persistentkv_norm_rope_write_kv(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor q_weight,
+                                     torch::Tensor k_weight, torch::Tensor cos_sin, torch::Tensor positions,
+                                     torch::Tensor q_out, torch::Tensor k_pages, torch::Tensor v_pages,
+                                     torch::Tensor slot_mapping, double eps, bool interleaved) {
+  rope_op(q, k, &v, q_weight, k_weight, cos_sin, positions, q_out, nullptr, &k_pages, &v_pages, &slot_mapping, eps, interleaved);
+}
+
+void persistentkv_fork_rows(torch::Tensor parents, torch::Tensor children, torch::Tensor lens,
+                            torch::Tensor block_table, torch::Tensor page_shares, torch::Tensor free_pages,
+                            torch::Tensor num_free, torch::Tensor num_free_out, torch::Tensor copy_src,
+                            torch::Tensor copy_dst, int64_t page_size) {
+  check_ints(parents, "parents", 1, parents);
+  check_ints(children, "children", 1, parents);
+  check_ints(lens, "lens", 1, parents);
+  check_ints(block_table, "block_table", 2, parents);
+  check_ints(page_shares, "page_shares", 1, parents);
+  check_ints(free_pages, "free_pages", 1, parents);
+  check_ints(num_free, "num_free", 1, parents);
+  check_ints(num_free_out, "num_free_out", 1, parents);
+  check_ints(copy_src, "copy_src", 1, parents);
+  check_ints(copy_dst, "copy_dst", 1, parents);
+  const int64_t n = parents.size(0);
+  TORCH_CHECK(children.size(0) == n, "children must have one row a parent");
+  TORCH_CHECK(copy_src.size(0) == n && copy_dst.size(0) == n, "copy_src and copy_dst must have one entry a parent");
+  TORCH_CHECK(block_table.size(0) == lens.size(0), "block_table batch mismatch");
+  check_counts(num_free, num_free_out);
+  TORCH_CHECK(page_size > 0, "page_size must be positive");
+  const c10::DeviceGuard guard(parents.device());
+  raise_on(pkv_fork_rows(parents.data_ptr<int>(), children.data_ptr<int>(), lens.data_ptr<int>(),
+                         block_table.data_ptr<int>(), page_shares.data_ptr<int>(), free_pages.data_ptr<int>(),
+                         num_free.data_ptr<int>(), num_free_out.data_ptr<int>(), copy_src.data_ptr<int>(),
+                         copy_dst.data_ptr<int>(), i32(n, "parents.size(0)"), i32(lens.size(0), "batch"),
+                         i32(block_table.size(1), "block_table.size(1)"), i32(page_shares.size(0), "page_shares.size(0)"),
+                         i32(free_pages.size(0), "free_pages.size(0)"), i32(page_size, "page_size"), stream_of(parents)));
+}
+
+void persistentkv_free_rows(torch::Tensor rows, torch::Tensor lens, torch::Tensor block_table,
+                            torch::Tensor page_shares, torch::Tensor free_pages, torch::Tensor num_free,
+                            torch::Tensor num_free_out, torch::Tensor workspace, int64_t page_size) {
+  check_ints(rows, "rows", 1, rows);
+  check_ints(lens, "lens", 1, rows);
+  check_ints(block_table, "block_table", 2, rows);
+  check_ints(page_shares, "page_shares", 1, rows);
+  check_ints(free_pages, "free_pages", 1, rows);
+  check_ints(num_free, "num_free", 1, rows);
+  check_ints(num_free_out, "num_free_out", 1, rows);
+  check_workspace(workspace);
+  check_device(workspace, "workspace", rows);
+  TORCH_CHECK(block_table.size(0) == lens.size(0), "block_table batch mismatch");
+  check_counts(num_free, num_free_out);
+  TORCH_CHECK(page_size > 0, "page_size must be positive");
+  const c10::DeviceGuard guard(rows.device());
+  raise_on(pkv_free_rows(rows.data_ptr<int>(), lens.data_ptr<int>(), block_table.data_ptr<int>(),
+                         page_shares.data_ptr<int>(), free_pages.data_ptr<int>(), num_free.data_ptr<int>(),
+                         num_free_out.data_ptr<int>(), ws_ptr(workspace), ws_bytes(workspace),
+                         i32(rows.size(0), "rows.size(0)"), i32(lens.size(0), "batch"),
+                         i32(block_table.size(1), "block_table.size(1)"), i32(page_shares.size(0), "page_shares.size(0)"),
+                         i32(free_pages.size(0), "free_pages.size(0)"), i32(page_size, "page_size"), stream_of(rows)));
+}
+
+void persistentkv_compact_pages(torch::Tensor block_table, torch::Tensor page_shares, torch::Tensor free_pages,
+                                torch::Tensor num_free, torch::Tensor page_map, torch::Tensor block_table_out,
+                                torch::Tensor page_shares_out, torch::Tensor free_pages_out,
+                                torch::Tensor num_free_out, torch::Tensor copy_src, torch::Tensor copy_dst,
+                                torch::Tensor workspace) {
+  check_ints(block_table, "block_table", 2, block_table);
+  check_ints(page_shares, "page_shares", 1, block_table);
+  check_ints(free_pages, "free_pages", 1, block_table);
+  check_ints(num_free, "num_free", 1, block_table);
+  check_ints(page_map, "page_map", 1, block_table);
+  check_ints(block_table_out, "block_table_out", 2, block_table);
+  check_ints(page_shares_out, "page_shares_out", 1, block_table);
+  check_ints(free_pages_out, "free_pages_out", 1, block_table);
+  check_ints(num_free_out, "num_free_out", 1, block_table);
+  check_ints(copy_src, "copy_src", 1, block_table);
+  check_ints(copy_dst, "copy_dst", 1, block_table);
+  check_workspace(workspace);
+  check_device(workspace, "workspace", block_table);
+  const int64_t pages = page_shares.size(0);
+  TORCH_CHECK(page_map.size(0) == pages, "page_map must have one entry a page");
+  TORCH_CHECK(page_shares_out.size(0) == pages, "page_shares_out shape must match page_shares");
+  TORCH_CHECK(block_table_out.sizes() == block_table.sizes(), "block_table_out shape must match block_table");
+  TORCH_CHECK(free_pages_out.sizes() == free_pages.sizes(), "free_pages_out shape must match free_pages");
+  TORCH_CHECK(copy_dst.sizes() == copy_src.sizes(), "copy_dst shape must match copy_src");
+  check_counts(num_free, num_free_out);
+  const c10::DeviceGuard guard(block_table.device());
+  raise_on(pkv_compact_pages(
+      block_table.data_ptr<int>(), page_shares.data_ptr<int>(), free_pages.data_ptr<int>(), num_free.data_ptr<int>(),
+      page_map.data_ptr<int>(), block_table_out.data_ptr<int>(), page_shares_out.data_ptr<int>(),
+      free_pages_out.data_ptr<int>(), num_free_out.data_ptr<int>(), copy_src.data_ptr<int>(), copy_dst.data_ptr<int>(),
+      ws_ptr(workspace), ws_bytes(workspace), i32(block_table.size(0), "batch"),
+      i32(block_table.size(1), "block_table.size(1)"), i32(pages, "page_shares.size(0)"),
+      i32(free_pages.size(0), "free_pages.size(0)"), i32(copy_src.size(0), "copy_src.size(0)"), stream_of(block_table)));
+}
+
+int64_t persistentkv_page_workspace_ints(int64_t num_pages) {
+  return (int64_t)(pkv_page_workspace_bytes(i32(num_pages, "num_pages")) / sizeof(int32_t));
+}
+
+void persistentkv_copy_pages(torch::Tensor copy_src, torch::Tensor copy_dst, torch::Tensor k_pages,
+                             torch::Tensor v_pages, c10::optional<torch::Tensor> kv_scales) {
+  const auto dt = k_pages.scalar_type();
+  TORCH_CHECK(dt == at::kHalf || dt == at::kBFloat16 || dt == at::kFloat8_e4m3fn, "k_pages has wrong dtype");
+  check_tensor(k_pages, "k_pages", dt, 4);
+  check_tensor(v_pages, "v_pages", dt, 4);
+  check_ints(copy_src, "copy_src", 1, k_pages);
+  check_ints(copy_dst, "copy_dst", 1, k_pages);
+  check_device(v_pages, "v_pages", k_pages);
+  TORCH_CHECK(copy_dst.sizes() == copy_src.sizes(), "copy_dst shape must match copy_src");
+  check_pages(k_pages, v_pages, k_pages.size(2), PKV_HEAD_DIM);
+  const int32_t pages = i32(k_pages.size(0), "k_pages.size(0)"), hkv = i32(k_pages.size(1), "Hkv");
+  if (kv_scales) {
+    check_tensor(*kv_scales, "kv_scales", at::kFloat, 3);
+    check_device(*kv_scales, "kv_scales", k_pages);
+    TORCH_CHECK(kv_scales->size(0) == pages && kv_scales->size(1) == hkv && kv_scales->size(2) == 2,
+                "kv_scales must have shape [num_pages, Hkv, 2]");
+  }
+  const c10::DeviceGuard guard(k_pages.device());
+  raise_on(pkv_copy_pages(copy_src.data_ptr<int>(), copy_dst.data_ptr<int>(), k_pages.data_ptr(), v_pages.data_ptr(),
+                          kv_scales ? kv_scales->data_ptr<float>() : nullptr, i32(copy_src.size(0), "copy_src.size(0)"),
+                          pages, hkv, i32(k_pages.size(2), "page_size"), PKV_HEAD_DIM,
+                          (int32_t)k_pages.element_size(), stream_of(k_pages)));
+}
+
+void persistentkv_paged_prefill_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages,
+                                          torch::Tensor block_table, torch::Tensor seq_lens,
+                                          torch::Tensor token_offsets, torch::Tensor output,
+                                          torch::Tensor workspace, int64_t page_size) {
+  const auto dt = activation_dtype(q, "q");
+  check_packed(q, "q", dt);
+  check_tensor(k_pages, "k_pages", dt, 4);
+  check_tensor(v_pages, "v_pages", dt, 4);
+  check_ints(block_table, "block_table", 2, q);
+  check_ints(seq_lens, "seq_lens", 1, q);
+  check_ints(token_offsets, "token_offsets", 1, q);
+  check_tensor(output, "output", dt, 3);
+  check_workspace(workspace);
+  check_device(k_pages, "k_pages", q);
+  check_device(v_pages, "v_pages", q);
+  check_device(output, "output", q);
+  check_device(workspace, "workspace", q);
+  const int64_t B = seq_lens.size(0);
+  TORCH_CHECK(output.sizes() == q.sizes(), "output shape must match q");
+  TORCH_CHECK(block_table.size(0) == B, "block_table batch mismatch");
+  TORCH_CHECK(token_offsets.size(0) == B + 1, "token_offsets must have batch + 1 elements");
+  TORCH_CHECK(page_size > 0, "page_size must be positive");
+  check_pages(k_pages, v_pages, page_size, PKV_HEAD_DIM);
+  const int32_t Hq = i32(q.size(1), "q.size(1)"), Hkv = i32(k_pages.size(1), "k_pages.size(1)");
+  check_supported_gqa(Hq, Hkv);
+  const c10::DeviceGuard guard(q.device());
+  raise_on(pkv_paged_prefill_attention(
+      q.data_ptr(), token_stride(q), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr<int>(),
+      seq_lens.data_ptr<int>(), token_offsets.data_ptr<int>(), output.data_ptr(), ws_ptr(workspace), ws_bytes(workspace),
+      i32(B, "batch"), i32(q.size(0), "q.size(0)"), Hq, Hkv, PKV_HEAD_DIM, i32(k_pages.size(0), "k_pages.size(0)"),
+      i32(page_size, "page_size"), i32(block_table.size(1), "block_table.size(1)"), pkv_dtype_of(dt), stream_of(q)));
+}
+
+int64_t persistentkv_paged_prefill_workspace_floats(int64_t batch, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads) {
+  return (int64_t)(pkv_paged_prefill_workspace_bytes(i32(batch, "batch"), i32(tokens, "tokens"), i32(num_q_heads, "Hq"),
+                                                     i32(num_kv_heads, "Hkv")) /
+                   sizeof(float));
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention_workqueue_stage", &persistentkv_paged_attention_workqueue_stage,
         "one stage (1 decode, 2 merge) of paged_attention_workqueue in the schedule it takes");
@@ -968,6 +1223,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "paged decode attention over float8_e4m3fn pools with one scale per (page, KV head)");
   m.def("fp8_block_workspace_floats", &persistentkv_fp8_block_workspace_floats,
         "fp32 workspace elements of paged_attention_fp8_block on the current device");
+  m.def("norm_rope", &persistentkv_norm_rope,
+        "norm of every head of q and k and its rotation by position, in one pass");
+  m.def("norm_rope_write_kv", &persistentkv_norm_rope_write_kv,
+        "norm_rope with K and V written into the page pools by slot");
+  m.def("fork_rows", &persistentkv_fork_rows,
+        "table rows that continue other rows' tokens: full pages shared, a page of their own for the last");
+  m.def("free_rows", &persistentkv_free_rows, "pages of ended rows back to the list, unless other rows hold them");
+  m.def("compact_pages", &persistentkv_compact_pages, "new ids that move the used pages to the front of the pool");
+  m.def("page_workspace_ints", &persistentkv_page_workspace_ints,
+        "int32 workspace elements of free_rows and compact_pages");
+  m.def("copy_pages", &persistentkv_copy_pages, "copy pages (and their scales) within one layer's pools",
+        py::arg("copy_src"), py::arg("copy_dst"), py::arg("k_pages"), py::arg("v_pages"), py::arg("kv_scales") = py::none());
+  m.def("paged_prefill_attention", &persistentkv_paged_prefill_attention,
+        "causal attention of each row's newest tokens over its pages");
+  m.def("paged_prefill_workspace_floats", &persistentkv_paged_prefill_workspace_floats,
+        "fp32 workspace elements of paged_prefill_attention on the current device");
   m.def("attention_query_head_baseline", &persistentkv_attention_query_head_baseline,
         "Query-head baseline over contiguous K/V (each query head streams its KV head)");
 }

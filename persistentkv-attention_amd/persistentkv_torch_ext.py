@@ -87,6 +87,29 @@ write_kv_fp8_block = _ext.write_kv_fp8_block
 paged_attention_fp8_block = _ext.paged_attention_fp8_block
 fp8_block_workspace_floats = _ext.fp8_block_workspace_floats
 
+# A further turn over cached rows.  norm_rope(q, k, q_weight, k_weight, cos_sin, positions, q_out,
+# k_out, eps, interleaved) and norm_rope_write_kv(q, k, v, q_weight, k_weight, cos_sin, positions,
+# q_out, k_pages, v_pages, slot_mapping, eps, interleaved) norm and rotate every head (weights of no
+# elements: no norm); paged_prefill_attention(q, k_pages, v_pages, block_table, seq_lens,
+# token_offsets, output, workspace, page_size) attends from each row's newest tokens to its pages,
+# with a workspace of paged_prefill_workspace_floats(batch, tokens, Hq, Hkv) fp32 elements.
+norm_rope = _ext.norm_rope
+norm_rope_write_kv = _ext.norm_rope_write_kv
+paged_prefill_attention = _ext.paged_prefill_attention
+paged_prefill_workspace_floats = _ext.paged_prefill_workspace_floats
+# Pages that rows share (page_shares [num_pages]: holders beyond the first).  fork_rows(parents,
+# children, lens, block_table, page_shares, free_pages, num_free, num_free_out, copy_src, copy_dst,
+# page_size); free_rows(rows, lens, block_table, page_shares, free_pages, num_free, num_free_out,
+# workspace, page_size); compact_pages(block_table, page_shares, free_pages, num_free, page_map,
+# block_table_out, page_shares_out, free_pages_out, num_free_out, copy_src, copy_dst, workspace); and
+# for every layer copy_pages(copy_src, copy_dst, k_pages, v_pages, kv_scales=None).  Workspaces are of
+# page_workspace_ints(num_pages) int32 elements.
+fork_rows = _ext.fork_rows
+free_rows = _ext.free_rows
+compact_pages = _ext.compact_pages
+copy_pages = _ext.copy_pages
+page_workspace_ints = _ext.page_workspace_ints
+
 # fp32 workspace elements with which a direct (num_splits == 1) launch of paged_attention,
 # paged_attention_masked / _indexed or attention_contiguous runs its full internal split
 # (0 when it is not split; a smaller workspace gives a smaller split, an empty one none).
@@ -118,6 +141,8 @@ __all__ = [
     "paged_attention_workqueue_append",
     "paged_attention_indexed_fp8_append", "paged_attention_workqueue_fp8_append",
     "build_block_tables", "prefill_attention", "write_kv", "write_kv_fp8_block",
-    "paged_attention_fp8_block", "fp8_block_workspace_floats", "workspace_floats",
+    "paged_attention_fp8_block", "fp8_block_workspace_floats",
+    "norm_rope", "norm_rope_write_kv", "paged_prefill_attention", "paged_prefill_workspace_floats",
+    "fork_rows", "free_rows", "compact_pages", "copy_pages", "page_workspace_ints", "workspace_floats",
     "workqueue_workspace_floats", "direct_workspace_floats", "split_workspace_floats", "EXTENSION_PATH", "LIBRARY_PATH",
 ]

@@ -120,6 +120,23 @@ def lib():
         f.restype = ctypes.c_int
     so.pkv_fp8_block_workspace_bytes.argtypes = [_I32] * 3
     so.pkv_fp8_block_workspace_bytes.restype = size
+    # A further turn over cached rows.
+    f32 = ctypes.c_float
+    weights = [ptr, _I32, ptr, _I32]  # q's and k's, each with its number of heads
+    so.pkv_norm_rope.argtypes = token_major + weights + [ptr, ptr] + token_major + [_I32] * 7 + [f32, _I32, ptr]
+    so.pkv_norm_rope_write_kv.argtypes = (
+        token_major + [ptr, i64] + weights + [ptr, ptr] + [ptr, i64] + [ptr] * 3 + [_I32] * 7 + [f32] + [_I32] * 3 + [ptr])
+    so.pkv_fork_rows.argtypes = [ptr] * 10 + [_I32] * 6 + [ptr]
+    so.pkv_free_rows.argtypes = [ptr] * 8 + [size] + [_I32] * 6 + [ptr]
+    so.pkv_compact_pages.argtypes = [ptr] * 12 + [size] + [_I32] * 5 + [ptr]
+    so.pkv_copy_pages.argtypes = [ptr] * 5 + [_I32] * 6 + [ptr]
+    so.pkv_paged_prefill_attention.argtypes = [ptr, i64] + [ptr] * 7 + [size] + [_I32] * 9 + [ptr]
+    for f in (so.pkv_norm_rope, so.pkv_norm_rope_write_kv, so.pkv_fork_rows, so.pkv_free_rows, so.pkv_compact_pages,
+              so.pkv_copy_pages, so.pkv_paged_prefill_attention):
+        f.restype = ctypes.c_int
+    so.pkv_page_workspace_bytes.argtypes = [_I32]
+    so.pkv_paged_prefill_workspace_bytes.argtypes = [_I32] * 4
+    so.pkv_page_workspace_bytes.restype = so.pkv_paged_prefill_workspace_bytes.restype = size
     _lib = so
     return so
 

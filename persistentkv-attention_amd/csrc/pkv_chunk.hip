@@ -40,6 +40,8 @@ namespace {
 constexpr int kIds = 512;      // page ids in LDS
 constexpr int kMinTiles = 4;
 constexpr int kSmallBatch = 64;  // rows of a table whose plan every wave makes for itself
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kStateFloats = kD + 2;  // of one row: its sums, maximum and sum of weights
 
 struct ChunkArgs {
@@ -73,14 +75,23 @@ __device__ inline int tiles_of(int len) { return (int)(((uint32_t)len + kKeys - 
 template <int ROWS>
 __device__ inline int blocks_of(const ChunkArgs& a, int n) { return (int)(((uint32_t)(n * a.group) + ROWS - 1) / ROWS); }
 
-__device__ inline double wave_sum(double x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
+template <int CTRL, int ROW_MASK>
+__device__ inline float add_lane(float x) {  // 0 where the lane has no source
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROW_MASK, 0xf, false));
 }
-// `tiles`: blocks times tiles of all rows, whole and so the same in any order (below 2^53).
-__device__ inline int part_tiles(const ChunkArgs& a, double tiles) {
-  return max(kMinTiles, (int)fmin(ceil(tiles * a.hkv / a.parts), 1e9));
+__device__ inline float wave_sum(float x) {
+  x = add_lane<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8; row_bcast 15, 31
+  x = add_lane<0x112, 0xf>(x);
+  x = add_lane<0x114, 0xf>(x);
+  x = add_lane<0x118, 0xf>(x);
+  x = add_lane<0x142, 0xa>(x);
+  x = add_lane<0x143, 0xc>(x);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+// C for the sum of blocks times tiles of all rows: a little more than W / P, so that the roundings of
+// the sum (less than 2^-17 of it) never make more parts than the grid and the workspace hold.
+__device__ inline int part_tiles(const ChunkArgs& a, float tiles) {
+  return max(kMinTiles, (int)fminf(ceilf(tiles * (float)a.hkv / (float)a.parts * 1.0001f), 1e9f));
 }
 __device__ inline int parts_of(int tiles, int each) { return max((int)(((uint32_t)tiles + each - 1) / each), 1); }
 
@@ -104,18 +115,18 @@ constexpr int kPlanThreads = 1024;
 template <int ROWS>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
   constexpr int kPlanWaves = kPlanThreads / 64;
-  __shared__ double total[kPlanWaves];
+  __shared__ float total[kPlanWaves];
   __shared__ int sums[3][kPlanWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  double tiles = 0;
+  float tiles = 0.f;
   for (int b = tid; b < a.batch; b += kPlanThreads) {
     const Seq s = seq_of(a, b);
-    tiles += (double)blocks_of<ROWS>(a, s.n) * tiles_of(s.len);
+    tiles += (float)blocks_of<ROWS>(a, s.n) * (float)tiles_of(s.len);
   }
   tiles = wave_sum(tiles);
   if (lane == 0) total[wave] = tiles;
   __syncthreads();
-  tiles = 0;
+  tiles = 0.f;
   for (int w = 0; w < kPlanWaves; ++w) tiles += total[w];
   const int each = part_tiles(a, tiles);
   int before[3] = {0, 0, 0};
@@ -166,7 +177,7 @@ __device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
   if (a.batch <= kSmallBatch) {
     Seq s{0, 0, 0, 0};
     if (lane < a.batch) s = seq_of(a, lane);
-    u.each = uniform(part_tiles(a, wave_sum((double)blocks_of<ROWS>(a, s.n) * tiles_of(s.len))));
+    u.each = uniform(part_tiles(a, wave_sum((float)blocks_of<ROWS>(a, s.n) * (float)tiles_of(s.len))));
     const Share x = share_of<ROWS>(a, s, u.each);
     const int units = wave_scan(x.units), states = wave_scan(x.states);
     const uint64_t past = __builtin_amdgcn_ballot_w64(units > slot);
@@ -216,6 +227,14 @@ __device__ inline void load_to_lds(uint32_t lds, const uint8_t* from) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(from) : "memory");
 }
 
+// The lane's number, made anew where it is asked for: what follows from it is then neither kept
+// in registers from tile to tile nor computed before the first one and spilled.
+__device__ inline int fresh_lane() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+  return x;
+}
+
 // GROUPS = 1: four waves of 32 rows each.  2: two pairs of waves share 64 rows' tiles, the even
 // ones and the odd ones, and join their sums.
 template <class Elem, int GROUPS>
@@ -224,8 +243,8 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
   constexpr int kGroupBytes = kBuffers * 2 * kTileBytes;
   __shared__ __attribute__((aligned(1024))) uint8_t all_lds[GROUPS * kGroupBytes];
   __shared__ int ids[kIds];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int group = GROUPS == 1 ? 0 : uniform(tid >> 6) / kGroupWaves, wave = (tid >> 6) - group * kGroupWaves;
+  const int lane = threadIdx.x & 63, workgroup_wave = uniform((int)threadIdx.x >> 6);
+  const int group = GROUPS == 1 ? 0 : workgroup_wave / kGroupWaves, wave = workgroup_wave - group * kGroupWaves;
   uint8_t* const lds = all_lds + group * kGroupBytes;  // K and V of the group's tiles
   const int col = lane & 31, half = lane >> 5;
   const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
@@ -259,11 +278,9 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
   // (K) or of 64 bytes of four rows (V) spread over all banks.
   constexpr int kMoved = kKeys / kGroupWaves;
   constexpr int kLoads = kMoved / 4;  // per wave and tile of K, and of V
-  const int srow = wave * kMoved + (lane >> 4), chunk = lane & 15;
   const uint32_t lds0 = (uint32_t)uniform((int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds +
                                                 (uint32_t)(wave * kMoved * kRowBytes)));
   const uint32_t head = (uint32_t)(kvh * a.page_size) * kRowBytes;
-  const uint32_t kchunk = (chunk ^ (srow & 15)) << 4, vchunk = (chunk ^ ((srow & 3) << 2)) << 4;
   const int32_t* const table = a.block_table + (long)u.row * a.max_pages;
   // ids[] holds the pages from `first_id` on, of the tiles before `id_end`.
   const int window = (int)min((long)(kIds - 1) * a.page_size / kKeys, 1L << 26);
@@ -272,12 +289,14 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
     first_id = uniform(page_index(a, tile * kKeys));
     id_end = tile + window;
     const int last = page_index(a, len - 1);
-    for (int i = tid; i < kIds && first_id + i <= last; i += kWaves * 64)
+    for (int i = workgroup_wave * 64 + fresh_lane(); i < kIds && first_id + i <= last; i += kWaves * 64)
       ids[i] = min(max(table[first_id + i], 0), a.num_pages - 1);
     __syncthreads();
   };
   auto fetch = [&](int i, int buf) __attribute__((always_inline)) {  // the group's i-th tile
     const uint32_t to = (uint32_t)uniform((int)(lds0 + buf * 2 * kTileBytes));
+    const int l = fresh_lane(), srow = wave * kMoved + (l >> 4), chunk = l & 15;
+    const uint32_t kchunk = (chunk ^ (srow & 15)) << 4, vchunk = (chunk ^ ((srow & 3) << 2)) << 4;
     const int key0 = (tile0 + GROUPS * i + group) * kKeys + srow;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
@@ -324,7 +343,7 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
   bool careful = false;
   const int masked = max((last_key(seq, block * kRows / a.group) + 1) / kKeys - tile0, 0) / GROUPS;
   auto clean = [&](int buf) {
-    u32x4* const v = (u32x4*)(lds + buf * 2 * kTileBytes + kTileBytes) + wave * 64 + lane;
+    u32x4* const v = (u32x4*)(lds + buf * 2 * kTileBytes + kTileBytes) + wave * 64 + fresh_lane();
     for (int i = 0; i < kTileBytes / 16; i += kGroupWaves * 64) {
       u32x4 x = v[i];
 #pragma unroll
@@ -407,7 +426,6 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
     else landed<0>();
     __syncthreads();
   };
-  u32x2 out[16];
   for (;;) {
     landed<0>();
     __syncthreads();
@@ -423,7 +441,7 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
       step(i + 2, 2);
     }
     if constexpr (GROUPS > 1) {  // the second group's sums to the first's waves
-      float* const at = (float*)all_lds + wave * 66 * 64 + lane;
+      float* const at = (float*)all_lds + wave * 66 * 64 + fresh_lane();
       if (group == 1) {
 #pragma unroll
         for (int j = 0; j < 64; ++j) at[j * 64] = o[j >> 4][j & 15];
@@ -440,6 +458,7 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
       __syncthreads();  // the places are free
     }
     if (careful) {
+      const int half = fresh_lane() >> 5;
       const int stop = min(see, end * kKeys - 1);
       for (int key = (tile0 + masked * GROUPS) * kKeys; key <= stop; ++key) {
         const int page = page_index(a, key), id = min(max(table[page], 0), a.num_pages - 1);
@@ -454,57 +473,48 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
           }
       }
     }
-    // `zero` turns NaN where a value is not finite.
+    // The rows go out; where one is not finite (`zero` is NaN), once more after the second pass.
     const float sum = l + __shfl_xor(l, 32);
     float zero = 0.f;
-    if (whole) {  // the rows in the output's type; 0 for a token that sees no key
-      const float inv = see < 0 ? 0.f : 1.0f / sum;
-#pragma unroll
-      for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const uint32_t x = Elem::pack2(o[db][i] * inv, o[db][i + 1] * inv);
-          out[4 * db + (i >> 2)][(i >> 1) & 1] = x;
-          zero = Elem::times0(x, zero);
-        }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 64; ++j) zero = __builtin_fmaf(o[j >> 4][j & 15], 0.f, zero);
-    }
-    l = sum;
-    if (careful || !__syncthreads_or(group == 0 && live > 0 && zero != 0.f)) break;
-    careful = true;
-    begin();
-  }
-
-  if (group != 0) return;
-  if (!whole) {
-    if (col < live) {
+    const int here = fresh_lane(), col = here & 31, half = here >> 5;
+    if (group == 0 && !whole) {
       const long state = ((long)u.states + (long)part * rows + row0 + col) * a.hkv + kvh;
       float* const to = a.sums + state * kD + 4 * half;
-      typedef float f32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-      for (int c = 0; c < 16; ++c)
-        *(f32x4*)(to + 8 * c) = f32x4{o[c >> 2][4 * (c & 3)], o[c >> 2][4 * (c & 3) + 1], o[c >> 2][4 * (c & 3) + 2],
-                                      o[c >> 2][4 * (c & 3) + 3]};
-      if (half == 0) *(f32x2*)(a.tops + 2 * state) = f32x2{m, l};
+      for (int c = 0; c < 16; ++c) {
+        const f32x4 x{o[c >> 2][4 * (c & 3)], o[c >> 2][4 * (c & 3) + 1], o[c >> 2][4 * (c & 3) + 2], o[c >> 2][4 * (c & 3) + 3]};
+        if (col < live) *(f32x4*)(to + 8 * c) = x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(x[i], 0.f, zero);
+      }
+      if (half == 0 && col < live) *(f32x2*)(a.tops + 2 * state) = f32x2{m, sum};
+    } else if (group == 0) {
+      // In the output's type, 0 for a token that sees no key.  The wave's 32 rows pass through LDS,
+      // so that 16 lanes write one row of 256 bytes; 16-byte chunks lie under an exclusive or with
+      // the row.
+      const float inv = see < 0 ? 0.f : 1.0f / sum;
+      uint8_t* const mine = lds + wave * kWaveRows * kRowBytes;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const float* const x = (const float*)&o[c >> 2] + 4 * (c & 3);
+        const u32x2 y{Elem::pack2(x[0] * inv, x[1] * inv), Elem::pack2(x[2] * inv, x[3] * inv)};
+        zero = Elem::times0(y[1], Elem::times0(y[0], zero));
+        *(u32x2*)(mine + col * kRowBytes + ((c ^ (col & 15)) << 4) + 8 * half) = y;
+      }
+      // Row R of the (sequence, KV head), a row of its token t, is row R + t (Hq - G) of the output.
+      uint8_t* const to = a.output + ((long)start * a.hq + kvh * a.group + row0 + (long)tok0 * (a.hq - a.group)) * kRowBytes +
+                          (here & 15) * 16;
+#pragma unroll
+      for (int i = 0; i < kWaveRows / 4; ++i) {
+        const int j = 4 * i + (here >> 4);
+        if (j < live)
+          *(u32x4*)(to + (long)(j + token_of(j) * (a.hq - a.group)) * kRowBytes) =
+              *(const u32x4*)(mine + j * kRowBytes + (((here & 15) ^ (j & 15)) << 4));
+      }
     }
-    return;
-  }
-  // The wave's 32 rows pass through LDS, so that 16 lanes write one row of 256 bytes; 16-byte
-  // chunks lie under an exclusive or with the row.
-  uint8_t* const mine = lds + wave * kWaveRows * kRowBytes;
-#pragma unroll
-  for (int c = 0; c < 16; ++c) *(u32x2*)(mine + col * kRowBytes + ((c ^ (col & 15)) << 4) + 8 * half) = out[c];
-  // Row R of the (sequence, KV head), a row of its token t, is row R + t (Hq - G) of the output.
-  uint8_t* const to = a.output + ((long)start * a.hq + kvh * a.group + row0 + (long)tok0 * (a.hq - a.group)) * kRowBytes +
-                      (lane & 15) * 16;
-#pragma unroll
-  for (int i = 0; i < kWaveRows / 4; ++i) {
-    const int j = 4 * i + (lane >> 4);
-    if (j < live)
-      *(u32x4*)(to + (long)(j + token_of(j) * (a.hq - a.group)) * kRowBytes) =
-          *(const u32x4*)(mine + j * kRowBytes + (((lane & 15) ^ (j & 15)) << 4));
+    if (careful || !__syncthreads_or(live > 0 && zero != 0.f)) return;
+    careful = true;
+    begin();
   }
 }
 
@@ -513,7 +523,6 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
 constexpr int kJoin = 8;
 template <class Elem, int ROWS>
 __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
-  typedef float f32x4 __attribute__((ext_vector_type(4)));
   __shared__ f32x4 part_sums[kJoin][32];
   __shared__ float part_m[kJoin], part_l[kJoin];
   __shared__ int small_states[kSmallBatch + 1], small_joins[kSmallBatch + 1];
@@ -522,7 +531,7 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
   if (a.batch <= kSmallBatch) {
     Seq s{0, 0, 0, 0};
     if (lane < a.batch) s = seq_of(a, lane);
-    each = part_tiles(a, wave_sum((double)blocks_of<ROWS>(a, s.n) * tiles_of(s.len)));
+    each = part_tiles(a, wave_sum((float)blocks_of<ROWS>(a, s.n) * (float)tiles_of(s.len)));
     const Share x = share_of<ROWS>(a, s, each);
     const int states = wave_scan(x.states), joins = wave_scan(x.joins);
     if (tid < 64) {

@@ -37,6 +37,7 @@ int ok();
 
 namespace {
 
+constexpr int kRows = kWaves * kWaveRows;  // of a block
 constexpr int kIds = 512;      // page ids in LDS
 constexpr int kMinTiles = 4;
 constexpr int kSmallBatch = 64;  // rows of a table whose plan every wave makes for itself
@@ -55,8 +56,9 @@ struct ChunkArgs {
   int32_t* plan;                 // of more than kSmallBatch rows
   float* sums;                   // [state rows, Hkv, 128]
   float* tops;                   // [state rows, Hkv, 2]: maximum, sum of weights
-  long q_stride, page_bytes;
+  long q_stride;
   int32_t batch, tokens, hq, hkv, group, num_pages, max_pages, page_size, parts;
+  uint32_t page_bytes;
   uint32_t page_magic, page_shift;  // key / page_size = mulhi(2 key, magic) >> shift, key < 2^31
   float inv_group;
 };
@@ -72,8 +74,7 @@ __device__ inline Seq seq_of(const ChunkArgs& a, int b) {
   return {start, n, total - n, min(total, a.max_pages * a.page_size)};
 }
 __device__ inline int tiles_of(int len) { return (int)(((uint32_t)len + kKeys - 1) / kKeys); }
-template <int ROWS>
-__device__ inline int blocks_of(const ChunkArgs& a, int n) { return (int)(((uint32_t)(n * a.group) + ROWS - 1) / ROWS); }
+__device__ inline int blocks_of(const ChunkArgs& a, int n) { return (int)(((uint32_t)(n * a.group) + kRows - 1) / kRows); }
 
 template <int CTRL, int ROW_MASK>
 __device__ inline float add_lane(float x) {  // 0 where the lane has no source
@@ -100,10 +101,9 @@ __device__ inline int parts_of(int tiles, int each) { return max((int)(((uint32_
 struct Share {
   int units, states, joins;
 };
-template <int ROWS>
 __device__ inline Share share_of(const ChunkArgs& a, const Seq& s, int each) {
   const int parts = parts_of(tiles_of(s.len), each), rows = parts > 1 ? s.n * a.group : 0;
-  return {blocks_of<ROWS>(a, s.n) * parts, rows * parts, rows};
+  return {blocks_of(a, s.n) * parts, rows * parts, rows};
 }
 
 // The plan in memory: C, 0, then for every row of the table, and behind the last, the sums before it.
@@ -112,7 +112,6 @@ __device__ inline int32_t* states_before(const ChunkArgs& a) { return a.plan + 2
 __device__ inline int32_t* joins_before(const ChunkArgs& a) { return a.plan + 2 + 2 * (a.batch + 1); }
 
 constexpr int kPlanThreads = 1024;
-template <int ROWS>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
   constexpr int kPlanWaves = kPlanThreads / 64;
   __shared__ float total[kPlanWaves];
@@ -121,7 +120,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
   float tiles = 0.f;
   for (int b = tid; b < a.batch; b += kPlanThreads) {
     const Seq s = seq_of(a, b);
-    tiles += (float)blocks_of<ROWS>(a, s.n) * (float)tiles_of(s.len);
+    tiles += (float)blocks_of(a, s.n) * (float)tiles_of(s.len);
   }
   tiles = wave_sum(tiles);
   if (lane == 0) total[wave] = tiles;
@@ -134,7 +133,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
   for (int base = 0; base <= a.batch; base += kPlanThreads) {
     const int b = base + tid;
     Share x{0, 0, 0};
-    if (b < a.batch) x = share_of<ROWS>(a, seq_of(a, b), each);
+    if (b < a.batch) x = share_of(a, seq_of(a, b), each);
     const int mine[3] = {x.units, x.states, x.joins};
     int sum[3];
 #pragma unroll
@@ -170,15 +169,14 @@ __device__ inline Seq seq_from(const Seq& s, int lane) {
 
 // Units go through the rows of the table, part by part, a part's last block first: the blocks at
 // work at one time share their keys in L2.
-template <int ROWS>
 __device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
   Unit u;
   int unit;
   if (a.batch <= kSmallBatch) {
     Seq s{0, 0, 0, 0};
     if (lane < a.batch) s = seq_of(a, lane);
-    u.each = uniform(part_tiles(a, wave_sum((float)blocks_of<ROWS>(a, s.n) * (float)tiles_of(s.len))));
-    const Share x = share_of<ROWS>(a, s, u.each);
+    u.each = uniform(part_tiles(a, wave_sum((float)blocks_of(a, s.n) * (float)tiles_of(s.len))));
+    const Share x = share_of(a, s, u.each);
     const int units = wave_scan(x.units), states = wave_scan(x.states);
     const uint64_t past = __builtin_amdgcn_ballot_w64(units > slot);
     u.block = -1;
@@ -207,7 +205,7 @@ __device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
     u.states = uniform(states_before(a)[u.row]);
     unit = slot - uniform(first[u.row]);
   }
-  const int blocks = blocks_of<ROWS>(a, u.seq.n);
+  const int blocks = blocks_of(a, u.seq.n);
   u.part = unit / blocks;
   u.block = blocks - 1 - (unit - u.part * blocks);
   return u;
@@ -235,20 +233,14 @@ __device__ inline int fresh_lane() {
   return x;
 }
 
-// GROUPS = 1: four waves of 32 rows each.  2: two pairs of waves share 64 rows' tiles, the even
-// ones and the odd ones, and join their sums.
-template <class Elem, int GROUPS>
-__global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel(ChunkArgs a) {
-  constexpr int kGroupWaves = kWaves / GROUPS, kRows = kGroupWaves * kWaveRows;
-  constexpr int kGroupBytes = kBuffers * 2 * kTileBytes;
-  __shared__ __attribute__((aligned(1024))) uint8_t all_lds[GROUPS * kGroupBytes];
+template <class Elem>
+__global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers * 2 * kTileBytes];  // K and V of a tile
   __shared__ int ids[kIds];
-  const int lane = threadIdx.x & 63, workgroup_wave = uniform((int)threadIdx.x >> 6);
-  const int group = GROUPS == 1 ? 0 : workgroup_wave / kGroupWaves, wave = workgroup_wave - group * kGroupWaves;
-  uint8_t* const lds = all_lds + group * kGroupBytes;  // K and V of the group's tiles
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
-  const Unit u = unit_of<kRows>(a, uniform((int)(blockIdx.x / (unsigned)a.hkv)), lane);
+  const Unit u = unit_of(a, uniform((int)(blockIdx.x / (unsigned)a.hkv)), lane);
   if (u.block < 0) return;
   const int start = uniform(u.seq.start), n = uniform(u.seq.n), len = uniform(u.seq.len);
   const Seq seq{start, n, uniform(u.seq.before), len};
@@ -270,13 +262,12 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
   if (part > 0 && tile0 >= block_tiles) return;
   const int end = min(block_tiles, tile0 + uniform(u.each));
   const bool whole = block_tiles <= u.each;
-  const int tiles = (end - tile0 - group + GROUPS - 1) / GROUPS;  // the group's: tile0 + GROUPS i + group
-  const int steps = (end - tile0 + GROUPS - 1) / GROUPS;
+  const int tiles = end - tile0;
 
   // A wave moves rows kMoved wave + 4 i + lane / 16 of a tile, 256 bytes a row.  16-byte chunk p of
   // row r in LDS is chunk p ^ r of K's row (p ^ 4 r of V's), so that reads of one chunk column
   // (K) or of 64 bytes of four rows (V) spread over all banks.
-  constexpr int kMoved = kKeys / kGroupWaves;
+  constexpr int kMoved = kKeys / kWaves;
   constexpr int kLoads = kMoved / 4;  // per wave and tile of K, and of V
   const uint32_t lds0 = (uint32_t)uniform((int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds +
                                                 (uint32_t)(wave * kMoved * kRowBytes)));
@@ -289,26 +280,30 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
     first_id = uniform(page_index(a, tile * kKeys));
     id_end = tile + window;
     const int last = page_index(a, len - 1);
-    for (int i = workgroup_wave * 64 + fresh_lane(); i < kIds && first_id + i <= last; i += kWaves * 64)
+    for (int i = wave * 64 + fresh_lane(); i < kIds && first_id + i <= last; i += kWaves * 64)
       ids[i] = min(max(table[first_id + i], 0), a.num_pages - 1);
     __syncthreads();
   };
-  auto fetch = [&](int i, int buf) __attribute__((always_inline)) {  // the group's i-th tile
+  auto fetch = [&](int i, int buf) __attribute__((always_inline)) {  // the i-th tile
     const uint32_t to = (uint32_t)uniform((int)(lds0 + buf * 2 * kTileBytes));
     const int l = fresh_lane(), srow = wave * kMoved + (l >> 4), chunk = l & 15;
     const uint32_t kchunk = (chunk ^ (srow & 15)) << 4, vchunk = (chunk ^ ((srow & 3) << 2)) << 4;
-    const int key0 = (tile0 + GROUPS * i + group) * kKeys + srow;
+    const int key0 = (tile0 + i) * kKeys + srow;
+    uint64_t at[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int key = min(key0 + 4 * j, len - 1), page = page_index(a, key);
-      const uint64_t at = (uint64_t)(uint32_t)ids[page - first_id] * (uint64_t)a.page_bytes +
-                          (head + (uint32_t)(key - page * a.page_size) * kRowBytes);
-      load_to_lds(to + j * 4 * kRowBytes, a.k_pages + at + (kchunk ^ (j << 6)));
-      load_to_lds(to + kTileBytes + j * 4 * kRowBytes, a.v_pages + at + vchunk);
+      at[j] = (uint64_t)(uint32_t)ids[page - first_id] * a.page_bytes +
+              (head + (uint32_t)(key - page * a.page_size) * kRowBytes);
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      load_to_lds(to + j * 4 * kRowBytes, a.k_pages + at[j] + (kchunk ^ (j << 6)));
+      load_to_lds(to + kTileBytes + j * 4 * kRowBytes, a.v_pages + at[j] + vchunk);
     }
   };
   auto begin = [&]() __attribute__((always_inline)) {
-    if (steps > 0) renew_ids(tile0);
+    if (tiles > 0) renew_ids(tile0);
     if (tiles > 0) fetch(0, 0);
     if (tiles > 1) fetch(1, 1);
   };
@@ -341,10 +336,10 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
   // that a row of it masks in part, those of the steps from `masked` on (the keys read twice past
   // the end among them), and put back at the end for the rows that see their token.
   bool careful = false;
-  const int masked = max((last_key(seq, block * kRows / a.group) + 1) / kKeys - tile0, 0) / GROUPS;
+  const int masked = max((last_key(seq, block * kRows / a.group) + 1) / kKeys - tile0, 0);
   auto clean = [&](int buf) {
     u32x4* const v = (u32x4*)(lds + buf * 2 * kTileBytes + kTileBytes) + wave * 64 + fresh_lane();
-    for (int i = 0; i < kTileBytes / 16; i += kGroupWaves * 64) {
+    for (int i = 0; i < kTileBytes / 16; i += kWaves * 64) {
       u32x4 x = v[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = drop_nonfinite<Elem>(x[j]);
@@ -353,20 +348,24 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
     __syncthreads();
   };
 
-  // The group's i-th tile, which lies in buffer `buf`.
+  // The i-th tile, which lies in buffer `buf`.
   auto step = [&](int i, int buf) __attribute__((always_inline)) {
     const int at = buf * 2 * kTileBytes;
     if (careful && i >= masked) clean(buf);
-    if (GROUPS * (i + 3) > id_end - tile0 && GROUPS * (i + 2) < end - tile0) {
+    if (i + 2 < tiles && tile0 + i + 2 >= id_end) {
       __syncthreads();  // the old ids have been read
-      renew_ids(tile0 + GROUPS * (i + 2));
+      renew_ids(tile0 + i + 2);
     }
-    if (i + 2 < tiles) fetch(i + 2, buf >= 1 ? buf - 1 : buf + 2);
-    const int k0 = (tile0 + GROUPS * i + group) * kKeys;
-    if (k0 <= wave_last && (GROUPS == 1 || i < tiles)) {
-      f32x16 s = {};
+    const int k0 = (tile0 + i) * kKeys;
+    const bool on = k0 <= wave_last;
+    f32x16 s = {};
+    if (on) {
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) s = Elem::mma(*(const u32x4*)(kat[kk] + at), q[kk], s);
+    }
+    // Under the products: the addresses take about 40 instructions and a read of LDS.
+    if (i + 2 < tiles) fetch(i + 2, buf >= 1 ? buf - 1 : buf + 2);
+    if (on) {
       auto value = [&](int c, int db) __attribute__((always_inline)) {  // keys 16 c ..., dims 32 db + lane % 32
         typedef __attribute__((address_space(3))) s16x4* Lds;
         const uint8_t* v = vat[db] + at + c * 16 * kRowBytes;
@@ -433,36 +432,19 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
     large = true;
 #pragma unroll
     for (int db = 0; db < 4; ++db) o[db] = f32x16{};
-    for (int i = 0; i < steps; i += kBuffers) {  // LDS places known at compile time
+    for (int i = 0; i < tiles; i += kBuffers) {  // LDS places known at compile time
       step(i, 0);
-      if (i + 1 >= steps) break;
+      if (i + 1 >= tiles) break;
       step(i + 1, 1);
-      if (i + 2 >= steps) break;
+      if (i + 2 >= tiles) break;
       step(i + 2, 2);
-    }
-    if constexpr (GROUPS > 1) {  // the second group's sums to the first's waves
-      float* const at = (float*)all_lds + wave * 66 * 64 + fresh_lane();
-      if (group == 1) {
-#pragma unroll
-        for (int j = 0; j < 64; ++j) at[j * 64] = o[j >> 4][j & 15];
-        at[64 * 64] = m, at[65 * 64] = l;
-      }
-      __syncthreads();
-      if (group == 0) {
-        const float m1 = at[64 * 64], l1 = at[65 * 64], mn = fmaxf(m, m1);
-        const float c0 = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2), c1 = __builtin_amdgcn_exp2f((m1 - mn) * kScaleLog2);
-        m = mn, l = l * c0 + l1 * c1;
-#pragma unroll
-        for (int j = 0; j < 64; ++j) o[j >> 4][j & 15] = o[j >> 4][j & 15] * c0 + at[j * 64] * c1;
-      }
-      __syncthreads();  // the places are free
     }
     if (careful) {
       const int half = fresh_lane() >> 5;
       const int stop = min(see, end * kKeys - 1);
-      for (int key = (tile0 + masked * GROUPS) * kKeys; key <= stop; ++key) {
+      for (int key = (tile0 + masked) * kKeys; key <= stop; ++key) {
         const int page = page_index(a, key), id = min(max(table[page], 0), a.num_pages - 1);
-        const u32x2* const x = (const u32x2*)(a.v_pages + (uint64_t)(uint32_t)id * (uint64_t)a.page_bytes +
+        const u32x2* const x = (const u32x2*)(a.v_pages + (uint64_t)(uint32_t)id * a.page_bytes +
                                               (head + (uint32_t)(key - page * a.page_size) * kRowBytes)) + half;
 #pragma unroll
         for (int c = 0; c < 16; ++c)
@@ -477,23 +459,33 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
     const float sum = l + __shfl_xor(l, 32);
     float zero = 0.f;
     const int here = fresh_lane(), col = here & 31, half = here >> 5;
-    if (group == 0 && !whole) {
-      const long state = ((long)u.states + (long)part * rows + row0 + col) * a.hkv + kvh;
-      float* const to = a.sums + state * kD + 4 * half;
+    // The wave's 32 rows pass through LDS, so that 16 lanes write 256 bytes of one; 16-byte chunks lie
+    // under an exclusive or with the row.
+    uint8_t* const mine = lds + wave * kWaveRows * kRowBytes;
+    if (!whole) {  // sums in 32 bits, half of a row's dims at a time
+      const long state = ((long)u.states + (long)part * rows + row0) * a.hkv + kvh;
+      float* const to = a.sums + (state + (long)(here >> 4) * a.hkv) * kD + 4 * (here & 15);
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const f32x4 x{o[c >> 2][4 * (c & 3)], o[c >> 2][4 * (c & 3) + 1], o[c >> 2][4 * (c & 3) + 2], o[c >> 2][4 * (c & 3) + 3]};
-        if (col < live) *(f32x4*)(to + 8 * c) = x;
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(x[i], 0.f, zero);
+        for (int c = 0; c < 8; ++c) {
+          const f32x16& y = o[2 * h + (c >> 2)];
+          const f32x4 x{y[4 * (c & 3)], y[4 * (c & 3) + 1], y[4 * (c & 3) + 2], y[4 * (c & 3) + 3]};
+          *(f32x4*)(mine + col * kRowBytes + (((2 * c + half) ^ (col & 15)) << 4)) = x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(x[i], 0.f, zero);
+        }
+#pragma unroll
+        for (int i = 0; i < kWaveRows / 4; ++i) {
+          const int j = 4 * i + (here >> 4);
+          const f32x4 x = *(const f32x4*)(mine + j * kRowBytes + (((here & 15) ^ (j & 15)) << 4));
+          if (j < live) *(f32x4*)(to + (long)i * 4 * a.hkv * kD + 64 * h) = x;
+        }
       }
-      if (half == 0 && col < live) *(f32x2*)(a.tops + 2 * state) = f32x2{m, sum};
-    } else if (group == 0) {
-      // In the output's type, 0 for a token that sees no key.  The wave's 32 rows pass through LDS,
-      // so that 16 lanes write one row of 256 bytes; 16-byte chunks lie under an exclusive or with
-      // the row.
+      if (half == 0 && col < live) *(f32x2*)(a.tops + 2 * (state + (long)col * a.hkv)) = f32x2{m, sum};
+    } else {
+      // In the output's type, 0 for a token that sees no key.
       const float inv = see < 0 ? 0.f : 1.0f / sum;
-      uint8_t* const mine = lds + wave * kWaveRows * kRowBytes;
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
         const float* const x = (const float*)&o[c >> 2] + 4 * (c & 3);
@@ -518,10 +510,10 @@ __global__ __launch_bounds__(kWaves * 64, GROUPS == 1 ? 3 : 1) void chunk_kernel
   }
 }
 
-// Joins the parts of the rows that were cut: 32 lanes hold a row, four dims each, and kJoin of them
-// take its parts in turn.
+// Joins the parts of the rows that were cut.  32 lanes hold a row, four dims each.  With fewer rows
+// than such groups of lanes, the kJoin groups of a workgroup share one row's parts out.
 constexpr int kJoin = 8;
-template <class Elem, int ROWS>
+template <class Elem>
 __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
   __shared__ f32x4 part_sums[kJoin][32];
   __shared__ float part_m[kJoin], part_l[kJoin];
@@ -531,8 +523,8 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
   if (a.batch <= kSmallBatch) {
     Seq s{0, 0, 0, 0};
     if (lane < a.batch) s = seq_of(a, lane);
-    each = part_tiles(a, wave_sum((float)blocks_of<ROWS>(a, s.n) * (float)tiles_of(s.len)));
-    const Share x = share_of<ROWS>(a, s, each);
+    each = part_tiles(a, wave_sum((float)blocks_of(a, s.n) * (float)tiles_of(s.len)));
+    const Share x = share_of(a, s, each);
     const int states = wave_scan(x.states), joins = wave_scan(x.joins);
     if (tid < 64) {
       small_states[lane] = states - x.states, small_joins[lane] = joins - x.joins;
@@ -545,7 +537,9 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
   const bool small = a.batch <= kSmallBatch;
   auto joins_at = [&](int b) { return small ? small_joins[b] : joins_before(a)[b]; };
   const long total = (long)joins_at(a.batch) * a.hkv;
-  for (long i = blockIdx.x; i < total; i += gridDim.x) {
+  const bool shared = total <= (long)gridDim.x * kJoin;  // one row a workgroup at a time
+  const int first = shared ? sub : 0, stride = shared ? kJoin : 1;
+  for (long i = shared ? blockIdx.x : (long)blockIdx.x * kJoin + sub; i < total; i += (long)gridDim.x * (shared ? 1 : kJoin)) {
     const int join = (int)(i / a.hkv), kvh = (int)(i - (long)join * a.hkv);
     int b = 0;  // the last row of the table whose first join is at most `join`
     for (int step = 1 << (31 - __builtin_clz(a.batch)); step; step >>= 1)
@@ -553,27 +547,40 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
     const Seq s = seq_of(a, b);
     const int row = join - joins_at(b), rows = s.n * a.group;
     const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
-    const int last = min((row / ROWS + 1) * ROWS, rows) - 1;
+    const int last = min((row / kRows + 1) * kRows, rows) - 1;
     const int parts = parts_of(tiles_of(last_key(s, last / a.group) + 1), each);
     if (parts == 1) continue;  // written by its only part
-    const long states = small ? small_states[b] : states_before(a)[b];
+    const long state = ((long)(small ? small_states[b] : states_before(a)[b]) + row) * a.hkv + kvh, next = (long)rows * a.hkv;
+    const float* const tops = a.tops + 2 * state;
+    const float* const sums = a.sums + state * kD + 4 * quad;
     float m = -FLT_MAX, l = 0.f;
     f32x4 o = {};
-    for (int p = sub; p < parts; p += kJoin) {
-      const long state = (states + (long)p * rows + row) * a.hkv + kvh;
-      const f32x2 top = *(const f32x2*)(a.tops + 2 * state);
-      const f32x4 x = *(const f32x4*)(a.sums + state * kD + 4 * quad);
-      const float mn = fmaxf(m, top[0]);
-      const float c0 = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2), c1 = __builtin_amdgcn_exp2f((top[0] - mn) * kScaleLog2);
-      m = mn, l = l * c0 + top[1] * c1;
+    for (int p = first; p < parts; p += 4 * stride) {  // four parts' loads at once
+      f32x2 top[4];
+      f32x4 x[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = o[j] * c0 + x[j] * c1;
+      for (int k = 0; k < 4; ++k) {
+        top[k] = f32x2{-FLT_MAX, 0.f}, x[k] = f32x4{};
+        if (p + k * stride < parts) {
+          top[k] = *(const f32x2*)(tops + 2 * (p + k * stride) * next);
+          x[k] = *(const f32x4*)(sums + (p + k * stride) * next * kD);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float mn = fmaxf(m, top[k][0]);
+        const float c0 = __builtin_amdgcn_exp2f((m - mn) * kScaleLog2), c1 = __builtin_amdgcn_exp2f((top[k][0] - mn) * kScaleLog2);
+        m = mn, l = l * c0 + top[k][1] * c1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = o[j] * c0 + x[k][j] * c1;
+      }
     }
-    __syncthreads();  // the row before has been read
-    part_sums[sub][quad] = o;
-    if (quad == 0) part_m[sub] = m, part_l[sub] = l;
-    __syncthreads();
-    if (sub == 0) {
+    if (shared) {
+      __syncthreads();  // the row before has been read
+      part_sums[sub][quad] = o;
+      if (quad == 0) part_m[sub] = m, part_l[sub] = l;
+      __syncthreads();
+      if (sub != 0) continue;
       for (int p = 1; p < kJoin; ++p) m = fmaxf(m, part_m[p]);
       l = 0.f, o = f32x4{};
       for (int p = 0; p < kJoin; ++p) {
@@ -583,10 +590,10 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] += x[j] * c;
       }
-      const float inv = last_key(s, tok) < 0 ? 0.f : 1.0f / l;
-      *(u32x2*)(a.output + (((long)s.start + tok) * a.hq + head) * kRowBytes + 8 * quad) =
-          u32x2{Elem::pack2(o[0] * inv, o[1] * inv), Elem::pack2(o[2] * inv, o[3] * inv)};
     }
+    const float inv = last_key(s, tok) < 0 ? 0.f : 1.0f / l;
+    *(u32x2*)(a.output + (((long)s.start + tok) * a.hq + head) * kRowBytes + 8 * quad) =
+        u32x2{Elem::pack2(o[0] * inv, o[1] * inv), Elem::pack2(o[2] * inv, o[3] * inv)};
   }
 }
 
@@ -595,20 +602,17 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
 // ---------------------------------------------------------------------------------
 int parts_wanted() { return 2 * pkv::compute_units(); }
 
-// The blocks of `rows` rows that a call can have, over all KV heads.
-int64_t blocks_at_most(int64_t batch, int64_t tokens, int64_t group, int64_t hkv, int rows) {
-  return (tokens * group / rows + batch) * hkv;
-}
-bool shares_keys(int64_t batch, int64_t tokens, int64_t group, int64_t hkv) {
-  return blocks_at_most(batch, tokens, group, hkv, kWaves * kWaveRows) <= pkv::compute_units() / 2;
+// The blocks that a call can have, over all KV heads.
+int64_t blocks_at_most(int64_t batch, int64_t tokens, int64_t group, int64_t hkv) {
+  return (tokens * group / kRows + batch) * hkv;
 }
 size_t plan_bytes(int64_t batch) { return batch > kSmallBatch ? (size_t)((2 + 3 * (batch + 1)) * 4 + 15) / 16 * 16 : 0; }
 
 // Rows of states, over all KV heads: a row of the table is cut only where its tiles pass C >= W / P,
 // so that its parts are at most 2 tiles / C, and all rows' at most 2 P blocks' or calls' rows.
-int64_t states_at_most(int64_t tokens, int64_t group, int rows) {
+int64_t states_at_most(int64_t tokens, int64_t group) {
   const int64_t all = tokens * group;
-  return 2 * (int64_t)parts_wanted() * (all < rows ? all : rows);
+  return 2 * (int64_t)parts_wanted() * (all < kRows ? all : kRows);
 }
 
 }  // namespace
@@ -618,8 +622,7 @@ extern "C" {
 size_t pkv_paged_prefill_workspace_bytes(int32_t batch, int32_t tokens, int32_t num_q_heads, int32_t num_kv_heads) {
   if (batch <= 0 || tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return 0;
   const int64_t group = num_q_heads / num_kv_heads;
-  const int rows = kWaves * kWaveRows / (shares_keys(batch, tokens, group, num_kv_heads) ? 2 : 1);
-  return plan_bytes(batch) + (size_t)states_at_most(tokens, group, rows) * kStateFloats * sizeof(float);
+  return plan_bytes(batch) + (size_t)states_at_most(tokens, group) * kStateFloats * sizeof(float);
 }
 
 int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
@@ -644,9 +647,8 @@ int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_p
   const int64_t page_bytes = (int64_t)num_kv_heads * page_size * kRowBytes;
   if ((int64_t)max_pages * page_size > INT32_MAX - kKeys || page_bytes > INT32_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "%s: max_pages * page_size must be below 2^31 - 32, and a page below 2 GiB", op);
-  const bool split = shares_keys(batch, tokens, group, num_kv_heads);
-  const int rows = kWaves * kWaveRows / (split ? 2 : 1), parts = parts_wanted();
-  const int64_t groups = blocks_at_most(batch, tokens, group, num_kv_heads, rows) +
+  const int parts = parts_wanted();
+  const int64_t groups = blocks_at_most(batch, tokens, group, num_kv_heads) +
                          (int64_t)((parts + num_kv_heads - 1) / num_kv_heads) * num_kv_heads;
   if ((int64_t)tokens * group > INT32_MAX || !pkv::fits_grid(groups, kWaves * 64))
     return fail(PKV_ERR_UNSUPPORTED, "%s: too many tokens or sequences", op);
@@ -670,17 +672,15 @@ int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_p
   const uint64_t magic = ((1ull << (31 + log2)) + page_size - 1) / page_size;
   float* const states = (float*)((uint8_t*)workspace + plan_bytes(batch));
   const ChunkArgs a{(const uint8_t*)q, (const uint8_t*)k_pages, (const uint8_t*)v_pages, block_table, seq_lens, token_offsets,
-                    (uint8_t*)output, (int32_t*)workspace, states, states + states_at_most(tokens, group, rows) * kD,
-                    2 * q_stride, page_bytes, batch, tokens, num_q_heads, num_kv_heads, group, num_pages, max_pages,
-                    page_size, parts, (uint32_t)magic, log2, 1.0f / (float)group};
+                    (uint8_t*)output, (int32_t*)workspace, states, states + states_at_most(tokens, group) * kD,
+                    2 * q_stride, batch, tokens, num_q_heads, num_kv_heads, group, num_pages, max_pages, page_size, parts,
+                    (uint32_t)page_bytes, (uint32_t)magic, log2, 1.0f / (float)group};
   const hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == PKV_DTYPE_BF16;
-  if (batch > kSmallBatch) (split ? plan_kernel<64> : plan_kernel<128>)<<<1, kPlanThreads, 0, st>>>(a);
-  auto* const kernel = split ? (bf16 ? chunk_kernel<BFloat, 2> : chunk_kernel<Half, 2>)
-                             : (bf16 ? chunk_kernel<BFloat, 1> : chunk_kernel<Half, 1>);
+  if (batch > kSmallBatch) plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+  auto* const kernel = bf16 ? chunk_kernel<BFloat> : chunk_kernel<Half>;
   kernel<<<dim3((unsigned)groups), dim3(kWaves * 64), 0, st>>>(a);
-  auto* const join = split ? (bf16 ? join_kernel<BFloat, 64> : join_kernel<Half, 64>)
-                           : (bf16 ? join_kernel<BFloat, 128> : join_kernel<Half, 128>);
+  auto* const join = bf16 ? join_kernel<BFloat> : join_kernel<Half>;
   join<<<dim3((unsigned)(4 * pkv::compute_units())), dim3(32 * kJoin), 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? pkv::ok() : fail(PKV_ERR_LAUNCH, "%s launch: %s", op, hipGetErrorString(e));

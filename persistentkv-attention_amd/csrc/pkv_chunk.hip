@@ -45,6 +45,14 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStateFloats = kD + 2;  // of one row: its sums, maximum and sum of weights
 
+// x / d for 0 <= x < 2^31 as mulhi(2 x, magic) >> shift: with 2^shift the power of two at or above d and
+// magic = ceil(2^(31 + shift) / d), which is below 2^32, the error x (magic d - 2^(31 + shift)) is below
+// 2^(31 + shift).
+struct Divisor {
+  uint32_t magic, shift;
+};
+__device__ inline int quotient(int x, Divisor d) { return (int)(__umulhi(2 * (uint32_t)x, d.magic) >> d.shift); }
+
 struct ChunkArgs {
   const uint8_t* q;  // token t, head h at q + t * q_stride + h * 256 (bytes)
   const uint8_t* k_pages;  // [num_pages, Hkv, ps, 128]
@@ -59,7 +67,7 @@ struct ChunkArgs {
   long q_stride;
   int32_t batch, tokens, hq, hkv, group, num_pages, max_pages, page_size, parts;
   uint32_t page_bytes;
-  uint32_t page_magic, page_shift;  // key / page_size = mulhi(2 key, magic) >> shift, key < 2^31
+  Divisor by_page, by_group, by_heads;  // page_size, group, hkv
   float inv_group;
 };
 
@@ -167,6 +175,13 @@ __device__ inline Seq seq_from(const Seq& s, int lane) {
           __builtin_amdgcn_readlane(s.before, lane), __builtin_amdgcn_readlane(s.len, lane)};
 }
 
+// x / d for x below 2^24 and a result below 2^20, which the product with 1 / d misses by one at most.
+__device__ inline int small_quotient(int x, int d) {
+  const int y = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+  const int r = x - y * d;
+  return y + (r >= d) - (r < 0);
+}
+
 // Units go through the rows of the table, part by part, a part's last block first: the blocks at
 // work at one time share their keys in L2.
 __device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
@@ -206,7 +221,7 @@ __device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
     unit = slot - uniform(first[u.row]);
   }
   const int blocks = blocks_of(a, u.seq.n);
-  u.part = unit / blocks;
+  u.part = small_quotient(unit, blocks);
   u.block = blocks - 1 - (unit - u.part * blocks);
   return u;
 }
@@ -214,15 +229,16 @@ __device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
 // The last key that token i of a row sees; -1: none.
 __device__ inline int last_key(const Seq& s, int i) { return max(min(s.before + i, s.len - 1), -1); }
 
-__device__ inline int page_index(const ChunkArgs& a, int key) {
-  return (int)(__umulhi(2 * (uint32_t)key, a.page_magic) >> a.page_shift);
-}
-
 // 64 x 16 bytes straight to LDS, lane l's to `lds` + 16 l.  In assembly because the compiler lets
-// every LDS read wait for every such load in flight; landed() is the wait.  m0 must be one wait
-// state old.
+// every LDS read wait for every such load in flight; landed() is the wait.  m0, which nothing else in
+// these kernels uses, must be one wait state old, and a scalar register that a vector instruction has
+// written (a descriptor's or base's, by readfirstlane or as a spilled one brought back) five: the
+// compiler keeps no distances to instructions in assembly, so this text carries them.
 __device__ inline void load_to_lds(uint32_t lds, const uint8_t* from) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(from) : "memory");
+}
+__device__ inline void load_to_lds(uint32_t lds, const uint8_t* base, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
 // The lane's number, made anew where it is asked for: what follows from it is then neither kept
@@ -239,8 +255,8 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   __shared__ int ids[kIds];
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int kvh = uniform((int)(blockIdx.x % (unsigned)a.hkv));
-  const Unit u = unit_of(a, uniform((int)(blockIdx.x / (unsigned)a.hkv)), lane);
+  const int slot = quotient((int)blockIdx.x, a.by_heads), kvh = (int)blockIdx.x - slot * a.hkv;
+  const Unit u = unit_of(a, slot, lane);
   if (u.block < 0) return;
   const int start = uniform(u.seq.start), n = uniform(u.seq.n), len = uniform(u.seq.len);
   const Seq seq{start, n, uniform(u.seq.before), len};
@@ -249,7 +265,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   // Row row0 + r of the wave is token tok0 + (rem + r) / G: a quotient of numbers below 64, which
   // the product with 1 / G in 32 bits gives exactly (it is off by less than 1 / (2 G)).
   const int row0 = uniform(min(block * kRows + wave * kWaveRows, rows));
-  const int tok0 = row0 / a.group, rem = row0 - tok0 * a.group, live = rows - row0;  // may be 0
+  const int tok0 = quotient(row0, a.by_group), rem = row0 - tok0 * a.group, live = rows - row0;  // may be 0
   auto token_of = [&](int r) { return (int)(((float)(rem + r) + 0.5f) * a.inv_group); };
   const int last_row = max(min(kWaveRows, live) - 1, 0);
   const int r = min(col, last_row), dt = token_of(r);
@@ -257,7 +273,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   const int see = last_key(seq, tok);
   const int wave_first = last_key(seq, min(tok0, n - 1));
   const int wave_last = live > 0 ? last_key(seq, tok0 + uniform(token_of(last_row))) : -1;
-  const int block_tiles = tiles_of(last_key(seq, (min((block + 1) * kRows, rows) - 1) / a.group) + 1);
+  const int block_tiles = tiles_of(last_key(seq, quotient(min((block + 1) * kRows, rows) - 1, a.by_group)) + 1);
   const int part = uniform(u.part), tile0 = part * uniform(u.each);
   if (part > 0 && tile0 >= block_tiles) return;
   const int end = min(block_tiles, tile0 + uniform(u.each));
@@ -277,29 +293,44 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   const int window = (int)min((long)(kIds - 1) * a.page_size / kKeys, 1L << 26);
   int first_id = 0, id_end = 0;
   auto renew_ids = [&](int tile) __attribute__((always_inline)) {
-    first_id = uniform(page_index(a, tile * kKeys));
+    first_id = uniform(quotient(tile * kKeys, a.by_page));
     id_end = tile + window;
-    const int last = page_index(a, len - 1);
+    const int last = quotient(len - 1, a.by_page);
     for (int i = wave * 64 + fresh_lane(); i < kIds && first_id + i <= last; i += kWaves * 64)
       ids[i] = min(max(table[first_id + i], 0), a.num_pages - 1);
     __syncthreads();
   };
+  // A wave's rows of a tile are eight keys in a row.  In pages of a multiple of 8 they lie in one page,
+  // whose place is found once for all lanes; else, and at the row's end, every lane finds its own.
+  static_assert(kMoved == 8 && kLoads == 2);
+  const uint32_t row_in = (uint32_t)lane >> 4, swizzle = (8 * (wave & 1) + row_in) ^ ((uint32_t)lane & 15);
+  const uint32_t koff = row_in * kRowBytes + (swizzle << 4);
+  const uint32_t voff = row_in * kRowBytes + ((((uint32_t)lane & 15) ^ (row_in << 2)) << 4);
+  const bool eights = a.page_size % 8 == 0;
   auto fetch = [&](int i, int buf) __attribute__((always_inline)) {  // the i-th tile
-    const uint32_t to = (uint32_t)uniform((int)(lds0 + buf * 2 * kTileBytes));
-    const int l = fresh_lane(), srow = wave * kMoved + (l >> 4), chunk = l & 15;
-    const uint32_t kchunk = (chunk ^ (srow & 15)) << 4, vchunk = (chunk ^ ((srow & 3) << 2)) << 4;
-    const int key0 = (tile0 + i) * kKeys + srow;
-    uint64_t at[kLoads];
+    const uint32_t to = lds0 + buf * 2 * kTileBytes;
+    const int key0 = (tile0 + i) * kKeys + wave * kMoved;
+    if (eights && key0 + kMoved <= len) {
+      const int page = quotient(key0, a.by_page);
+      const uint64_t at = (uint64_t)(uint32_t)uniform(ids[page - first_id]) * a.page_bytes +
+                          (head + (uint32_t)(key0 - page * a.page_size) * kRowBytes);
+      const uint8_t* const k = a.k_pages + at;
+      const uint8_t* const v = a.v_pages + at;
+      load_to_lds(to, k, koff);
+      load_to_lds(to + 4 * kRowBytes, k + 4 * kRowBytes, koff ^ 64);
+      load_to_lds(to + kTileBytes, v, voff);
+      load_to_lds(to + kTileBytes + 4 * kRowBytes, v + 4 * kRowBytes, voff);
+    } else {
+      const int l = fresh_lane(), chunk = l & 15;
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int key = min(key0 + 4 * j, len - 1), page = page_index(a, key);
-      at[j] = (uint64_t)(uint32_t)ids[page - first_id] * a.page_bytes +
-              (head + (uint32_t)(key - page * a.page_size) * kRowBytes);
-    }
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      load_to_lds(to + j * 4 * kRowBytes, a.k_pages + at[j] + (kchunk ^ (j << 6)));
-      load_to_lds(to + kTileBytes + j * 4 * kRowBytes, a.v_pages + at[j] + vchunk);
+      for (int j = 0; j < kLoads; ++j) {
+        const int srow = wave * kMoved + 4 * j + (l >> 4);
+        const int key = min((tile0 + i) * kKeys + srow, len - 1), page = quotient(key, a.by_page);
+        const uint64_t at = (uint64_t)(uint32_t)ids[page - first_id] * a.page_bytes +
+                            (head + (uint32_t)(key - page * a.page_size) * kRowBytes);
+        load_to_lds(to + j * 4 * kRowBytes, a.k_pages + at + ((chunk ^ (srow & 15)) << 4));
+        load_to_lds(to + kTileBytes + j * 4 * kRowBytes, a.v_pages + at + ((chunk ^ ((srow & 3) << 2)) << 4));
+      }
     }
   };
   auto begin = [&]() __attribute__((always_inline)) {
@@ -336,7 +367,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   // that a row of it masks in part, those of the steps from `masked` on (the keys read twice past
   // the end among them), and put back at the end for the rows that see their token.
   bool careful = false;
-  const int masked = max((last_key(seq, block * kRows / a.group) + 1) / kKeys - tile0, 0);
+  const int masked = max((last_key(seq, quotient(block * kRows, a.by_group)) + 1) / kKeys - tile0, 0);
   auto clean = [&](int buf) {
     u32x4* const v = (u32x4*)(lds + buf * 2 * kTileBytes + kTileBytes) + wave * 64 + fresh_lane();
     for (int i = 0; i < kTileBytes / 16; i += kWaves * 64) {
@@ -356,16 +387,12 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
       __syncthreads();  // the old ids have been read
       renew_ids(tile0 + i + 2);
     }
+    if (i + 2 < tiles) fetch(i + 2, buf >= 1 ? buf - 1 : buf + 2);
     const int k0 = (tile0 + i) * kKeys;
-    const bool on = k0 <= wave_last;
-    f32x16 s = {};
-    if (on) {
+    if (k0 <= wave_last) {
+      f32x16 s = {};
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) s = Elem::mma(*(const u32x4*)(kat[kk] + at), q[kk], s);
-    }
-    // Under the products: the addresses take about 40 instructions and a read of LDS.
-    if (i + 2 < tiles) fetch(i + 2, buf >= 1 ? buf - 1 : buf + 2);
-    if (on) {
       auto value = [&](int c, int db) __attribute__((always_inline)) {  // keys 16 c ..., dims 32 db + lane % 32
         typedef __attribute__((address_space(3))) s16x4* Lds;
         const uint8_t* v = vat[db] + at + c * 16 * kRowBytes;
@@ -443,7 +470,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
       const int half = fresh_lane() >> 5;
       const int stop = min(see, end * kKeys - 1);
       for (int key = (tile0 + masked) * kKeys; key <= stop; ++key) {
-        const int page = page_index(a, key), id = min(max(table[page], 0), a.num_pages - 1);
+        const int page = quotient(key, a.by_page), id = min(max(table[page], 0), a.num_pages - 1);
         const u32x2* const x = (const u32x2*)(a.v_pages + (uint64_t)(uint32_t)id * a.page_bytes +
                                               (head + (uint32_t)(key - page * a.page_size) * kRowBytes)) + half;
 #pragma unroll
@@ -600,6 +627,12 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
 // ---------------------------------------------------------------------------------
 // Host.
 // ---------------------------------------------------------------------------------
+Divisor divisor(int d) {
+  uint32_t shift = 0;
+  while ((1u << shift) < (uint32_t)d) ++shift;
+  return {(uint32_t)(((1ull << (31 + shift)) + d - 1) / d), shift};
+}
+
 int parts_wanted() { return 2 * pkv::compute_units(); }
 
 // The blocks that a call can have, over all KV heads.
@@ -667,21 +700,19 @@ int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_p
   if (!(output == q && (tokens == 1 || 2 * q_stride == row)) &&
       pkv::meets_rows(output, tokens * row, q, tokens, 2 * q_stride, row))
     return fail(PKV_ERR_INVALID_ARGUMENT, "%s: output must be a contiguous q itself, or not overlap q", op);
-  uint32_t log2 = 0;  // ceil(log2(page_size)); magic = ceil(2^(31 + log2) / page_size) is at most 2^32 - 1 but for powers of two
-  while ((1u << log2) < (uint32_t)page_size) ++log2;
-  const uint64_t magic = ((1ull << (31 + log2)) + page_size - 1) / page_size;
   float* const states = (float*)((uint8_t*)workspace + plan_bytes(batch));
   const ChunkArgs a{(const uint8_t*)q, (const uint8_t*)k_pages, (const uint8_t*)v_pages, block_table, seq_lens, token_offsets,
                     (uint8_t*)output, (int32_t*)workspace, states, states + states_at_most(tokens, group) * kD,
                     2 * q_stride, batch, tokens, num_q_heads, num_kv_heads, group, num_pages, max_pages, page_size, parts,
-                    (uint32_t)page_bytes, (uint32_t)magic, log2, 1.0f / (float)group};
+                    (uint32_t)page_bytes, divisor(page_size), divisor(group), divisor(num_kv_heads), 1.0f / (float)group};
   const hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == PKV_DTYPE_BF16;
   if (batch > kSmallBatch) plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
   auto* const kernel = bf16 ? chunk_kernel<BFloat> : chunk_kernel<Half>;
   kernel<<<dim3((unsigned)groups), dim3(kWaves * 64), 0, st>>>(a);
   auto* const join = bf16 ? join_kernel<BFloat> : join_kernel<Half>;
-  join<<<dim3((unsigned)(4 * pkv::compute_units())), dim3(32 * kJoin), 0, st>>>(a);
+  const int64_t joins = (int64_t)tokens * num_q_heads, most = 4L * pkv::compute_units();
+  join<<<dim3((unsigned)(joins < most ? joins : most)), dim3(32 * kJoin), 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? pkv::ok() : fail(PKV_ERR_LAUNCH, "%s launch: %s", op, hipGetErrorString(e));
 }

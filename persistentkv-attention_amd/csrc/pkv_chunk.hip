@@ -97,53 +97,76 @@ __device__ inline float wave_sum(float x) {
   x = add_lane<0x143, 0xc>(x);
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
-// C for the sum of blocks times tiles of all rows: a little more than W / P, so that the roundings of
+// Rows whose tokens are one wave's ("small": decoding rows, guessed tokens) and others have budgets of
+// their own: a small row's parts cost little memory, and cut finer than long pieces of prompts they
+// fill the compute units that those leave.
+__device__ inline bool is_small(const ChunkArgs& a, const Seq& s) { return s.n * a.group <= kWaveRows; }
+__device__ inline float tiles_in(const ChunkArgs& a, const Seq& s) { return (float)blocks_of(a, s.n) * (float)tiles_of(s.len); }
+struct Cut {
+  int large, small;  // the most tiles of a part
+};
+// For the sum of blocks times tiles of a class: a little more than W / P, so that the roundings of
 // the sum (less than 2^-17 of it) never make more parts than the grid and the workspace hold.
 __device__ inline int part_tiles(const ChunkArgs& a, float tiles) {
   return max(kMinTiles, (int)fminf(ceilf(tiles * (float)a.hkv / (float)a.parts * 1.0001f), 1e9f));
 }
-__device__ inline int parts_of(int tiles, int each) { return max((int)(((uint32_t)tiles + each - 1) / each), 1); }
+__device__ inline int ratio_up(int x, int d) { return (int)(((uint32_t)x + d - 1) / d); }
+// A row's parts, as even as whole tiles are.
+struct Parts {
+  int count, tiles;
+};
+__device__ inline Parts parts_of(const ChunkArgs& a, const Seq& s, const Cut& cut) {
+  const int tiles = tiles_of(s.len), count = max(ratio_up(tiles, is_small(a, s) ? cut.small : cut.large), 1);
+  return {count, max(ratio_up(tiles, count), 1)};
+}
 
-// What a row adds to the plan's three running sums: units of work (blocks by parts), rows of states
-// in the workspace, and rows to join.
+// What a row adds to the plan's running sums: units of work (blocks by parts), rows of states in the
+// workspace, and rows to join.
 struct Share {
   int units, states, joins;
 };
-__device__ inline Share share_of(const ChunkArgs& a, const Seq& s, int each) {
-  const int parts = parts_of(tiles_of(s.len), each), rows = parts > 1 ? s.n * a.group : 0;
+__device__ inline Share share_of(const ChunkArgs& a, const Seq& s, const Cut& cut) {
+  const int parts = parts_of(a, s, cut).count, rows = parts > 1 ? s.n * a.group : 0;
   return {blocks_of(a, s.n) * parts, rows * parts, rows};
 }
 
-// The plan in memory: C, 0, then for every row of the table, and behind the last, the sums before it.
+// The plan in memory: the cut; the units before every row of the table, the large rows' first, then
+// the small ones' (2 batch + 1 numbers); the states and the joins before every row (batch + 1 each).
 __device__ inline int32_t* units_before(const ChunkArgs& a) { return a.plan + 2; }
-__device__ inline int32_t* states_before(const ChunkArgs& a) { return a.plan + 2 + (a.batch + 1); }
-__device__ inline int32_t* joins_before(const ChunkArgs& a) { return a.plan + 2 + 2 * (a.batch + 1); }
+__device__ inline int32_t* states_before(const ChunkArgs& a) { return a.plan + 3 + 2 * a.batch; }
+__device__ inline int32_t* joins_before(const ChunkArgs& a) { return a.plan + 4 + 3 * a.batch; }
 
 constexpr int kPlanThreads = 1024;
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
   constexpr int kPlanWaves = kPlanThreads / 64;
-  __shared__ float total[kPlanWaves];
+  __shared__ float total[2][kPlanWaves];
   __shared__ int sums[3][kPlanWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  float tiles = 0.f;
+  float tiles[2] = {0.f, 0.f};
   for (int b = tid; b < a.batch; b += kPlanThreads) {
     const Seq s = seq_of(a, b);
-    tiles += (float)blocks_of(a, s.n) * (float)tiles_of(s.len);
+    tiles[is_small(a, s)] += tiles_in(a, s);
   }
-  tiles = wave_sum(tiles);
-  if (lane == 0) total[wave] = tiles;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    tiles[i] = wave_sum(tiles[i]);
+    if (lane == 0) total[i][wave] = tiles[i];
+  }
   __syncthreads();
-  tiles = 0.f;
-  for (int w = 0; w < kPlanWaves; ++w) tiles += total[w];
-  const int each = part_tiles(a, tiles);
+  tiles[0] = tiles[1] = 0.f;
+  for (int w = 0; w < kPlanWaves; ++w) tiles[0] += total[0][w], tiles[1] += total[1][w];
+  const Cut cut{part_tiles(a, tiles[0]), part_tiles(a, tiles[1])};
   int before[3] = {0, 0, 0};
   int32_t* const to[3] = {units_before(a), states_before(a), joins_before(a)};
-  for (int base = 0; base <= a.batch; base += kPlanThreads) {
-    const int b = base + tid;
-    Share x{0, 0, 0};
-    if (b < a.batch) x = share_of(a, seq_of(a, b), each);
-    const int mine[3] = {x.units, x.states, x.joins};
-    int sum[3];
+  for (int base = 0; base <= 2 * a.batch; base += kPlanThreads) {
+    const int e = base + tid, b = e < a.batch ? e : e - a.batch;
+    int mine[3] = {0, 0, 0}, sum[3];
+    if (e < 2 * a.batch) {
+      const Seq s = seq_of(a, b);
+      const Share x = share_of(a, s, cut);
+      if (is_small(a, s) == (e >= a.batch)) mine[0] = x.units;
+      if (e < a.batch) mine[1] = x.states, mine[2] = x.joins;
+    }
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
       sum[i] = wave_scan(mine[i]);
@@ -157,17 +180,34 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
         if (w < wave) at += sums[i][w];
         before[i] += sums[i][w];
       }
-      if (b <= a.batch) to[i][b] = at;
+      if (e <= (i == 0 ? 2 : 1) * a.batch) to[i][e] = at;
     }
     __syncthreads();
   }
-  if (tid == 0) a.plan[0] = each;
+  if (tid == 0) a.plan[0] = cut.large, a.plan[1] = cut.small;
 }
 
-// A unit of work: part `part` of block `block` of a row of the table.  block < 0: none.
+// The plan of up to kSmallBatch rows, lane b's row, made by every wave for itself.
+struct LanePlan {
+  Seq seq;
+  Cut cut;
+  Share share;
+  bool small;
+};
+__device__ inline LanePlan lane_plan(const ChunkArgs& a, int lane) {
+  LanePlan p{};
+  if (lane < a.batch) p.seq = seq_of(a, lane);
+  p.small = is_small(a, p.seq);
+  const float tiles = tiles_in(a, p.seq);
+  p.cut = {part_tiles(a, wave_sum(p.small ? 0.f : tiles)), part_tiles(a, wave_sum(p.small ? tiles : 0.f))};
+  p.share = share_of(a, p.seq, p.cut);
+  return p;
+}
+
+// A unit of work: part `part`, of `tiles` tiles, of block `block` of a row of the table.  block < 0: none.
 struct Unit {
   Seq seq;
-  int row, block, part, each, states;
+  int row, block, part, tiles, states;
 };
 
 __device__ inline Seq seq_from(const Seq& s, int lane) {
@@ -182,47 +222,70 @@ __device__ inline int small_quotient(int x, int d) {
   return y + (r >= d) - (r < 0);
 }
 
-// Units go through the rows of the table, part by part, a part's last block first: the blocks at
-// work at one time share their keys in L2.
+// Which unit of its class the `slot`-th is: two of large rows, which wait for products, then one of
+// small ones, which wait for memory, as long as there are both.
+struct Turn {
+  bool small;
+  int unit;  // negative: none
+};
+__device__ inline Turn turn_of(int slot, int large, int small) {
+  const int thirds = min(large >> 1, small), third = (int)(__umulhi((uint32_t)slot, 0xaaaaaaabu) >> 1);
+  if (third < thirds) {
+    const int r = slot - 3 * third;
+    return r < 2 ? Turn{false, 2 * third + r} : Turn{true, third};
+  }
+  slot -= thirds;  // less the small ones
+  if (slot < large) return {false, slot};
+  slot -= large - thirds;  // the small ones again, less the large
+  return {true, slot < small ? slot : -1};
+}
+
+// Units go through the rows of their class; a row's part by part, a part's last block first: the
+// blocks at work at one time share their keys in L2.
 __device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
   Unit u;
-  int unit;
+  u.block = -1;
+  Cut cut;
   if (a.batch <= kSmallBatch) {
-    Seq s{0, 0, 0, 0};
-    if (lane < a.batch) s = seq_of(a, lane);
-    u.each = uniform(part_tiles(a, wave_sum((float)blocks_of(a, s.n) * (float)tiles_of(s.len))));
-    const Share x = share_of(a, s, u.each);
-    const int units = wave_scan(x.units), states = wave_scan(x.states);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(units > slot);
-    u.block = -1;
-    if (!past) return u;
-    u.row = __builtin_ctzll(past);
-    u.seq = seq_from(s, u.row);
-    u.states = __builtin_amdgcn_readlane(states - x.states, u.row);
-    unit = slot - __builtin_amdgcn_readlane(units - x.units, u.row);
+    const LanePlan p = lane_plan(a, lane);
+    const int large = wave_scan(p.small ? 0 : p.share.units), small = wave_scan(p.small ? p.share.units : 0);
+    const Turn t = turn_of(slot, __builtin_amdgcn_readlane(large, 63), __builtin_amdgcn_readlane(small, 63));
+    if (t.unit < 0) return u;
+    const int units = t.small ? small : large, own = t.small == p.small ? p.share.units : 0;
+    slot = t.unit;
+    const int states = wave_scan(p.share.states);
+    u.row = __builtin_ctzll(__builtin_amdgcn_ballot_w64(units > slot));
+    u.seq = seq_from(p.seq, u.row);
+    u.states = __builtin_amdgcn_readlane(states - p.share.states, u.row);
+    slot -= __builtin_amdgcn_readlane(units - own, u.row);
+    cut = p.cut;
   } else {
     // The last row whose first unit is at most `slot` (rows without units share the next one's),
     // found among 64 candidates at a time.
     const int32_t* const first = units_before(a);
-    u.each = uniform(a.plan[0]);
-    u.block = -1;
-    if (slot >= uniform(first[a.batch])) return u;
-    int b = 0, n = a.batch;
+    const int large = uniform(first[a.batch]);
+    const Turn t = turn_of(slot, large, uniform(first[2 * a.batch]) - large);
+    if (t.unit < 0) return u;
+    slot = t.unit + (t.small ? large : 0);
+    int b = 0, n = 2 * a.batch;
     while (n > 1) {
       const int stride = (n + 63) / 64, at = b + lane * stride;
-      const uint64_t fits = __builtin_amdgcn_ballot_w64(lane * stride < n && first[min(at, a.batch)] <= slot);
+      const uint64_t fits = __builtin_amdgcn_ballot_w64(lane * stride < n && first[min(at, 2 * a.batch)] <= slot);
       const int found = 63 - __builtin_clzll(fits);  // the first candidate always fits
       n = min(stride, n - found * stride);
       b += found * stride;
     }
-    u.row = uniform(b);
+    b = uniform(b);
+    slot -= uniform(first[b]);
+    u.row = b < a.batch ? b : b - a.batch;
     u.seq = seq_of(a, u.row);
     u.states = uniform(states_before(a)[u.row]);
-    unit = slot - uniform(first[u.row]);
+    cut = {uniform(a.plan[0]), uniform(a.plan[1])};
   }
+  u.tiles = parts_of(a, u.seq, cut).tiles;
   const int blocks = blocks_of(a, u.seq.n);
-  u.part = small_quotient(unit, blocks);
-  u.block = blocks - 1 - (unit - u.part * blocks);
+  u.part = small_quotient(slot, blocks);
+  u.block = blocks - 1 - (slot - u.part * blocks);
   return u;
 }
 
@@ -274,10 +337,10 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   const int wave_first = last_key(seq, min(tok0, n - 1));
   const int wave_last = live > 0 ? last_key(seq, tok0 + uniform(token_of(last_row))) : -1;
   const int block_tiles = tiles_of(last_key(seq, quotient(min((block + 1) * kRows, rows) - 1, a.by_group)) + 1);
-  const int part = uniform(u.part), tile0 = part * uniform(u.each);
+  const int part = uniform(u.part), most = uniform(u.tiles), tile0 = part * most;
   if (part > 0 && tile0 >= block_tiles) return;
-  const int end = min(block_tiles, tile0 + uniform(u.each));
-  const bool whole = block_tiles <= u.each;
+  const int end = min(block_tiles, tile0 + most);
+  const bool whole = block_tiles <= most;
   const int tiles = end - tile0;
 
   // A wave moves rows kMoved wave + 4 i + lane / 16 of a tile, 256 bytes a row.  16-byte chunk p of
@@ -546,20 +609,18 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
   __shared__ float part_m[kJoin], part_l[kJoin];
   __shared__ int small_states[kSmallBatch + 1], small_joins[kSmallBatch + 1];
   const int tid = threadIdx.x, lane = tid & 63, sub = tid >> 5, quad = tid & 31;
-  int each;
+  Cut cut;
   if (a.batch <= kSmallBatch) {
-    Seq s{0, 0, 0, 0};
-    if (lane < a.batch) s = seq_of(a, lane);
-    each = part_tiles(a, wave_sum((float)blocks_of(a, s.n) * (float)tiles_of(s.len)));
-    const Share x = share_of(a, s, each);
-    const int states = wave_scan(x.states), joins = wave_scan(x.joins);
+    const LanePlan p = lane_plan(a, lane);
+    const int states = wave_scan(p.share.states), joins = wave_scan(p.share.joins);
     if (tid < 64) {
-      small_states[lane] = states - x.states, small_joins[lane] = joins - x.joins;
+      small_states[lane] = states - p.share.states, small_joins[lane] = joins - p.share.joins;
       if (lane == 63) small_joins[64] = joins;
     }
+    cut = p.cut;
     __syncthreads();
   } else {
-    each = a.plan[0];
+    cut = {a.plan[0], a.plan[1]};
   }
   const bool small = a.batch <= kSmallBatch;
   auto joins_at = [&](int b) { return small ? small_joins[b] : joins_before(a)[b]; };
@@ -575,8 +636,8 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
     const int row = join - joins_at(b), rows = s.n * a.group;
     const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
     const int last = min((row / kRows + 1) * kRows, rows) - 1;
-    const int parts = parts_of(tiles_of(last_key(s, last / a.group) + 1), each);
-    if (parts == 1) continue;  // written by its only part
+    const int parts = ratio_up(tiles_of(last_key(s, last / a.group) + 1), parts_of(a, s, cut).tiles);
+    if (parts <= 1) continue;  // written by its only part
     const long state = ((long)(small ? small_states[b] : states_before(a)[b]) + row) * a.hkv + kvh, next = (long)rows * a.hkv;
     const float* const tops = a.tops + 2 * state;
     const float* const sums = a.sums + state * kD + 4 * quad;
@@ -639,13 +700,14 @@ int parts_wanted() { return 2 * pkv::compute_units(); }
 int64_t blocks_at_most(int64_t batch, int64_t tokens, int64_t group, int64_t hkv) {
   return (tokens * group / kRows + batch) * hkv;
 }
-size_t plan_bytes(int64_t batch) { return batch > kSmallBatch ? (size_t)((2 + 3 * (batch + 1)) * 4 + 15) / 16 * 16 : 0; }
+size_t plan_bytes(int64_t batch) { return batch > kSmallBatch ? (size_t)((5 + 4 * batch) * 4 + 15) / 16 * 16 : 0; }
 
-// Rows of states, over all KV heads: a row of the table is cut only where its tiles pass C >= W / P,
-// so that its parts are at most 2 tiles / C, and all rows' at most 2 P blocks' or calls' rows.
+// Rows of states, over all KV heads.  A row of the table is cut only where its tiles pass C >= W / P, so
+// that it has at most 2 tiles / C parts, and the parts of all blocks of a class are at most 2 P: of 128
+// rows each for large rows, of 32 for small ones, and of no more than the call has in either case.
 int64_t states_at_most(int64_t tokens, int64_t group) {
   const int64_t all = tokens * group;
-  return 2 * (int64_t)parts_wanted() * (all < kRows ? all : kRows);
+  return 2 * (int64_t)parts_wanted() * ((all < kRows ? all : kRows) + (all < kWaveRows ? all : kWaveRows));
 }
 
 }  // namespace
@@ -680,9 +742,9 @@ int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_p
   const int64_t page_bytes = (int64_t)num_kv_heads * page_size * kRowBytes;
   if ((int64_t)max_pages * page_size > INT32_MAX - kKeys || page_bytes > INT32_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "%s: max_pages * page_size must be below 2^31 - 32, and a page below 2 GiB", op);
-  const int parts = parts_wanted();
+  const int parts = parts_wanted(), classes = (int64_t)tokens * group <= kWaveRows ? 1 : 2;
   const int64_t groups = blocks_at_most(batch, tokens, group, num_kv_heads) +
-                         (int64_t)((parts + num_kv_heads - 1) / num_kv_heads) * num_kv_heads;
+                         (int64_t)((parts + num_kv_heads - 1) / num_kv_heads) * num_kv_heads * classes;
   if ((int64_t)tokens * group > INT32_MAX || !pkv::fits_grid(groups, kWaves * 64))
     return fail(PKV_ERR_UNSUPPORTED, "%s: too many tokens or sequences", op);
   if (batch == 0 || tokens == 0) return pkv::ok();

@@ -65,10 +65,11 @@ struct ChunkArgs {
   float* sums;                   // [state rows, Hkv, 128]
   float* tops;                   // [state rows, Hkv, 2]: maximum, sum of weights
   long q_stride;
-  int32_t batch, tokens, hq, hkv, group, num_pages, max_pages, page_size, parts;
+  int32_t batch, tokens, hq, hkv, group, num_pages, max_pages, page_size;
   uint32_t page_bytes;
   Divisor by_page, by_group, by_heads;  // page_size, group, hkv
   float inv_group;
+  float heads_per_part;  // Hkv / P, and a little more
 };
 
 // A row of the table: its n tokens of the call from `start` on, the first at position `before`
@@ -97,6 +98,16 @@ __device__ inline float wave_sum(float x) {
   x = add_lane<0x143, 0xc>(x);
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
+// x / d for 0 <= x < 2^31, d > 0: the product with 1 / d is off by at most 2^-22 of the result, a
+// second one for what is left over by one.
+__device__ inline int divide(int x, int d) {
+  const float inv = __builtin_amdgcn_rcpf((float)d);
+  int y = (int)((float)x * inv), r = x - y * d;
+  const int more = (int)floorf((float)r * inv);
+  y += more, r -= more * d;
+  return y + (r >= d) - (r < 0);
+}
+
 // Rows whose tokens are one wave's ("small": decoding rows, guessed tokens) and others have budgets of
 // their own: a small row's parts cost little memory, and cut finer than long pieces of prompts they
 // fill the compute units that those leave.
@@ -105,12 +116,12 @@ __device__ inline float tiles_in(const ChunkArgs& a, const Seq& s) { return (flo
 struct Cut {
   int large, small;  // the most tiles of a part
 };
-// For the sum of blocks times tiles of a class: a little more than W / P, so that the roundings of
-// the sum (less than 2^-17 of it) never make more parts than the grid and the workspace hold.
+// C for the sum of blocks times tiles of a class and one KV head: a little more than W / P, so that the
+// roundings of the sum (less than 2^-17 of it) never make more parts than the grid and the workspace hold.
 __device__ inline int part_tiles(const ChunkArgs& a, float tiles) {
-  return max(kMinTiles, (int)fminf(ceilf(tiles * (float)a.hkv / (float)a.parts * 1.0001f), 1e9f));
+  return max(kMinTiles, (int)fminf(ceilf(tiles * a.heads_per_part), 1e9f));
 }
-__device__ inline int ratio_up(int x, int d) { return (int)(((uint32_t)x + d - 1) / d); }
+__device__ inline int ratio_up(int x, int d) { return divide(x + d - 1, d); }
 // A row's parts, as even as whole tiles are.
 struct Parts {
   int count, tiles;
@@ -215,13 +226,6 @@ __device__ inline Seq seq_from(const Seq& s, int lane) {
           __builtin_amdgcn_readlane(s.before, lane), __builtin_amdgcn_readlane(s.len, lane)};
 }
 
-// x / d for x below 2^24 and a result below 2^20, which the product with 1 / d misses by one at most.
-__device__ inline int small_quotient(int x, int d) {
-  const int y = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
-  const int r = x - y * d;
-  return y + (r >= d) - (r < 0);
-}
-
 // Which unit of its class the `slot`-th is: two of large rows, which wait for products, then one of
 // small ones, which wait for memory, as long as there are both.
 struct Turn {
@@ -284,7 +288,7 @@ __device__ inline Unit unit_of(const ChunkArgs& a, int slot, int lane) {
   }
   u.tiles = parts_of(a, u.seq, cut).tiles;
   const int blocks = blocks_of(a, u.seq.n);
-  u.part = small_quotient(slot, blocks);
+  u.part = divide(slot, blocks);
   u.block = blocks - 1 - (slot - u.part * blocks);
   return u;
 }
@@ -312,10 +316,19 @@ __device__ inline int fresh_lane() {
   return x;
 }
 
+// x with the bit BIT the other way, likewise not kept: it seems to depend on the step.
+template <int BIT>
+__device__ inline uint32_t flipped(uint32_t x, int step) {
+  uint32_t y;
+  asm("v_xor_b32 %0, %2, %1" : "=v"(y) : "v"(x), "n"(BIT), "s"(step));
+  return y;
+}
+
 template <class Elem>
 __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers * 2 * kTileBytes];  // K and V of a tile
   __shared__ int ids[kIds];
+  __shared__ int failed[kWaves];
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int slot = quotient((int)blockIdx.x, a.by_heads), kvh = (int)blockIdx.x - slot * a.hkv;
@@ -396,13 +409,6 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
       }
     }
   };
-  auto begin = [&]() __attribute__((always_inline)) {
-    if (tiles > 0) renew_ids(tile0);
-    if (tiles > 0) fetch(0, 0);
-    if (tiles > 1) fetch(1, 1);
-  };
-  begin();
-
   u32x4 q[8];
   const uint8_t* qp = a.q + (start + (long)tok) * a.q_stride +
                       (long)(kvh * a.group + rem + r - dt * a.group) * kRowBytes + half * 16;
@@ -418,12 +424,13 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   f32x16 o[4];
   float m, l;
   bool large = false;  // a row of the wave has a large maximum
-  const uint8_t* kat[8];
-  const uint8_t* vat[4];
+  // Half of the addresses; the others differ in one bit, and are made where they are used.
+  uint32_t kat[4], vat[2];
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk) kat[kk] = lds + (ksrc ^ (kk << 5));
+  for (int kk = 0; kk < 4; ++kk) kat[kk] = lds_at + (ksrc ^ (kk << 5));
 #pragma unroll
-  for (int db = 0; db < 4; ++db) vat[db] = lds + kTileBytes + (vsrc ^ (db << 6));
+  for (int db = 0; db < 2; ++db) vat[db] = lds_at + kTileBytes + (vsrc ^ (db << 6));
 
   // A masked weight is 0, and 0 times an infinity or NaN in V is NaN.  So where a row comes out
   // not finite, its workgroup computes once more, `careful`: such values are taken out of the tiles
@@ -455,10 +462,13 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
     if (k0 <= wave_last) {
       f32x16 s = {};
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) s = Elem::mma(*(const u32x4*)(kat[kk] + at), q[kk], s);
+      for (int kk = 0; kk < 8; ++kk) {
+        const uint32_t k = kk < 4 ? kat[kk] : flipped<128>(kat[kk - 4], i);
+        s = Elem::mma(*(const __attribute__((address_space(3))) u32x4*)(k + at), q[kk], s);
+      }
       auto value = [&](int c, int db) __attribute__((always_inline)) {  // keys 16 c ..., dims 32 db + lane % 32
         typedef __attribute__((address_space(3))) s16x4* Lds;
-        const uint8_t* v = vat[db] + at + c * 16 * kRowBytes;
+        const uint32_t v = (db < 2 ? vat[db] : flipped<128>(vat[db - 2], i)) + at + c * 16 * kRowBytes;
         const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)v));
         const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v + 8 * kRowBytes)));
         return u32x4{v0[0], v0[1], v1[0], v1[1]};
@@ -516,6 +526,9 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
     __syncthreads();
   };
   for (;;) {
+    if (tiles > 0) renew_ids(tile0);
+#pragma unroll 1
+    for (int i = 0; i < min(tiles, 2); ++i) fetch(i, i);
     landed<0>();
     __syncthreads();
     m = -FLT_MAX, l = 0.f;  // finite where a row sees no key, or none but of score -inf
@@ -594,9 +607,15 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
               *(const u32x4*)(mine + j * kRowBytes + (((here & 15) ^ (j & 15)) << 4));
       }
     }
-    if (careful || !__syncthreads_or(live > 0 && zero != 0.f)) return;
+    if (careful) return;
+    const int bad = __builtin_amdgcn_ballot_w64(live > 0 && zero != 0.f) != 0;
+    if (fresh_lane() == 0) failed[wave] = bad;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) any |= failed[w];
+    if (!uniform(any)) return;
     careful = true;
-    begin();
   }
 }
 
@@ -765,8 +784,9 @@ int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_p
   float* const states = (float*)((uint8_t*)workspace + plan_bytes(batch));
   const ChunkArgs a{(const uint8_t*)q, (const uint8_t*)k_pages, (const uint8_t*)v_pages, block_table, seq_lens, token_offsets,
                     (uint8_t*)output, (int32_t*)workspace, states, states + states_at_most(tokens, group) * kD,
-                    2 * q_stride, batch, tokens, num_q_heads, num_kv_heads, group, num_pages, max_pages, page_size, parts,
-                    (uint32_t)page_bytes, divisor(page_size), divisor(group), divisor(num_kv_heads), 1.0f / (float)group};
+                    2 * q_stride, batch, tokens, num_q_heads, num_kv_heads, group, num_pages, max_pages, page_size,
+                    (uint32_t)page_bytes, divisor(page_size), divisor(group), divisor(num_kv_heads), 1.0f / (float)group,
+                    (float)num_kv_heads / (float)parts * 1.0001f};
   const hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == PKV_DTYPE_BF16;
   if (batch > kSmallBatch) plan_kernel<<<1, kPlanThreads, 0, st>>>(a);

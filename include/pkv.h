@@ -496,12 +496,12 @@ int pkv_free_rows(const int32_t* rows, const int32_t* lens, const int32_t* block
  *   block_table_out             the table [batch, max_pages] with its ids mapped (free pages' as -1;
  *                               entries that are no ids stay); it may be block_table itself
  *   page_shares_out             the counts at the new ids, 0 behind; not page_shares itself
- *   free_pages_out              num_pages - 1 down to U, so that the lowest is taken first; it may be
- *                               free_pages itself (both have free_capacity >= num_pages places)
+ *   free_pages_out              num_pages - 1 down to U, so that the lowest is taken first (it and
+ *                               free_pages have free_capacity >= num_pages places; not free_pages itself)
  *   num_free_out [1]            num_pages - U; not num_free itself
  *   copy_src, copy_dst          [num_copies >= num_pages / 2] the moves, for pkv_copy_pages, once for
  *                               every layer's pools; -1 behind them
- * The inputs stay as they are but where outputs are said to lie over them.  Workspace as above. */
+ * The inputs stay as they are but where the table is said to be its own output.  Workspace as above. */
 int pkv_compact_pages(const int32_t* block_table, const int32_t* page_shares, const int32_t* free_pages,
                       const int32_t* num_free, int32_t* page_map, int32_t* block_table_out,
                       int32_t* page_shares_out, int32_t* free_pages_out, int32_t* num_free_out,

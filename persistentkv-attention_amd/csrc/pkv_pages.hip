@@ -31,6 +31,7 @@ constexpr int kMaxPairs = 8000;  // rows of a table, and rows that one call fork
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // The sums of x over the threads before this one, and over all of them.
+template <int WAVES = kWaves>
 __device__ inline void block_scan(int x, int* lds, int& before, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int sum = x;
@@ -44,7 +45,7 @@ __device__ inline void block_scan(int x, int* lds, int& before, int& total) {
   __syncthreads();
   before = sum - x, total = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     if (w < wave) before += lds[w];
     total += lds[w];
   }
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void reclaim_kernel(FreeArgs a, int chunk
   before_chunk(a.counts, chunks, lds, before, total);
   block_scan(n, lds, earlier, unused);
   const int avail = min(max(*a.num_free, 0), a.free_capacity);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.num_free_out = min(avail + total, a.free_capacity);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.num_free_out = (int32_t)min((long)avail + total, (long)a.free_capacity);
   long at = (long)avail + before + earlier;
   const int first = blockIdx.x * kChunk + threadIdx.x * kEach;
 #pragma unroll
@@ -230,6 +231,85 @@ struct CompactArgs {
   int32_t num_pages, free_capacity, copies, chunks;
 };
 
+// Pools of up to kBitPages pages: one launch.  Every workgroup keeps a bit for every page in LDS, and
+// the number of used pages before every 32, reads the whole list for it, and then places its
+// share of the table's entries and of the pages without a word from the others.
+constexpr int kBitPages = 1 << 19;  // 16384 words, twice: 128 of the 160 KB
+constexpr int kBitThreads = 1024;
+struct PageBits {
+  const uint32_t* used;
+  const int* before;
+  int words, total;  // total: of used pages
+  __device__ inline bool is_used(int p) const { return used[p >> 5] >> (p & 31) & 1; }
+  __device__ inline int rank(int p) const { return before[p >> 5] + __popc(used[p >> 5] & ((1u << (p & 31)) - 1)); }
+  // The free page with h free ones before it (there is one).
+  __device__ inline int hole(int h) const {
+    int w = 0;  // the last word with at most h free pages before it
+    for (int step = 1 << (31 - __builtin_clz(words)); step; step >>= 1)
+      if (w + step < words && 32 * (w + step) - before[w + step] <= h) w += step;
+    uint32_t free = ~used[w];
+    for (int skip = h - (32 * w - before[w]); skip > 0; --skip) free &= free - 1;
+    return 32 * w + __builtin_ctz(free);
+  }
+  __device__ inline int place(int p) const {
+    if (!is_used(p)) return -1;
+    return p < total ? p : hole(total - 1 - rank(p));
+  }
+};
+__global__ __launch_bounds__(kBitThreads) void compact_kernel(CompactArgs a) {
+  extern __shared__ uint32_t bits[];  // [words], then the counts [words]
+  __shared__ int lds[kBitThreads / 64];
+  const int tid = threadIdx.x, words = (a.num_pages + 31) / 32;
+  int* const counts = (int*)bits + words;
+  for (int w = tid; w < words; w += kBitThreads) bits[w] = 0xffffffffu;
+  __syncthreads();
+  if (tid == 0 && (a.num_pages & 31)) bits[words - 1] = (1u << (a.num_pages & 31)) - 1;
+  __syncthreads();
+  const int avail = min(max(*a.num_free, 0), a.free_capacity);
+  for (int i = tid; i < avail; i += 4 * kBitThreads) {
+    int page[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) page[k] = i + k * kBitThreads < avail ? a.free_pages[i + k * kBitThreads] : -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if ((unsigned)page[k] < (unsigned)a.num_pages) atomicAnd(&bits[page[k] >> 5], ~(1u << (page[k] & 31)));
+  }
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int base = 0; base < words; base += kBitThreads) {
+    const int w = base + tid;
+    int earlier, sum;
+    block_scan<kBitThreads / 64>(w < words ? __popc(bits[w]) : 0, lds, earlier, sum);
+    if (w < words) counts[w] = before + earlier;
+    before += sum;
+  }
+  total = before;
+  __syncthreads();
+  const PageBits b{bits, counts, words, total};
+  const int moved = total < a.num_pages ? total - b.rank(total) : 0, left = a.num_pages - total;
+  const long id = (long)blockIdx.x * kBitThreads + tid, threads = (long)gridDim.x * kBitThreads;
+  if (id == 0) *a.num_free_out = left;
+  for (long i = id; i < a.entries; i += threads) {
+    const int page = a.block_table[i];
+    a.block_table_out[i] = (unsigned)page < (unsigned)a.num_pages ? b.place(page) : page;
+  }
+  for (long p = id; p < a.num_pages; p += threads) {
+    const int to = b.place((int)p);
+    a.page_map[p] = to;
+    if (to >= 0) a.page_shares_out[to] = a.page_shares[p];
+    if (p >= total) {
+      a.page_shares_out[p] = 0;
+      if (to >= 0) {
+        const int h = total - 1 - b.rank((int)p);
+        a.copy_src[h] = (int)p, a.copy_dst[h] = to;
+      }
+    }
+    if (p < left) a.free_pages_out[p] = a.num_pages - 1 - (int)p;
+  }
+  for (long k = moved + id; k < a.copies; k += threads) a.copy_src[k] = a.copy_dst[k] = -1;
+}
+
+// Larger pools, pass by pass.
 __global__ __launch_bounds__(kThreads) void all_used_kernel(CompactArgs a) {
   const long p = (long)blockIdx.x * kThreads + threadIdx.x;
   if (p < a.num_pages) a.page_map[p] = 0;
@@ -437,9 +517,11 @@ int pkv_compact_pages(const int32_t* block_table, const int32_t* page_shares, co
   if (!page_shares || !free_pages || !num_free || !page_map || !page_shares_out || !free_pages_out || !num_free_out ||
       (num_copies > 0 && (!copy_src || !copy_dst)) || (entries > 0 && (!block_table || !block_table_out)))
     return fail(PKV_ERR_INVALID_ARGUMENT, "compact_pages: null pointer");
-  if (num_free == num_free_out || page_shares == page_shares_out)
-    return fail(PKV_ERR_INVALID_ARGUMENT, "compact_pages: %s_out must not be %s",
-                num_free == num_free_out ? "num_free" : "page_shares", num_free == num_free_out ? "num_free" : "page_shares");
+  const char* const same = num_free == num_free_out         ? "num_free"
+                           : page_shares == page_shares_out ? "page_shares"
+                           : free_pages == free_pages_out   ? "free_pages"
+                                                            : nullptr;
+  if (same) return fail(PKV_ERR_INVALID_ARGUMENT, "compact_pages: %s_out must not be %s", same, same);
   if (!workspace || workspace_size < pkv_page_workspace_bytes(num_pages) || ((uintptr_t)workspace & 3))
     return fail(PKV_ERR_WORKSPACE_TOO_SMALL, "compact_pages: workspace of %zu bytes is smaller than %zu, or misaligned",
                 workspace_size, pkv_page_workspace_bytes(num_pages));
@@ -449,6 +531,16 @@ int pkv_compact_pages(const int32_t* block_table, const int32_t* page_shares, co
                       free_capacity, num_copies, chunks};
   const hipStream_t st = (hipStream_t)stream;
   auto groups = [](int64_t n) { return dim3((unsigned)((n + kThreads - 1) / kThreads)); };
+  if (num_pages <= kBitPages) {
+    const int64_t share = 2L * kBitThreads, wanted = (entries + num_pages + share - 1) / share, units = pkv::compute_units();
+    const size_t lds = (size_t)(num_pages + 31) / 32 * 8;
+    if (lds > 64 * 1024) {
+      const hipError_t e = hipFuncSetAttribute((const void*)compact_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e != hipSuccess) return fail(PKV_ERR_LAUNCH, "compact_pages: %s", hipGetErrorString(e));
+    }
+    compact_kernel<<<dim3((unsigned)(wanted < units ? wanted : units)), dim3(kBitThreads), lds, st>>>(a);
+    return launched("compact_pages");
+  }
   all_used_kernel<<<groups(num_pages), dim3(kThreads), 0, st>>>(a);
   unused_kernel<<<groups(free_capacity), dim3(kThreads), 0, st>>>(a);
   count_kernel<false><<<dim3((unsigned)chunks), dim3(kThreads), 0, st>>>(page_map, num_pages, a.counts);

@@ -128,14 +128,13 @@ def _compact(ext, gpu, table, shares, free, num_free, extra=0, in_place=False):
     before = [x.clone() for x in ins]
     page_map, shares_out, left = (i32([99] * n, gpu) for n in (pages, pages, 1))
     src, dst = i32([99] * copies, gpu), i32([99] * copies, gpu)
-    table_out, free_out = (ins[0], ins[2]) if in_place else (torch.full_like(ins[0], 99), ins[2].clone())
+    table_out, free_out = ins[0] if in_place else torch.full_like(ins[0], 99), ins[2].clone()
     ws = torch.full((ext.page_workspace_ints(pages),), -12345, dtype=torch.int32, device=gpu)
     ext.compact_pages(*ins, page_map, table_out, shares_out, free_out, left, src, dst, ws)
     want = turn.compact_pages(table, shares, free, num_free, copies)
     for got, w in zip((page_map, table_out, shares_out, free_out, left, src, dst), want):
         _equal(got, w)
-    if not in_place:
-        assert all(torch.equal(a, b) for a, b in zip(ins, before))
+    assert all(torch.equal(a, b) for a, b in list(zip(ins, before))[in_place:])
 
 
 @pytest.mark.parametrize("rows,hi,page,columns,spare", [(1, 40, 16, 7, 1), (10, 700, 16, 60, 3), (64, 300, 16, 40, 30), (2, 900, 1, 900, 2), (200, 500, 8, 64, 1), (3, 0, 16, 3, 1)])
@@ -157,6 +156,49 @@ def test_compactions_of_full_empty_and_single_pools(ext, gpu):
     _compact(ext, gpu, [[0]], [4], [0], 0)
     _compact(ext, gpu, [[0]], [4], [0], 1, extra=2)
     _compact(ext, gpu, np.zeros((0, 3), dtype=np.int64), [0, 0], [1, 0], 1)
+
+
+@pytest.mark.parametrize("pages", [65535, 65536, 65537, 300001, 524288, 524289, 1100000])
+def test_large_pools(ext, gpu, pages):
+    """On both sides of the sizes where the counting moves to launches of its own."""
+    rng = np.random.default_rng(pages)
+    order = rng.permutation(pages)
+    used = pages * 2 // 5
+    shares = np.zeros(pages, dtype=np.int64)
+    shares[order[:used]] = rng.integers(0, 3, used)
+    free = np.concatenate([order[used:], np.zeros(used, dtype=np.int64)])
+    columns = used // 7
+    table = order[:7 * columns].reshape(7, columns)
+    # numpy forms of the loops
+    in_use = np.ones(pages, dtype=bool)
+    in_use[free[:pages - used]] = False
+    holes, movers = np.nonzero(~in_use[:used])[0], used + np.nonzero(in_use[used:])[0][::-1]
+    page_map = np.where(in_use, np.arange(pages), -1)
+    page_map[movers] = holes
+    moved = np.zeros(pages, dtype=np.int64)
+    moved[page_map[in_use]] = shares[in_use]
+    list_out = free.copy()
+    list_out[:pages - used] = np.arange(pages - 1, used - 1, -1)
+    pad = np.full(pages // 2 - len(holes), -1)
+    ins = [i32(x, gpu) for x in (table, shares, free, [pages - used])]
+    outs = [i32(np.zeros(n), gpu) for n in (pages, pages, 1, pages // 2, pages // 2)]
+    table_out, free_out = torch.zeros_like(ins[0]), ins[2].clone()
+    ws = torch.empty(ext.page_workspace_ints(pages), dtype=torch.int32, device=gpu)
+    ext.compact_pages(*ins, outs[0], table_out, outs[1], free_out, outs[2], outs[3], outs[4], ws)
+    for got, w in zip((outs[0], table_out, outs[1], free_out, outs[2], outs[3], outs[4]),
+                      (page_map, page_map[table], moved, list_out, [pages - used], np.concatenate([movers, pad]), np.concatenate([holes, pad]))):
+        _equal(got, w)
+    # and all rows but two freed
+    left = shares.copy()
+    np.subtract.at(left, table[:5].reshape(-1), 1)
+    gone = np.nonzero(left < 0)[0]
+    want = free.copy()
+    want[pages - used:pages - used + len(gone)] = gone
+    s, n = ins[1].clone(), i32([0], gpu)
+    ext.free_rows(i32([4, 2, 0, 1, 3], gpu), i32([columns * 16] * 7, gpu), ins[0], s, ins[2], ins[3], n, ws, 16)
+    _equal(s, np.maximum(left, 0))
+    _equal(ins[2], want)
+    assert n.item() == pages - used + len(gone)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, F8])

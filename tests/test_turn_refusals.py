@@ -35,7 +35,7 @@ def _free(**o):
 
 
 def _compact(**o):
-    a = dict(table=AT, shares=AT, free=AT, num=NUM, map=AT, to=AT, so=OUT, fo=AT, left=AT, src=AT, dst=AT, ws=AT, size=1 << 20,
+    a = dict(table=AT, shares=AT, free=AT, num=NUM, map=AT, to=AT, so=OUT, fo=OUT, left=AT, src=AT, dst=AT, ws=AT, size=1 << 20,
              batch=4, cols=3, pages=9, cap=9, copies=4)
     a.update(o)
     return pkv_native.lib().pkv_compact_pages(*a.values(), None)
@@ -76,7 +76,7 @@ def _write(**o):
     (_fork, dict(left=NUM), 1, "num_free"), (_fork, dict(pages=0), 1, "num_pages"),
     (_free, dict(n=8001), 2, "8000"), (_free, dict(cap=8), 1, "places"), (_free, dict(ws=None), 3, "workspace"), (_free, dict(size=7), 3, "workspace"),
     (_free, dict(ws=AT + 2), 3, "workspace"), (_free, dict(left=NUM), 1, "num_free"), (_free, dict(rows=None), 1, "null"), (_free, dict(batch=-1), 1, "batch"),
-    (_compact, dict(copies=3), 1, "num_pages / 2"), (_compact, dict(cap=8), 1, "places"), (_compact, dict(so=AT), 1, "page_shares_out must not be"),
+    (_compact, dict(copies=3), 1, "num_pages / 2"), (_compact, dict(cap=8), 1, "places"), (_compact, dict(so=AT), 1, "page_shares_out must not be"), (_compact, dict(fo=AT), 1, "free_pages_out must not be"),
     (_compact, dict(left=NUM), 1, "num_free_out must not be"), (_compact, dict(size=7), 3, "workspace"), (_compact, dict(map=None), 1, "null"),
     (_compact, dict(table=None), 1, "null"), (_compact, dict(pages=0), 1, "num_pages"),
     (_copy, dict(d=64), 2, "head_dim"), (_copy, dict(elem=4), 1, "1 or 2"), (_copy, dict(k=AT + 8), 1, "aligned"), (_copy, dict(dst=None), 1, "null"),

@@ -39,7 +39,7 @@ namespace {
 
 constexpr int kRows = kWaves * kWaveRows;  // of a block
 constexpr int kIds = 512;      // page ids in LDS
-constexpr int kMinTiles = 4;
+constexpr int kMinTiles = 2;
 constexpr int kSmallBatch = 64;  // rows of a table whose plan every wave makes for itself
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -644,7 +644,7 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
   const bool small = a.batch <= kSmallBatch;
   auto joins_at = [&](int b) { return small ? small_joins[b] : joins_before(a)[b]; };
   const long total = (long)joins_at(a.batch) * a.hkv;
-  const bool shared = total <= (long)gridDim.x * kJoin;  // one row a workgroup at a time
+  const bool shared = total <= 2L * gridDim.x;  // one row a workgroup at a time
   const int first = shared ? sub : 0, stride = shared ? kJoin : 1;
   for (long i = shared ? blockIdx.x : (long)blockIdx.x * kJoin + sub; i < total; i += (long)gridDim.x * (shared ? 1 : kJoin)) {
     const int join = (int)(i / a.hkv), kvh = (int)(i - (long)join * a.hkv);

@@ -215,9 +215,12 @@ int run(const char* op, RopeArgs& a, int32_t head_dim, int64_t num_pages, int32_
     if (a.stride[i] < (long)a.heads[i] * kRowBytes || a.stride[i] % 16 ||
         (i < outs && (a.out_stride[i] < (long)a.heads[i] * kRowBytes || a.out_stride[i] % 16)))
       return fail(PKV_ERR_INVALID_ARGUMENT, "%s: a token stride must hold its heads and be a multiple of 8 elements", op);
-  // Few heads in all: one or two a wave, so that none waits for another's; else eight.
-  const long rows = (long)a.tokens * (a.heads[0] + ins * (long)a.heads[1]);
-  const int each = rows <= 4096 ? 1 : 8;
+  // Heads a wave.  Few in all: one, so that none waits for another's (16 tokens of 56 heads 4.7 us for
+  // 5.2 with two, 5.7 with four); then two (4096 tokens: 20.7 us for 23.6 with one, 22.4 with four and
+  // 26 with eight); four where memory is what all wait for (53,000 tokens: 241 us for 249 with two,
+  // 328 with one, 244 with eight).
+  const long rows = (long)a.tokens * (a.heads[0] + (ins - 1) * (long)a.heads[1]);
+  const int each = rows <= 2048 ? 1 : rows <= 1 << 20 ? 2 : 4;
   long parts = 0;
   for (int i = 0; i < 3; ++i) parts += a.parts[i] = (a.heads[i] + each - 1) / each;
   const long waves = (long)((a.tokens + kTokens - 1) / kTokens) * parts, groups = (waves + 3) / 4;
@@ -244,8 +247,9 @@ int run(const char* op, RopeArgs& a, int32_t head_dim, int64_t num_pages, int32_
                              (long)a.heads[1] * kRowBytes, a.out_stride[1], a.tokens))
     return fail(PKV_ERR_INVALID_ARGUMENT, "%s: q_out and k_out must not overlap", op);
   const bool bf16 = dtype == PKV_DTYPE_BF16;
-  auto* const kernel = each == 1 ? (bf16 ? rope_kernel<true, 1> : rope_kernel<false, 1>)
-                                 : (bf16 ? rope_kernel<true, 8> : rope_kernel<false, 8>);
+  auto* const kernel = each == 1   ? (bf16 ? rope_kernel<true, 1> : rope_kernel<false, 1>)
+                       : each == 2 ? (bf16 ? rope_kernel<true, 2> : rope_kernel<false, 2>)
+                                   : (bf16 ? rope_kernel<true, 4> : rope_kernel<false, 4>);
   kernel<<<dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream>>>(a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? pkv::ok() : fail(PKV_ERR_LAUNCH, "%s launch: %s", op, hipGetErrorString(e));

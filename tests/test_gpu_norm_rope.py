@@ -63,6 +63,25 @@ def test_sizes(ext, gpu, tokens, hq, hkv, dtype):
     _check(ext, gpu, qkv, pos, w, table, hq, hkv, False, what=f"{tokens} tokens")
 
 
+@pytest.mark.parametrize("hq,hkv,dtype,weights", [(8, 2, F16, "one"), (7, 7, BF16, "each"), (5, 1, F16, "none")])
+def test_hundreds_of_thousands_of_heads(ext, gpu, hq, hkv, dtype, weights):
+    """Four heads a wave, the last ones of a part of fewer: as the same tokens in calls of few."""
+    tokens = (1 << 20) // (hq + hkv) + 37
+    gen = torch.Generator(device=gpu).manual_seed(hq)
+    qkv = torch.randn(tokens, hq + hkv, 128, generator=gen, device=gpu).to(dtype)
+    _, pos, w, table = _inputs(tokens, hq, hkv, dtype, 3, weights=weights)
+    args = [x.to(gpu) for x in w] + [table.to(gpu)]
+    q, k = qkv[:, :hq], qkv[:, hq:]
+    outs = [torch.zeros(tokens, h, 128, dtype=dtype, device=gpu) for h in (hq, hkv)]
+    pos = pos.to(gpu)
+    ext.norm_rope(q, k, *args, pos, *outs, EPS, False)
+    for first, n in ((0, 200), (tokens // 2 - 7, 3), (tokens - 4000, 4000)):
+        few = [torch.zeros(n, h, 128, dtype=dtype, device=gpu) for h in (hq, hkv)]
+        at = slice(first, first + n)
+        ext.norm_rope(q[at], k[at], *args, pos[at], *few, EPS, False)
+        assert all(torch.equal(a[at], b) for a, b in zip(outs, few))
+
+
 @pytest.mark.parametrize("rot", [16, 32, 48, 64, 80, 96, 112, 128])
 @pytest.mark.parametrize("pairs", [False, True])
 @pytest.mark.parametrize("weights,tokens", [("one", 20), ("each", 400), ("none", 400), ("each", 3)])

@@ -466,7 +466,8 @@ int pkv_norm_rope_write_kv(const void* q, int64_t q_stride, const void* k, int64
  * (the parent's page and the child's; -1, -1 where there is none) for pkv_copy_pages, once for every
  * layer's pools.  num_free_out is num_free less the pages taken; negative when that many were
  * missing: then nothing else is written but -1 to the copy lists, and the call can be repeated.
- * Lengths are the caller's: the children's are set by it.  Pairs whose rows are outside the table,
+ * Lengths are the caller's: the children's are set by it.  A child's row must hold no pages (its entries
+ * are written over, not returned).  Pairs whose rows are outside the table,
  * or the same, are skipped; a row must not be a child twice, nor a child and a parent in one call
  * (unspecified entries and counts, nothing outside the tables).  num_free counts as clamped to [0,
  * free_capacity], lengths to the table.  num_free_out must not be num_free. */
@@ -528,8 +529,8 @@ int pkv_copy_pages(const int32_t* copy_src, const int32_t* copy_dst, void* k_pag
  * page_size; G = num_q_heads / num_kv_heads in [1, 32].  Lengths count as clamped to the table, page ids
  * into the pool, offsets (which must not decrease) to [0, tokens].  Page slots past a row's length are
  * not read.  An infinity or NaN in K or V reaches the tokens that see its key, and no other.
- * (tokens * G / 128 + batch) * num_kv_heads must be below 2^24 less the number of the GPU's compute
- * units times 8.  The workspace is required: pkv_paged_prefill_workspace_bytes on the same device, for
+ * (tokens * G / 128 + batch) * num_kv_heads must be below 2^24 less four for every compute unit of
+ * the GPU and two for every KV head.  The workspace is required: pkv_paged_prefill_workspace_bytes on the same device, for
  * any lengths; it holds nothing between calls, and calls that may overlap need one each. */
 int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                                 const int32_t* block_table, const int32_t* seq_lens,

@@ -153,11 +153,12 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
   __shared__ float total[2][kPlanWaves];
   __shared__ int sums[3][kPlanWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  float tiles[2] = {0.f, 0.f};
+  double many[2] = {0., 0.};
   for (int b = tid; b < a.batch; b += kPlanThreads) {
     const Seq s = seq_of(a, b);
-    tiles[is_small(a, s)] += tiles_in(a, s);
+    many[is_small(a, s)] += (double)tiles_in(a, s);
   }
+  float tiles[2] = {(float)many[0], (float)many[1]};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     tiles[i] = wave_sum(tiles[i]);

@@ -370,7 +370,8 @@ int pkv_build_block_tables(
  * below 2^24.  An infinity or NaN in K or V reaches the tokens from its own on, and no other (a
  * key of score -inf has weight 0).  K and V of the call are all that is attended to: tokens that
  * the cache holds already are not, so a row that continues a cached prefix (cached_lens > 0 in
- * pkv_build_block_tables) must not go in for its new tokens alone. */
+ * pkv_build_block_tables) must not go in for its new tokens alone (pkv_paged_prefill_attention
+ * is for those). */
 int pkv_prefill_attention(
     const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
     int64_t v_stride, const int32_t* token_offsets, void* output, int32_t batch, int32_t tokens,

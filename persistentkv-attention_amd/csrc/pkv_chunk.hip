@@ -11,15 +11,32 @@
 // head of the group) pairs of a KV head, S^T = K Q^T and O^T += V^T P^T on 32x32x16 tiles, K/V
 // tiles of 32 keys straight to LDS in a ring of three.  What is new:
 //
-// Pages.  A tile's keys lie in any pages: every lane computes its key's place, a 64-bit address from
-// the page's id in LDS (a window of the row's table, renewed every few hundred keys), and loads 16
-// bytes of it.  Keys past the row's end read its last key again; their weights are 0.
+// Pages.  A tile's keys lie in any pages, whose ids are in LDS (a window of the row's table, renewed
+// every 512 pages).  A wave moves eight keys at a time: in pages of a multiple of 8 they lie in one
+// page, whose place is scalar arithmetic; else, and at the row's end, every lane computes its key's
+// (that for all tiles: 2048 tokens over 32768 in 1174 us instead of 1012).  Keys past the row's end
+// read its last key again; their weights are 0.
 //
-// Splits.  Rows differ in length by orders of magnitude and a call may have very few rows, so work
-// is cut by keys as well: with W tiles in all blocks of the call (as if every block saw all keys)
-// and P parts wanted, no workgroup takes more than C = max(kMinTiles, W / P) tiles.  All
-// workgroups compute C and their own part from the lengths on the GPU.  The parts of a block
-// leave their sums in the workspace, and a second kernel joins them.
+// Splits.  Rows differ in length by orders of magnitude and a call may have very few rows, so work is
+// cut by keys as well: with W tiles in all blocks of the call (as if every block saw all keys) and P
+// parts wanted, two for every compute unit, no workgroup takes more than about C = W / P tiles.  All
+// workgroups compute C and their own part from the lengths on the GPU.  The parts of a block leave
+// their sums in the workspace in 32 bits, and a second kernel joins them.  Parts cost: the states of
+// 128 rows are 66 KB each way, as much as a workgroup's 30 tiles, so more parts than the compute units
+// ask for are slower (512 tokens over 8192: 512 parts 84 us, 768 88, 256 117), but rows of one wave
+// at most (decoding rows, guessed tokens) cost little and are counted apart.  Large and small rows
+// take turns, two to one, so that the ones' products run next to the others' reads (28 single tokens
+// and 4 pieces of 512 over up to 8192: 242 us; one after the other 280, in equal turns 270).
+//
+// P is rounded to the activation type, as in the prompt attention, also where memory is the bound:
+// bf16 outputs are 2.3e-3 from the exact ones (relative 2-norm; 1.7e-3 is the output's own rounding),
+// fp16 2.7e-4 (2.1e-4).
+//
+// Measured (bf16, 32 / 8 heads, pages of 16): 2048 tokens over 32768 1.01 ms, 1.05 PFLOP/s, the matrix
+// units busy half the cycles with two workgroups a CU; the step of a workgroup, 0.48 us a CU, is the same
+// with three.  64 single tokens of 128-65536 keys (32 / 4 heads) 4.9 TB/s, the rate of a copy.  5 tokens
+// over 2011: 11.4 us, 7.8 of it the first kernel (four dependent reads before the first product), 3.7
+// the join.
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -39,7 +56,7 @@ namespace {
 
 constexpr int kRows = kWaves * kWaveRows;  // of a block
 constexpr int kIds = 512;      // page ids in LDS
-constexpr int kMinTiles = 2;
+constexpr int kMinTiles = 2;  // of a part: 5 tokens over 2011 11.5 us, with 4 12.0, with 8 14.7
 constexpr int kSmallBatch = 64;  // rows of a table whose plan every wave makes for itself
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 

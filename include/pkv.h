@@ -434,8 +434,8 @@ size_t pkv_fp8_block_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t
  * fp32 [max_positions, rotary_dim]: the cosines of the rotary_dim / 2 angles, then their sines.
  * rotary_dim is a multiple of 16 up to 128, eps (where a weight is given) in [2^-100, 2^100].
  * positions [tokens] count as clamped to the table.  An output is its own input (same pointer and
- * stride), or overlaps neither the inputs nor the other output (refused).  The same number of
- * elements from token to token as for the inputs above, for outputs too. */
+ * stride), or overlaps neither the inputs nor the other output (refused).  Strides between tokens
+ * as for the token-major inputs above, the outputs' too. */
 int pkv_norm_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
                   const float* q_weight, int32_t q_weight_heads, const float* k_weight,
                   int32_t k_weight_heads, const float* cos_sin, const int32_t* positions, void* q_out,

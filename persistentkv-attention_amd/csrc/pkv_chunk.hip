@@ -55,12 +55,12 @@ int ok();
 namespace {
 
 constexpr int kRows = kWaves * kWaveRows;  // of a block
-constexpr int kIds = 512;      // page ids in LDS
-constexpr int kMinTiles = 2;  // of a part: 5 tokens over 2011 11.5 us, with 4 12.0, with 8 14.7
-constexpr int kSmallBatch = 64;  // rows of a table whose plan every wave makes for itself
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+constexpr int kIds = 512;                  // page ids in LDS
+constexpr int kMinTiles = 2;               // of a part: 5 tokens over 2011 11.5 us, with 4 12.0, with 8 14.7
+constexpr int kSmallBatch = 64;            // rows of a table whose plan every wave makes for itself
+constexpr int kStateFloats = kD + 2;       // of one row: its sums, maximum and sum of weights
 
-constexpr int kStateFloats = kD + 2;  // of one row: its sums, maximum and sum of weights
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // x / d for 0 <= x < 2^31 as mulhi(2 x, magic) >> shift: with 2^shift the power of two at or above d and
 // magic = ceil(2^(31 + shift) / d), which is below 2^32, the error x (magic d - 2^(31 + shift)) is below
@@ -430,6 +430,7 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
       }
     }
   };
+
   u32x4 q[8];
   const uint8_t* qp = a.q + (start + (long)tok) * a.q_stride +
                       (long)(kvh * a.group + rem + r - dt * a.group) * kRowBytes + half * 16;

@@ -679,9 +679,9 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
     const int last = min((row / kRows + 1) * kRows, rows) - 1;
     const int parts = ratio_up(tiles_of(last_key(s, last / a.group) + 1), parts_of(a, s, cut).tiles);
     if (parts <= 1) continue;  // written by its only part
-    const long state = ((long)(small ? small_states[b] : states_before(a)[b]) + row) * a.hkv + kvh, next = (long)rows * a.hkv;
-    const float* const tops = a.tops + 2 * state;
-    const float* const sums = a.sums + state * kD + 4 * quad;
+    // 32 bits: 2 P times 160 states of 512 bytes, for P of two a compute unit.
+    const uint32_t next = (uint32_t)(rows * a.hkv);
+    uint32_t state = (uint32_t)(((small ? small_states[b] : states_before(a)[b]) + row) * a.hkv + kvh) + first * next;
     float m = -FLT_MAX, l = 0.f;
     f32x4 o = {};
     for (int p = first; p < parts; p += 4 * stride) {  // four parts' loads at once
@@ -691,9 +691,10 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
       for (int k = 0; k < 4; ++k) {
         top[k] = f32x2{-FLT_MAX, 0.f}, x[k] = f32x4{};
         if (p + k * stride < parts) {
-          top[k] = *(const f32x2*)(tops + 2 * (p + k * stride) * next);
-          x[k] = *(const f32x4*)(sums + (p + k * stride) * next * kD);
+          top[k] = *(const f32x2*)(a.tops + 2 * state);
+          x[k] = *(const f32x4*)(a.sums + (state * kD + 4 * quad));
         }
+        state += stride * next;
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {

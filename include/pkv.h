@@ -530,8 +530,8 @@ int pkv_copy_pages(const int32_t* copy_src, const int32_t* copy_dst, void* k_pag
  * page_size; G = num_q_heads / num_kv_heads in [1, 32].  Lengths count as clamped to the table, page ids
  * into the pool, offsets (which must not decrease) to [0, tokens].  Page slots past a row's length are
  * not read.  An infinity or NaN in K or V reaches the tokens that see its key, and no other.
- * (tokens * G / 128 + batch) * num_kv_heads must be below 2^24 less four for every compute unit of
- * the GPU and two for every KV head.  The workspace is required: pkv_paged_prefill_workspace_bytes on the same device, for
+ * (tokens * G / 128 + batch) * num_kv_heads must be below 2^24 less ten for every compute unit of
+ * the GPU and five for every KV head.  The workspace is required: pkv_paged_prefill_workspace_bytes on the same device, for
  * any lengths; it holds nothing between calls, and calls that may overlap need one each. */
 int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                                 const int32_t* block_table, const int32_t* seq_lens,

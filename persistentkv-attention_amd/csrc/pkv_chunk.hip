@@ -17,16 +17,17 @@
 // (that for all tiles: 2048 tokens over 32768 in 1174 us instead of 1012).  Keys past the row's end
 // read its last key again; their weights are 0.
 //
-// Splits.  Rows differ in length by orders of magnitude and a call may have very few rows, so work is
-// cut by keys as well: with W tiles in all blocks of the call (as if every block saw all keys) and P
-// parts wanted, two for every compute unit, no workgroup takes more than about C = W / P tiles.  All
-// workgroups compute C and their own part from the lengths on the GPU.  The parts of a block leave
-// their sums in the workspace in 32 bits, and a second kernel joins them.  Parts cost: the states of
-// 128 rows are 66 KB each way, as much as a workgroup's 30 tiles, so more parts than the compute units
-// ask for are slower (512 tokens over 8192: 512 parts 84 us, 768 88, 256 117), but rows of one wave
-// at most (decoding rows, guessed tokens) cost little and are counted apart.  Large and small rows
-// take turns, two to one, so that the ones' products run next to the others' reads (28 single tokens
-// and 4 pieces of 512 over up to 8192: 242 us; one after the other 280, in equal turns 270).
+// Splits.  Rows differ in length by orders of magnitude and a call may have very few rows, so work
+// is cut by keys as well: with W tiles in all blocks of the call (as if every block saw all keys)
+// and P parts wanted, two for every compute unit (more where parts are long, see kLongPart), no
+// workgroup takes more than about C = W / P tiles.  All workgroups compute C and their own part
+// from the lengths on the GPU.  The parts of a block leave their sums in the workspace in 32 bits,
+// and a second kernel joins them.  Parts cost: the states of 128 rows are 66 KB each way, as much
+// as a workgroup's 30 tiles, so more parts than the compute units ask for are slower (512 tokens
+// over 8192: 512 parts 84 us, 768 88, 256 117), but rows of one wave at most (decoding rows,
+// guessed tokens) cost little and are counted apart.  Large and small rows take turns, two to one,
+// so that the ones' products run next to the others' reads (28 single tokens and 4 pieces of 512
+// over up to 8192: 238 us; one after the other 280, in equal turns 270).
 //
 // P is rounded to the activation type, as in the prompt attention, also where memory is the bound:
 // bf16 outputs are 2.3e-3 from the exact ones (relative 2-norm; 1.7e-3 is the output's own rounding),
@@ -135,8 +136,14 @@ struct Cut {
 };
 // C for the sum of blocks times tiles of a class and one KV head: a little more than W / P, so that the
 // roundings of the sum (less than 2^-17 of it) never make more parts than the grid and the workspace hold.
-__device__ inline int part_tiles(const ChunkArgs& a, float tiles) {
-  return max(kMinTiles, (int)fminf(ceilf(tiles * a.heads_per_part), 1e9f));
+// Large rows whose parts would be longer than kLongPart tiles have up to kFiner times as many: the GPU
+// deals them out as it goes, and rows of different lengths end together (12 rows of 1073 tokens over up
+// to 22304, 6 / 2 heads: 518 us, 610 with P parts; 8 of 1024 over 4096-32768 2.39 ms and 2.46).
+constexpr int kLongPart = 192, kFiner = 4;
+__device__ inline int part_tiles(float c) { return max(kMinTiles, (int)fminf(ceilf(c), 1e9f)); }
+__device__ inline Cut cut_of(const ChunkArgs& a, float large, float small) {
+  const float c = large * a.heads_per_part;
+  return {part_tiles(fmaxf(c * (1.0f / kFiner), fminf(c, (float)kLongPart))), part_tiles(small * a.heads_per_part)};
 }
 __device__ inline int ratio_up(int x, int d) { return divide(x + d - 1, d); }
 // A row's parts, as even as whole tiles are: as many as keep them to C for small rows, and the nearest
@@ -187,7 +194,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkArgs a) {
   __syncthreads();
   tiles[0] = tiles[1] = 0.f;
   for (int w = 0; w < kPlanWaves; ++w) tiles[0] += total[0][w], tiles[1] += total[1][w];
-  const Cut cut{part_tiles(a, tiles[0]), part_tiles(a, tiles[1])};
+  const Cut cut = cut_of(a, tiles[0], tiles[1]);
   int before[3] = {0, 0, 0};
   int32_t* const to[3] = {units_before(a), states_before(a), joins_before(a)};
   for (int base = 0; base <= 2 * a.batch; base += kPlanThreads) {
@@ -231,7 +238,7 @@ __device__ inline LanePlan lane_plan(const ChunkArgs& a, int lane) {
   if (lane < a.batch) p.seq = seq_of(a, lane);
   p.small = is_small(a, p.seq);
   const float tiles = tiles_in(a, p.seq);
-  p.cut = {part_tiles(a, wave_sum(p.small ? 0.f : tiles)), part_tiles(a, wave_sum(p.small ? tiles : 0.f))};
+  p.cut = cut_of(a, wave_sum(p.small ? 0.f : tiles), wave_sum(p.small ? tiles : 0.f));
   p.share = share_of(a, p.seq, p.cut);
   return p;
 }
@@ -744,12 +751,19 @@ int64_t blocks_at_most(int64_t batch, int64_t tokens, int64_t group, int64_t hkv
 }
 size_t plan_bytes(int64_t batch) { return batch > kSmallBatch ? (size_t)((5 + 4 * batch) * 4 + 15) / 16 * 16 : 0; }
 
-// Rows of states, over all KV heads.  A row of the table is cut only where its tiles pass C >= W / P, so
-// that it has at most 2 tiles / C parts, and the parts of all blocks of a class are at most 2 P: of 128
-// rows each for large rows, of 32 for small ones, and of no more than the call has in either case.
+// Parts that a call can have beyond one a block, over all KV heads: none of its rows is large where
+// all its tokens are one wave's.
+int64_t parts_at_most(int64_t tokens, int64_t group) {
+  return (int64_t)parts_wanted() * (tokens * group <= kWaveRows ? 1 : 1 + kFiner);
+}
+
+// Rows of states, over all KV heads.  A row of the table is cut only where its tiles pass C, so that it
+// has at most 2 tiles / C parts, and the parts of all blocks of a class are at most 2 W / C, with C at
+// least W / P for small rows and W / (kFiner P) for large ones: of 32 and of 128 rows each, and of no
+// more than the call has.
 int64_t states_at_most(int64_t tokens, int64_t group) {
-  const int64_t all = tokens * group;
-  return 2 * (int64_t)parts_wanted() * ((all < kRows ? all : kRows) + (all < kWaveRows ? all : kWaveRows));
+  const int64_t all = tokens * group, small = all < kWaveRows ? all : kWaveRows, large = all < kRows ? all : kRows;
+  return 2 * (int64_t)parts_wanted() * (small + (all > kWaveRows ? kFiner * large : 0));
 }
 
 }  // namespace
@@ -784,9 +798,8 @@ int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_p
   const int64_t page_bytes = (int64_t)num_kv_heads * page_size * kRowBytes;
   if ((int64_t)max_pages * page_size > INT32_MAX - kKeys || page_bytes > INT32_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "%s: max_pages * page_size must be below 2^31 - 32, and a page below 2 GiB", op);
-  const int parts = parts_wanted(), classes = (int64_t)tokens * group <= kWaveRows ? 1 : 2;
   const int64_t groups = blocks_at_most(batch, tokens, group, num_kv_heads) +
-                         (int64_t)((parts + num_kv_heads - 1) / num_kv_heads) * num_kv_heads * classes;
+                         (parts_at_most(tokens, group) / num_kv_heads + 1 + kFiner) * num_kv_heads;
   if ((int64_t)tokens * group > INT32_MAX || !pkv::fits_grid(groups, kWaves * 64))
     return fail(PKV_ERR_UNSUPPORTED, "%s: too many tokens or sequences", op);
   if (batch == 0 || tokens == 0) return pkv::ok();
@@ -809,7 +822,7 @@ int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_p
                     (uint8_t*)output, (int32_t*)workspace, states, states + states_at_most(tokens, group) * kD,
                     2 * q_stride, batch, tokens, num_q_heads, num_kv_heads, group, num_pages, max_pages, page_size,
                     (uint32_t)page_bytes, divisor(page_size), divisor(group), divisor(num_kv_heads), 1.0f / (float)group,
-                    (float)num_kv_heads / (float)parts * 1.0001f};
+                    (float)num_kv_heads / (float)parts_wanted() * 1.0001f};
   const hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == PKV_DTYPE_BF16;
   if (batch > kSmallBatch) plan_kernel<<<1, kPlanThreads, 0, st>>>(a);

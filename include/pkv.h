@@ -527,7 +527,8 @@ int pkv_copy_pages(const int32_t* copy_src, const int32_t* copy_dst, void* k_pag
  * or none.  A token at a negative position (more new tokens than the row has) sees nothing: 0.
  * output [tokens, num_q_heads, 128], contiguous; rows outside every sequence are left as they are;
  * it may be a contiguous q itself, otherwise it must not overlap q (refused), nor the pools.  Any
- * page_size; G = num_q_heads / num_kv_heads in [1, 32].  Lengths count as clamped to the table, page ids
+ * page_size; G = num_q_heads / num_kv_heads in [1, 32].  Tokens past the table are not attended to
+ * (positions are those of seq_lens as given; negative lengths count as 0), page ids count as clamped
  * into the pool, offsets (which must not decrease) to [0, tokens].  Page slots past a row's length are
  * not read.  An infinity or NaN in K or V reaches the tokens that see its key, and no other.
  * (tokens * G / 128 + batch) * num_kv_heads must be below 2^24 less ten for every compute unit of

@@ -32,7 +32,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kChunk = 1024;     // pages that a workgroup counts and ranks
-constexpr int kMaxPairs = 8000;  // rows of a table, and rows that one call forks or frees
+constexpr int kMaxPairs = 8000;  // rows that one call forks or frees
+constexpr int kMaxColumns = 1 << 30;  // of a table: column numbers plus a workgroup's stay in 32 bits
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -457,8 +458,9 @@ int pkv_fork_rows(const int32_t* parents, const int32_t* children, const int32_t
                 "fork_rows: num_forks %d, batch %d, max_pages %d, num_pages %d, free_capacity %d, page_size %d",
                 num_forks, batch, max_pages, num_pages, free_capacity, page_size);
   if (num_forks > kMaxPairs) return fail(PKV_ERR_UNSUPPORTED, "fork_rows: %d forks (at most %d)", num_forks, kMaxPairs);
-  if ((int64_t)max_pages * page_size > INT32_MAX)
-    return fail(PKV_ERR_UNSUPPORTED, "fork_rows: max_pages * page_size does not fit in int32");
+  if ((int64_t)max_pages * page_size > INT32_MAX || max_pages > kMaxColumns)
+    return fail(PKV_ERR_UNSUPPORTED, "fork_rows: max_pages * page_size does not fit in int32, or max_pages %d past %d",
+                max_pages, kMaxColumns);
   if (!num_free || !num_free_out || (free_capacity > 0 && !free_pages) ||
       (num_forks > 0 && (!parents || !children || !lens || !block_table || !page_shares || !copy_src || !copy_dst)))
     return fail(PKV_ERR_INVALID_ARGUMENT, "fork_rows: null pointer");
@@ -482,6 +484,8 @@ int pkv_free_rows(const int32_t* rows, const int32_t* lens, const int32_t* block
                 "free_rows: num_rows %d, batch %d, max_pages %d, num_pages %d, free_capacity %d, page_size %d",
                 num_rows, batch, max_pages, num_pages, free_capacity, page_size);
   if (num_rows > kMaxPairs) return fail(PKV_ERR_UNSUPPORTED, "free_rows: %d rows (at most %d)", num_rows, kMaxPairs);
+  if (max_pages > kMaxColumns)
+    return fail(PKV_ERR_UNSUPPORTED, "free_rows: max_pages %d (at most %d)", max_pages, kMaxColumns);
   if (free_capacity < num_pages)
     return fail(PKV_ERR_INVALID_ARGUMENT, "free_rows: a list of %d places for %d pages", free_capacity, num_pages);
   if (!page_shares || !free_pages || !num_free || !num_free_out ||

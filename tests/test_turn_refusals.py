@@ -74,6 +74,7 @@ def _write(**o):
     (_fork, dict(n=-1), 1, "num_forks"), (_fork, dict(ps=0), 1, "page_size"), (_fork, dict(cols=0), 1, "max_pages"), (_fork, dict(n=8001), 2, "8000"),
     (_fork, dict(cols=1 << 28, ps=16), 2, "int32"), (_fork, dict(parents=None), 1, "null"), (_fork, dict(free=None), 1, "null"),
     (_fork, dict(left=NUM), 1, "num_free"), (_fork, dict(pages=0), 1, "num_pages"),
+    (_fork, dict(cols=(1 << 30) + 1, ps=1), 2, "past 1073741824"), (_free, dict(cols=(1 << 30) + 1), 2, "at most 1073741824"),
     (_free, dict(n=8001), 2, "8000"), (_free, dict(cap=8), 1, "places"), (_free, dict(ws=None), 3, "workspace"), (_free, dict(size=7), 3, "workspace"),
     (_free, dict(ws=AT + 2), 3, "workspace"), (_free, dict(left=NUM), 1, "num_free"), (_free, dict(rows=None), 1, "null"), (_free, dict(batch=-1), 1, "batch"),
     (_compact, dict(copies=3), 1, "num_pages / 2"), (_compact, dict(cap=8), 1, "places"), (_compact, dict(so=AT), 1, "page_shares_out must not be"), (_compact, dict(fo=AT), 1, "free_pages_out must not be"),

@@ -466,7 +466,8 @@ int pkv_norm_rope_write_kv(const void* q, int64_t q_stride, const void* k, int64
  * num_free) in the order of i, entered in its table row, and named in copy_src[i], copy_dst[i]
  * (the parent's page and the child's; -1, -1 where there is none) for pkv_copy_pages, once for every
  * layer's pools.  num_free_out is num_free less the pages taken; negative when that many were
- * missing: then nothing else is written but -1 to the copy lists, and the call can be repeated.
+ * missing: then nothing else is written but -1 to the copy lists, and the call can be repeated.  Such
+ * a count must not become num_free, which is still the list's, nor may the children get lengths.
  * Lengths are the caller's: the children's are set by it.  A child's row must hold no pages (its entries
  * are written over, not returned).  Pairs whose rows are outside the table,
  * or the same, are skipped; a row must not be a child twice, nor a child and a parent in one call

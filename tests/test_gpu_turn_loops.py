@@ -1,0 +1,75 @@
+"""The loops around the page operators over the kernels; a captured fork that is taken or not on the GPU."""
+import pytest
+import torch
+
+from turn_cases import i32
+from turn_loops import refused_fork_and_retry
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def ops(ext, gpu):
+    def fork(parents, children, lens, table, shares, free, num_free, page):
+        t, s, left, src, dst = i32(table, gpu), i32(shares, gpu), i32([99], gpu), i32([9] * len(parents), gpu), i32([9] * len(parents), gpu)
+        ext.fork_rows(i32(parents, gpu), i32(children, gpu), i32(lens, gpu), t, s, i32(free, gpu), i32([num_free], gpu), left, src, dst, page)
+        return t.tolist(), s.tolist(), left.item(), src.tolist(), dst.tolist()
+
+    def release(rows, lens, table, shares, free, num_free, page):
+        s, f, left = i32(shares, gpu), i32(free, gpu), i32([99], gpu)
+        space = torch.empty(ext.page_workspace_ints(len(shares)), dtype=torch.int32, device=gpu)
+        ext.free_rows(i32(rows, gpu), i32(lens, gpu), i32(table, gpu), s, f, i32([num_free], gpu), left, space, page)
+        return s.tolist(), f.tolist(), left.item()
+
+    return fork, release
+
+
+def test_a_refused_fork_is_not_taken(ops):
+    refused_fork_and_retry(*ops)
+
+
+def test_a_captured_fork_takes_its_count_on_the_gpu(ext, gpu):
+    """The count and the children's lengths by torch.where on the GPU: replays with too few pages
+    leave the state as it was, those with enough go through."""
+    page, pages = 16, 12
+    table = i32([[0, 1, 2], [3, 4, 5], [-1] * 3, [-1] * 3], gpu)
+    lens, shares, free = i32([40, 33, 0, 0], gpu), i32([0] * pages, gpu), i32(list(range(11, -1, -1)), gpu)
+    num, left, src, dst = i32([1], gpu), i32([0], gpu), i32([0, 0], gpu), i32([0, 0], gpu)
+    parents, children = i32([0, 1], gpu), i32([2, 3], gpu)
+    pools = [torch.randn(pages, 1, page, 128, device=gpu).half() for _ in range(2)]
+
+    def step():
+        ext.fork_rows(parents, children, lens, table, shares, free, num, left, src, dst, page)
+        ext.copy_pages(src, dst, *pools)
+        fits = left >= 0
+        num.copy_(torch.where(fits, left, num))
+        lens[children.long()] = torch.where(fits, lens[parents.long()], lens[children.long()])
+
+    held = [x.clone() for x in (table, lens, shares, num, *pools)]
+
+    def restore(free_pages):
+        for x, y in zip((table, lens, shares, num, *pools), held):
+            x.copy_(y)
+        num.fill_(free_pages)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for have in (1, 2, 0, 6, 1):
+        restore(have)
+        graph.replay()
+        torch.cuda.synchronize()
+        if have < 2:
+            assert num.item() == have and lens.tolist() == [40, 33, 0, 0] and torch.equal(table, held[0]) and not shares.any()
+            assert all(torch.equal(x, y) for x, y in zip(pools, held[4:]))
+            continue
+        taken = free.tolist()[have - 2:have][::-1]
+        assert num.item() == have - 2 and lens.tolist() == [40, 33, 40, 33]
+        assert table.tolist()[2:] == [[0, 1, taken[0]], [3, 4, taken[1]]] and shares.tolist() == [1, 1, 0, 1, 1] + [0] * 7
+        for x, y in zip(pools, held[4:]):
+            assert torch.equal(x[taken], y[[2, 5]])

@@ -353,7 +353,8 @@ int pkv_workqueue_decode_fp8(
  * and num_free as they were, and pages returned to the list or rows left out (seq_lens =
  * cached_lens), the same call builds it again.
  * num_free [1] counts as clamped to [0, free_capacity].  At most 8000 rows, and 2^31 - 1 new
- * tokens.  Returning pages is the caller's: entries copied to the end of free_pages. */
+ * tokens.  Pages are returned by pkv_free_rows, or where no row was ever forked by the caller, who
+ * copies entries to the end of free_pages; a page that other rows hold must not go there. */
 int pkv_build_block_tables(
     const int32_t* cached_lens, const int32_t* seq_lens, const int32_t* free_pages,
     const int32_t* num_free, int32_t* block_table, int32_t* token_offsets, int32_t* slot_mapping,

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from turn_cases import i32
-from turn_loops import refused_fork_and_retry
+from turn_loops import pages_back_beside_forked_rows, refused_fork_and_retry
 
 pytestmark = pytest.mark.gpu
 
@@ -26,6 +26,10 @@ def ops(ext, gpu):
 
 def test_a_refused_fork_is_not_taken(ops):
     refused_fork_and_retry(*ops)
+
+
+def test_pages_that_other_rows_hold_stay_off_the_list(ops):
+    pages_back_beside_forked_rows(*ops)
 
 
 def test_a_captured_fork_takes_its_count_on_the_gpu(ext, gpu):

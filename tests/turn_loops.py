@@ -69,3 +69,24 @@ def refused_fork_and_retry(fork, free, took=lambda left: left >= 0):
     s.release([0, 1, 4, 5, 6])
     s.add_up()
     assert s.num == 12
+
+
+def pages_back_beside_forked_rows(fork, free, by_hand=lambda s, row: False):
+    """Rows that end beside rows forked from them: their shared pages stay off the list.  `by_hand` may
+    return a row's pages itself, where it says so."""
+    s = Pages(fork, free, rows=6, columns=4, pages=16, page=16)
+    s.grow(0, 40), s.grow(1, 32)
+    s.fork([0, 1], [2, 3], took=lambda left: True)
+    s.lens[2], s.lens[3] = 40, 32
+    s.add_up()
+    for row in (0, 3, 1):
+        if by_hand(s, row):
+            s.lens[row] = 0
+        else:
+            s.release([row])
+        s.add_up()
+    s.grow(4, 60)  # takes none of row 2's pages
+    s.add_up()
+    s.release([2, 4])
+    s.add_up()
+    assert s.num == 16

@@ -337,8 +337,9 @@ int pkv_workqueue_decode_fp8(
  * ------------------------------------------------------------------------------- */
 
 /* The metadata of one step, from lengths on the GPU.  Row b holds cached_lens[b] tokens, and
- * seq_lens[b] after the step (a row that shrinks takes no tokens and keeps its pages;
- * negative lengths count as 0):
+ * seq_lens[b] after the step (a row that shrinks takes no tokens and keeps its pages until
+ * cached_lens goes down too: those behind it are then the caller's to return; negative lengths
+ * count as 0):
  *   token_offsets [batch + 1]  where row b's new tokens start in packed order, and their count
  *   block_table   [batch, max_pages]  the pages that row b needs beyond the
  *                 ceil(cached / page_size) it has are entered, taken in row order from the

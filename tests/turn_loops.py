@@ -90,3 +90,30 @@ def pages_back_beside_forked_rows(fork, free, by_hand=lambda s, row: False):
     s.release([2, 4])
     s.add_up()
     assert s.num == 16
+
+
+def rows_that_get_shorter(fork, free, give_back=True):
+    """Guessed tokens that are not taken: the pages behind the tokens that a row keeps go back to the
+    list, through the operator that frees rows, as the pages of a table of their own."""
+    s = Pages(fork, free, rows=6, columns=6, pages=24, page=8)
+    for row, n in enumerate((20, 8, 0, 17)):
+        s.grow(row, n)
+    s.fork([0, 1], [4, 5], took=lambda left: True)
+    s.lens[4], s.lens[5] = 20, 8
+    s.add_up()
+    for grown, kept in (((37, 9, 16, 18, 24, 33), (24, 8, 1, 18, 21, 30)),   # across page borders, within pages, all of them
+                        ((40, 8, 1, 25, 25, 31), (24, 8, 0, 17, 21, 30)),
+                        ((24, 8, 0, 17, 21, 30), (8, 0, 0, 17, 21, 30))):    # into pages that other rows share
+        for row, n in enumerate(grown):
+            s.grow(row, n)
+        s.add_up()
+        first = [s.pages_of(n) for n in kept]
+        behind = [[row[min(f + c, len(row) - 1)] for c in range(len(row))] for row, f in zip(s.table, first)]
+        more = [(s.pages_of(n) - f) * s.page for n, f in zip(s.lens, first)]
+        if give_back:
+            s.shares, s.free, s.num = s.free_op(list(range(6)), more, behind, s.shares, s.free, s.num, s.page)
+        s.lens = list(kept)
+        s.add_up()
+    s.release(list(range(6)))
+    s.add_up()
+    assert s.num == 24

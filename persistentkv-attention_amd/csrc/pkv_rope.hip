@@ -225,8 +225,8 @@ int run(const char* op, RopeArgs& a, int32_t head_dim, int64_t num_pages, int32_
   const long rows = (long)a.tokens * (a.heads[0] + (ins - 1) * (long)a.heads[1]);
   const int each = rows <= 2048 ? 1 : rows <= 1 << 20 ? 2 : 4;
   long parts = 0;
-  for (int i = 0; i < 3; ++i) parts += a.parts[i] = (a.heads[i] + each - 1) / each;
-  const long waves = (long)((a.tokens + kTokens - 1) / kTokens) * parts, groups = (waves + 3) / 4;
+  for (int i = 0; i < 3; ++i) parts += a.parts[i] = (int32_t)(((long)a.heads[i] + each - 1) / each);
+  const long waves = ((long)a.tokens + kTokens - 1) / kTokens * parts, groups = (waves + 3) / 4;
   if (!pkv::fits_grid(groups, 256) || parts > INT32_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "%s: too many tokens or heads", op);
   if (a.tokens == 0) return pkv::ok();

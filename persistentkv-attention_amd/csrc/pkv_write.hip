@@ -335,7 +335,7 @@ int pkv_write_kv_fp8_block(const void* k_new, int64_t k_stride, const void* v_ne
   // window and three of four hold no start, and one without still costs 2 us of a CU's place.
   const bool bf16 = dtype == PKV_DTYPE_BF16, shared = page_size > 64;
   const int window = (long)tokens * num_kv_heads <= 4096 ? 1 : page_size > 16 ? 32 : 16;
-  const long units = (long)((tokens + window - 1) / window) * num_kv_heads * 2;
+  const long units = ((long)tokens + window - 1) / window * num_kv_heads * 2;
   const long groups = shared ? units : (units + 3) / 4;
   if (!pkv::fits_grid(groups, 256))
     return pkv::fail(PKV_ERR_UNSUPPORTED, "write_kv_fp8_block: tokens * num_kv_heads too large (below 2^28)");

@@ -2,6 +2,7 @@
 import pytest
 
 import pkv_native
+from test_prompt_refusals import _write as _write_kv
 from test_turn_refusals import _rope, _write
 
 MOST = 2 ** 31 - 1
@@ -20,3 +21,11 @@ def test_tokens_and_heads_of_norm_rope(call, overrides):
         overrides = {k: v for k, v in overrides.items() if k != "vs"}
     assert call(**overrides) == 2
     assert "too many tokens or heads" in pkv_native.last_error()
+
+
+@pytest.mark.parametrize("tokens", [MOST, MOST - 14, MOST - 40])
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("heads", [1, 2])
+def test_tokens_of_block_scaled_writes(tokens, page, heads):
+    assert _write_kv(block=True, tokens=tokens, hkv=heads, ps=page) == 2
+    assert "too large" in pkv_native.last_error()

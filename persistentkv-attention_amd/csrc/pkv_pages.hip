@@ -243,6 +243,8 @@ struct CompactArgs {
 // share of the table's entries and of the pages without a word from the others.
 constexpr int kBitPages = 1 << 19;  // 16384 words, twice: 128 of the 160 KB
 constexpr int kBitThreads = 1024;
+// The kernel's LDS, all of it in the launch's size, by which the host asks for more than 64 KB.
+constexpr size_t bit_bytes(int words) { return (2 * (size_t)words + kBitThreads / 64) * sizeof(int); }
 struct PageBits {
   const uint32_t* used;
   const int* before;
@@ -264,10 +266,10 @@ struct PageBits {
   }
 };
 __global__ __launch_bounds__(kBitThreads) void compact_kernel(CompactArgs a) {
-  extern __shared__ uint32_t bits[];  // [words], then the counts [words]
-  __shared__ int lds[kBitThreads / 64];
+  extern __shared__ uint32_t bits[];  // [words], then the counts [words], then the scan's [waves]
   const int tid = threadIdx.x, words = (a.num_pages + 31) / 32;
   int* const counts = (int*)bits + words;
+  int* const lds = counts + words;
   for (int w = tid; w < words; w += kBitThreads) bits[w] = 0xffffffffu;
   __syncthreads();
   if (tid == 0 && (a.num_pages & 31)) bits[words - 1] = (1u << (a.num_pages & 31)) - 1;
@@ -543,7 +545,7 @@ int pkv_compact_pages(const int32_t* block_table, const int32_t* page_shares, co
   auto groups = [](int64_t n) { return dim3((unsigned)((n + kThreads - 1) / kThreads)); };
   if (num_pages <= kBitPages) {
     const int64_t share = 2L * kBitThreads, wanted = (entries + num_pages + share - 1) / share, units = pkv::compute_units();
-    const size_t lds = (size_t)(num_pages + 31) / 32 * 8;
+    const size_t lds = bit_bytes((num_pages + 31) / 32);
     if (lds > 64 * 1024) {
       const hipError_t e = hipFuncSetAttribute((const void*)compact_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
       if (e != hipSuccess) return fail(PKV_ERR_LAUNCH, "compact_pages: %s", hipGetErrorString(e));

@@ -460,7 +460,8 @@ int pkv_norm_rope_write_kv(const void* q, int64_t q_stride, const void* k, int64
 
 /* Pages that several rows hold.  page_shares [num_pages] counts the holders of a page beyond the
  * first: 0 for a page that one row holds and for a free one, so pages that pkv_build_block_tables
- * hands out need nothing done.  All zero at the start; only these three operators write it.
+ * hands out need nothing done.  All zero at the start; only these three operators write it.  What one
+ * of the three writes, its workspace among it, must not overlap another tensor of its call (refused).
  *
  * Forks: row children[i] of the table becomes a copy of row parents[i], for i < num_forks (at most
  * 8000).  Of the parent's lens[parent] tokens, full pages are shared (entries copied, page_shares one
@@ -499,7 +500,7 @@ int pkv_free_rows(const int32_t* rows, const int32_t* lens, const int32_t* block
  * used page of the highest id goes to the lowest free id, and so on:
  *   page_map [num_pages]        every used page's new id; -1 for free ones
  *   block_table_out             the table [batch, max_pages] with its ids mapped (free pages' as -1;
- *                               entries that are no ids stay); it may be block_table itself
+ *                               entries that are no ids stay); it alone may be its input, block_table itself
  *   page_shares_out             the counts at the new ids, 0 behind; not page_shares itself
  *   free_pages_out              num_pages - 1 down to U, so that the lowest is taken first (it and
  *                               free_pages have free_capacity >= num_pages places; not free_pages itself)

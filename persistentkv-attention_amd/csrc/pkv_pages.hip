@@ -432,6 +432,24 @@ int launched(const char* op) {
   return e == hipSuccess ? pkv::ok() : pkv::fail(PKV_ERR_LAUNCH, "%s launch: %s", op, hipGetErrorString(e));
 }
 
+// A call's tensors: those that it writes first, then those that it only reads.  One that is written must
+// have no byte in common with another, which would be read or written while it changes.
+struct Span {
+  const char* name;
+  const void* at;
+  int64_t bytes;
+};
+template <int N>
+int refuse_overlaps(const char* op, const Span (&spans)[N], int written) {
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < N; ++j)
+      if (spans[i].bytes > 0 && spans[j].bytes > 0 && (uintptr_t)spans[i].at < (uintptr_t)spans[j].at + spans[j].bytes &&
+          (uintptr_t)spans[j].at < (uintptr_t)spans[i].at + spans[i].bytes)
+        return pkv::fail(PKV_ERR_INVALID_ARGUMENT, "%s: %s must not overlap %s", op, spans[i].name, spans[j].name);
+  return PKV_OK;
+}
+int64_t ints(int64_t n) { return n * (int64_t)sizeof(int32_t); }
+
 // Columns that one workgroup takes, so that about four workgroups a CU share `n` rows of them out.
 int columns_of(int n, int max_pages) {
   const long groups = 4L * pkv::compute_units() / n;
@@ -468,6 +486,13 @@ int pkv_fork_rows(const int32_t* parents, const int32_t* children, const int32_t
     return fail(PKV_ERR_INVALID_ARGUMENT, "fork_rows: null pointer");
   if (num_free == num_free_out)
     return fail(PKV_ERR_INVALID_ARGUMENT, "fork_rows: num_free_out must not be num_free");
+  const int64_t listed = ints(num_forks), one = ints(1);
+  const Span spans[] = {{"num_free_out", num_free_out, one}, {"copy_src", copy_src, listed}, {"copy_dst", copy_dst, listed},
+                        {"block_table", block_table, listed ? ints((int64_t)batch * max_pages) : 0},
+                        {"page_shares", page_shares, listed ? ints(num_pages) : 0}, {"parents", parents, listed},
+                        {"children", children, listed}, {"lens", lens, listed ? ints(batch) : 0},
+                        {"free_pages", free_pages, ints(free_capacity)}, {"num_free", num_free, one}};
+  if (const int status = refuse_overlaps("fork_rows", spans, 5)) return status;
   const int n = num_forks > 0 ? num_forks : 1, columns = columns_of(n, max_pages);
   const ForkArgs a{parents, children, lens, block_table, page_shares, free_pages, num_free, num_free_out,
                    copy_src, copy_dst, num_forks, batch, max_pages, num_pages, free_capacity, page_size, columns};
@@ -498,6 +523,12 @@ int pkv_free_rows(const int32_t* rows, const int32_t* lens, const int32_t* block
   if (!workspace || workspace_size < pkv_page_workspace_bytes(num_pages) || ((uintptr_t)workspace & 3))
     return fail(PKV_ERR_WORKSPACE_TOO_SMALL, "free_rows: workspace of %zu bytes is smaller than %zu, or misaligned",
                 workspace_size, pkv_page_workspace_bytes(num_pages));
+  const int64_t listed = ints(num_rows), one = ints(1);
+  const Span spans[] = {{"workspace", workspace, (int64_t)pkv_page_workspace_bytes(num_pages)}, {"num_free_out", num_free_out, one},
+                        {"page_shares", page_shares, ints(num_pages)}, {"free_pages", free_pages, ints(free_capacity)},
+                        {"rows", rows, listed}, {"lens", lens, listed ? ints(batch) : 0},
+                        {"block_table", block_table, listed ? ints((int64_t)batch * max_pages) : 0}, {"num_free", num_free, one}};
+  if (const int status = refuse_overlaps("free_rows", spans, 4)) return status;
   const int chunks = chunks_of(num_pages), columns = num_rows > 0 ? columns_of(num_rows, max_pages) : max_pages;
   const FreeArgs a{rows, lens, block_table, page_shares, free_pages, num_free, num_free_out, (int32_t*)workspace,
                    num_rows, batch, max_pages, num_pages, free_capacity, page_size, columns};
@@ -537,6 +568,14 @@ int pkv_compact_pages(const int32_t* block_table, const int32_t* page_shares, co
   if (!workspace || workspace_size < pkv_page_workspace_bytes(num_pages) || ((uintptr_t)workspace & 3))
     return fail(PKV_ERR_WORKSPACE_TOO_SMALL, "compact_pages: workspace of %zu bytes is smaller than %zu, or misaligned",
                 workspace_size, pkv_page_workspace_bytes(num_pages));
+  const int64_t table = ints(entries), pages = ints(num_pages), list = ints(free_capacity), moves = ints(num_copies), one = ints(1);
+  const Span spans[] = {{"workspace", workspace, (int64_t)pkv_page_workspace_bytes(num_pages)}, {"page_map", page_map, pages},
+                        {"page_shares_out", page_shares_out, pages}, {"free_pages_out", free_pages_out, list},
+                        {"num_free_out", num_free_out, one}, {"copy_src", copy_src, moves}, {"copy_dst", copy_dst, moves},
+                        {"block_table_out", block_table_out, table}, {"page_shares", page_shares, pages},
+                        {"free_pages", free_pages, list}, {"num_free", num_free, one},
+                        {"block_table", block_table, block_table_out == block_table ? 0 : table}};
+  if (const int status = refuse_overlaps("compact_pages", spans, 8)) return status;
   const int chunks = chunks_of(num_pages);
   const CompactArgs a{block_table, page_shares, free_pages, num_free, page_map, block_table_out, page_shares_out,
                       free_pages_out, num_free_out, copy_src, copy_dst, (int32_t*)workspace, entries, num_pages,

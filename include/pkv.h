@@ -536,8 +536,9 @@ int pkv_copy_pages(const int32_t* copy_src, const int32_t* copy_dst, void* k_pag
  * into the pool, offsets (which must not decrease) to [0, tokens].  Page slots past a row's length are
  * not read.  An infinity or NaN in K or V reaches the tokens that see its key, and no other.
  * (tokens * G / 128 + batch) * num_kv_heads must be below 2^24 less ten for every compute unit of
- * the GPU and five for every KV head.  The workspace is required: pkv_paged_prefill_workspace_bytes on the same device, for
- * any lengths; it holds nothing between calls, and calls that may overlap need one each. */
+ * the GPU and five for every KV head.  The workspace is required: pkv_paged_prefill_workspace_bytes on the
+ * same device, for any lengths (with 256 compute units up to 199 MB, from tokens * G = 128 on, and 17 MB
+ * up to tokens * G = 32); it holds nothing between calls, and calls that may overlap need one each. */
 int pkv_paged_prefill_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                                 const int32_t* block_table, const int32_t* seq_lens,
                                 const int32_t* token_offsets, void* output, void* workspace,

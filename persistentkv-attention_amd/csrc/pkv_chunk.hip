@@ -19,9 +19,10 @@
 //
 // Splits.  Rows differ in length by orders of magnitude and a call may have very few rows, so work
 // is cut by keys as well: with W tiles in all blocks of the call (as if every block saw all keys)
-// and P parts wanted, two for every compute unit (more where parts are long, see kLongPart), no
-// workgroup takes more than about C = W / P tiles.  All workgroups compute C and their own part
-// from the lengths on the GPU.  The parts of a block leave their sums in the workspace in 32 bits,
+// and P parts wanted, two for every compute unit (more where parts are long, see kLongPart), a
+// workgroup takes at most C = W / P tiles of a small row and, since large rows are cut into the
+// nearest number of parts, less than 1.5 C of a large one.  All workgroups compute C and their own
+// part from the lengths on the GPU.  The parts of a block leave their sums in the workspace in 32 bits,
 // and a second kernel joins them.  Parts cost: the states of 128 rows are 66 KB each way, as much
 // as a workgroup's 30 tiles, so more parts than the compute units ask for are slower (512 tokens
 // over 8192: 512 parts 84 us, 768 88, 256 117), but rows of one wave at most (decoding rows,
@@ -686,7 +687,7 @@ __global__ __launch_bounds__(32 * kJoin) void join_kernel(ChunkArgs a) {
     const int last = min((row / kRows + 1) * kRows, rows) - 1;
     const int parts = ratio_up(tiles_of(last_key(s, last / a.group) + 1), parts_of(a, s, cut).tiles);
     if (parts <= 1) continue;  // written by its only part
-    // 32 bits: 2 P times 160 states of 512 bytes, for P of two a compute unit.
+    // 32 bits: states_at_most() times 128 floats.
     const uint32_t next = (uint32_t)(rows * a.hkv);
     uint32_t state = (uint32_t)(((small ? small_states[b] : states_before(a)[b]) + row) * a.hkv + kvh) + first * next;
     float m = -FLT_MAX, l = 0.f;
@@ -757,14 +758,20 @@ int64_t parts_at_most(int64_t tokens, int64_t group) {
   return (int64_t)parts_wanted() * (tokens * group <= kWaveRows ? 1 : 1 + kFiner);
 }
 
-// Rows of states, over all KV heads.  A row of the table is cut only where its tiles pass C, so that it
-// has at most 2 tiles / C parts, and the parts of all blocks of a class are at most 2 W / C, with C at
-// least W / P for small rows and W / (kFiner P) for large ones: of 32 and of 128 rows each, and of no
-// more than the call has.
+// Rows of states, over all KV heads.  A small row is cut only where its tiles pass C, into less than
+// tiles / C + 1 parts, which is at most 2 tiles / C; a large one where they reach 1.5 C, into at most
+// tiles / C + 1/2, which is at most 4/3 tiles / C.  So the parts of all blocks of a class are at most
+// 2 W / C and 4/3 W / C, with C at least W / P and W / (kFiner P): of 32 and of 128 rows each, and of
+// no more than the call has.  With 256 compute units that is 199 MB for calls of 128 rows and more
+// and 17 MB for those of at most 32.
 int64_t states_at_most(int64_t tokens, int64_t group) {
   const int64_t all = tokens * group, small = all < kWaveRows ? all : kWaveRows, large = all < kRows ? all : kRows;
-  return 2 * (int64_t)parts_wanted() * (small + (all > kWaveRows ? kFiner * large : 0));
+  const int64_t parts = parts_wanted();
+  return 2 * parts * small + (all > kWaveRows ? (4 * kFiner * parts * large + 2) / 3 : 0);
 }
+// The joins address their floats in 32 bits.
+constexpr int64_t kMostUnits = 1024;  // compute units of any one GPU
+static_assert(2 * kMostUnits * (2 * kWaveRows + (4 * kFiner * kRows + 2) / 3) * kStateFloats <= UINT32_MAX);
 
 }  // namespace
 

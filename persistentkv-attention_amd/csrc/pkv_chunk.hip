@@ -30,9 +30,12 @@
 // so that the ones' products run next to the others' reads (28 single tokens and 4 pieces of 512
 // over up to 8192: 238 us; one after the other 280, in equal turns 270).
 //
-// P is rounded to the activation type, as in the prompt attention, also where memory is the bound:
-// bf16 outputs are 2.3e-3 from the exact ones (relative 2-norm; 1.7e-3 is the output's own rounding),
-// fp16 2.7e-4 (2.1e-4).
+// P enters the product with V in the activation type.  Large rows, which wait for products, round it
+// once, as the prompt attention does: bf16 outputs are 2.3e-3 from the exact ones (relative 2-norm;
+// 1.7e-3 is the output's own rounding), fp16 2.7e-4 (2.1e-4).  Rows of one wave, which wait for memory,
+// give bf16 P in two terms, as the decode kernels do, and are as exact as the output's rounding (1.66e-3
+// of 1.66e-3) for 3 % (64 single tokens of 128-65536 keys, 32 / 4 heads: 331 us, 323 with one term; the
+// 28 single tokens next to four pieces of 512: 249 for 239).
 //
 // Measured (bf16, 32 / 8 heads, pages of 16): 2048 tokens over 32768 1.01 ms, 1.05 PFLOP/s, the matrix
 // units busy half the cycles with two workgroups a CU; the step of a workgroup, 0.48 us a CU, is the same
@@ -44,6 +47,7 @@
 #include <float.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "pkv.h"
 #include "pkv_attention_tile.h"
@@ -366,6 +370,8 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   const int start = uniform(u.seq.start), n = uniform(u.seq.n), len = uniform(u.seq.len);
   const Seq seq{start, n, uniform(u.seq.before), len};
   const int block = uniform(u.block), rows = n * a.group;
+  // bf16 weights of rows that are one wave's: rounded, and the rest rounded again.
+  const bool two_terms = std::is_same_v<Elem, BFloat> && rows <= kWaveRows;
 
   // Row row0 + r of the wave is token tok0 + (rem + r) / G: a quotient of numbers below 64, which
   // the product with 1 / G in 32 bits gives exactly (it is off by less than 1 / (2 G)).
@@ -465,7 +471,8 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
   // A masked weight is 0, and 0 times an infinity or NaN in V is NaN.  So where a row comes out
   // not finite, its workgroup computes once more, `careful`: such values are taken out of the tiles
   // that a row of it masks in part, those of the steps from `masked` on (the keys read twice past
-  // the end among them), and put back at the end for the rows that see their token.
+  // the end among them), and put back at the end for the rows that see their token.  A second term,
+  // which may be 0 or negative, never meets them.
   bool careful = false;
   const int masked = max((last_key(seq, quotient(block * kRows, a.by_group)) + 1) / kKeys - tile0, 0);
   auto clean = [&](int buf) {
@@ -479,8 +486,10 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
     __syncthreads();
   };
 
-  // The i-th tile, which lies in buffer `buf`.
-  auto step = [&](int i, int buf) __attribute__((always_inline)) {
+  // The i-th tile, which lies in buffer `buf`, with the weights in `two` terms or in one.  The sum of the
+  // weights is that of the rounded ones, or, for two terms, of the weights themselves.  Each has a loop
+  // of its own: a branch between the exponentials and the products costs the large rows 3-9 %.
+  auto step = [&](auto two, int i, int buf) __attribute__((always_inline)) {
     const int at = buf * 2 * kTileBytes;
     if (careful && i >= masked) clean(buf);
     if (i + 2 < tiles && tile0 + i + 2 >= id_end) {
@@ -536,19 +545,44 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
       u32x4 p[2];
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const uint32_t x = Elem::pack2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kScaleLog2, -ms)),
-                                       __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], kScaleLog2, -ms)));
+        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kScaleLog2, -ms));
+        s[i + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], kScaleLog2, -ms));
+        const uint32_t x = Elem::pack2(s[i], s[i + 1]);
         p[i >> 3][(i & 7) >> 1] = x;
-        l = Elem::sum2(x, l);
+        l = two.value ? l + (s[i] + s[i + 1]) : Elem::sum2(x, l);
       }
-      u32x4 v1[4];
+      if constexpr (two.value) {
+        u32x4 rest[2];
 #pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        v1[db] = value(1, db);
-        o[db] = Elem::mma(v0[db], p[0], o[db]);
+        for (int i = 0; i < 16; i += 2) {
+          const uint32_t x = p[i >> 3][(i & 7) >> 1];
+          rest[i >> 3][(i & 7) >> 1] = Elem::pack2(s[i] - Elem::widen(x, false), s[i + 1] - Elem::widen(x, true));
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (c > 0)
+#pragma unroll
+            for (int db = 0; db < 4; ++db) v0[db] = value(c, db);
+#pragma unroll
+          for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v0[db], p[c], o[db]);
+          if (careful)
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v0[db][j] = drop_nonfinite<Elem>(v0[db][j]);
+#pragma unroll
+          for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v0[db], rest[c], o[db]);
+        }
+      } else {
+        u32x4 v1[4];
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          v1[db] = value(1, db);
+          o[db] = Elem::mma(v0[db], p[0], o[db]);
+        }
+#pragma unroll
+        for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v1[db], p[1], o[db]);
       }
-#pragma unroll
-      for (int db = 0; db < 4; ++db) o[db] = Elem::mma(v1[db], p[1], o[db]);
     }
     // The next tile has landed, and behind the barrier this one's place is free.
     if (i + 2 < tiles) landed<2 * kLoads>();
@@ -565,12 +599,20 @@ __global__ __launch_bounds__(kWaves * 64, 3) void chunk_kernel(ChunkArgs a) {
     large = true;
 #pragma unroll
     for (int db = 0; db < 4; ++db) o[db] = f32x16{};
-    for (int i = 0; i < tiles; i += kBuffers) {  // LDS places known at compile time
-      step(i, 0);
-      if (i + 1 >= tiles) break;
-      step(i + 1, 1);
-      if (i + 2 >= tiles) break;
-      step(i + 2, 2);
+    auto steps = [&](auto two) __attribute__((always_inline)) {
+      for (int i = 0; i < tiles; i += kBuffers) {  // LDS places known at compile time
+        step(two, i, 0);
+        if (i + 1 >= tiles) break;
+        step(two, i + 1, 1);
+        if (i + 2 >= tiles) break;
+        step(two, i + 2, 2);
+      }
+    };
+    if constexpr (std::is_same_v<Elem, BFloat>) {
+      if (two_terms) steps(std::true_type{});
+      else steps(std::false_type{});
+    } else {
+      steps(std::false_type{});
     }
     if (careful) {
       const int half = fresh_lane() >> 5;

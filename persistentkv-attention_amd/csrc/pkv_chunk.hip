@@ -28,7 +28,7 @@
 // over 8192: 512 parts 84 us, 768 88, 256 117), but rows of one wave at most (decoding rows,
 // guessed tokens) cost little and are counted apart.  Large and small rows take turns, two to one,
 // so that the ones' products run next to the others' reads (28 single tokens and 4 pieces of 512
-// over up to 8192: 238 us; one after the other 280, in equal turns 270).
+// over up to 8192, weights in one term: 238 us; one after the other 280, in equal turns 270).
 //
 // P enters the product with V in the activation type.  Large rows, which wait for products, round it
 // once, as the prompt attention does: bf16 outputs are 2.3e-3 from the exact ones (relative 2-norm;
@@ -37,11 +37,10 @@
 // of 1.66e-3) for 3 % (64 single tokens of 128-65536 keys, 32 / 4 heads: 331 us, 323 with one term; the
 // 28 single tokens next to four pieces of 512: 249 for 239).
 //
-// Measured (bf16, 32 / 8 heads, pages of 16): 2048 tokens over 32768 1.01 ms, 1.05 PFLOP/s, the matrix
-// units busy half the cycles with two workgroups a CU; the step of a workgroup, 0.48 us a CU, is the same
-// with three.  64 single tokens of 128-65536 keys (32 / 4 heads) 4.9 TB/s, the rate of a copy.  5 tokens
-// over 2011: 11.4 us, 7.8 of it the first kernel (four dependent reads before the first product), 3.7
-// the join.
+// Measured (bf16, 32 / 8 heads, pages of 16): 2048 tokens over 32768 1.00 ms, 1.06 PFLOP/s, the matrix
+// units busy 57 % of the cycles; a CU's step takes 0.5 us with two workgroups and with three.  64 single
+// tokens of 128-65536 keys (32 / 4 heads) 4.8 TB/s, where a copy reaches 5.1.  5 tokens over 2011: 11.3
+// us, 7.7 of it the first kernel (four dependent reads before the first product), 3.6 the join.
 
 #include <hip/hip_runtime.h>
 #include <float.h>
@@ -142,8 +141,9 @@ struct Cut {
 // C for the sum of blocks times tiles of a class and one KV head: a little more than W / P, so that the
 // roundings of the sum (less than 2^-17 of it) never make more parts than the grid and the workspace hold.
 // Large rows whose parts would be longer than kLongPart tiles have up to kFiner times as many: the GPU
-// deals them out as it goes, and rows of different lengths end together (12 rows of 1073 tokens over up
-// to 22304, 6 / 2 heads: 518 us, 610 with P parts; 8 of 1024 over 4096-32768 2.39 ms and 2.46).
+// deals them out as it goes, and rows end together (12 rows of 1073 tokens over up to 22304, 6 / 2 heads:
+// 518 us, 624 with P parts; 8 of 1024 over 4096-32768 2.31 ms and 2.41; of equal lengths 4 of 1024 over
+// 16384 1.03 and 1.09, 2048 over 32768 1.005 and 1.014, its 136 MB of states among them).
 constexpr int kLongPart = 192, kFiner = 4;
 __device__ inline int part_tiles(float c) { return max(kMinTiles, (int)fminf(ceilf(c), 1e9f)); }
 __device__ inline Cut cut_of(const ChunkArgs& a, float large, float small) {

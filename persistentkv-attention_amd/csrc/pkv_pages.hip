@@ -12,8 +12,8 @@
 //
 // What bounds them is latency, a launch and a few dependent reads each, but for the copies, which are
 // bound by memory.  8 forks: 3.7 us and 2.8 for a layer's copies; 64 of 700 pages each 6.8 (45,000
-// counts raised, 16 on each) and 4.5; 3 rows of a pool of 61,000 pages freed: 3.1, 2.7 and 3.5 us; 90
-// rows of 196,000 pages: 10.8, 3.9 and 4.0.  A pool of 31,000 pages compacted: 13 us, and 199 for the
+// counts raised, 16 on each) and 4.5; 3 rows of a pool of 61,000 pages freed: 3.2, 2.6 and 3.5 us; 90
+// rows of 196,000 pages: 10.8, 2.6 and 4.1.  A pool of 31,000 pages compacted: 13 us, and 198 for the
 // copies of a layer (1.0 GB, 5.0 TB/s).
 
 #include <hip/hip_runtime.h>
